@@ -564,6 +564,102 @@ int b200_ep_combine(const void* rows, const int32_t* row_of, int dtype, int hidd
                     int world_size, int64_t flag_base_words, int* status, unsigned int* scratch_counter, void* stream);
 
 /*
+ * Head rows: num_tokens x num_heads rows of head_dim neighbouring elements; element (t, h, d) is at
+ * ptr[t * stride_token + h * stride_head + d].  ptr is 16-byte aligned, both strides are non-negative multiples of 8.
+ */
+typedef struct {
+  const void* ptr;
+  int64_t stride_token, stride_head;
+} b200_heads;
+
+/*
+ * A paged key/value cache in e4m3: slot s is place s % page_size of page s / page_size.  The code of element d of head h is
+ * at k[page * k_stride[0] + place * k_stride[1] + h * k_stride[2] + d] (strides in elements, non-negative multiples of 16;
+ * k and v 16-byte aligned), its head's fp32 scale at k_scale[page * k_scale_stride[0] + ...].  num_pages * page_size < 2^31.
+ */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t k_stride[3], v_stride[3], k_scale_stride[3], v_scale_stride[3];
+  int64_t num_pages, page_size;
+} b200_kv_cache;
+
+/*
+ * RMSNorm of each query and key head, then the rotary position embedding, in one pass; all arithmetic in fp32, rounded once:
+ *   y = x * rsqrt(mean(x^2) + norm_eps) * weight            (weight [head_dim] in the data's type; NULL: no norm)
+ *   (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)            for rotary_dim / 2 pairs, the other elements stay
+ * is_neox: pair i is (i, i + rotary_dim / 2), otherwise (2 i, 2 i + 1).  c and s are elements i and rotary_dim / 2 + i of
+ * row positions[t] of cos_sin [max_position, rotary_dim] (NULL: no rotation).  positions are int32, or int64 with
+ * positions_i64.  A token whose position is negative is padding: nothing of it is read or written.  One whose position
+ * is >= max_position becomes NaN.  q_out / k_out may be q / k themselves.  dtype bf16 or fp16; head_dim a multiple of 16 up
+ * to 256, rotary_dim a multiple of 16.  num_q_heads or num_kv_heads may be 0.
+ * Stands in for RMSNorm on the heads (python/sglang/srt/layers/layernorm.py) followed by
+ * apply_rope_with_cos_sin_cache_inplace (sgl-kernel/csrc/elementwise/rope.cu).
+ */
+int b200_qk_norm_rope(const b200_heads* q, const b200_heads* k, const b200_heads* q_out, const b200_heads* k_out, int dtype,
+                      const void* positions, int positions_i64, const float* cos_sin, int64_t max_position, int rotary_dim,
+                      int is_neox, const void* q_weight, const void* k_weight, float norm_eps, int64_t num_tokens,
+                      int num_q_heads, int num_kv_heads, int head_dim, void* stream);
+
+/*
+ * Keys and values of num_tokens tokens quantised into the cache: scale = max(1e-10, max|y|) / 448 for each token and head,
+ * code = e4m3(y / scale) -- bit for bit what b200_per_token_group_quant_fp8 with group = head_dim makes of them.  Token t goes
+ * to slot slots[t] (int32, or int64 with slots_i64); a slot outside [0, num_pages * page_size) is skipped.  Tokens of one call
+ * that share a slot leave it undefined.  Every other slot stays as it was.
+ */
+int b200_store_kv_fp8(const b200_heads* k, const b200_heads* v, int dtype, const b200_kv_cache* cache, const void* slots,
+                      int slots_i64, int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
+
+/*
+ * b200_qk_norm_rope and b200_store_kv_fp8 of the resulting keys (which are not rounded in between) and of v, in one pass.
+ * k_out may be NULL: the keys then go to the cache only.
+ */
+int b200_qk_norm_rope_store_kv_fp8(const b200_heads* q, const b200_heads* k, const b200_heads* v, const b200_heads* q_out,
+                                   const b200_heads* k_out, int dtype, const void* positions, int positions_i64,
+                                   const float* cos_sin, int64_t max_position, int rotary_dim, int is_neox,
+                                   const void* q_weight, const void* k_weight, float norm_eps, const b200_kv_cache* cache,
+                                   const void* slots, int slots_i64, int64_t num_tokens, int num_q_heads, int num_kv_heads,
+                                   int head_dim, void* stream);
+
+/*
+ * The cache read back: k_out and v_out (dtype bf16 or fp16) get code * scale for the tokens of `batch` sequences, packed.
+ * Rows [indptr[b], indptr[b + 1]) are the tokens starts[b], starts[b] + 1, ... of sequence b (starts NULL: from 0), token i
+ * lying at place i % page_size of page page_table[b * page_table_stride + i / page_size].  indptr [batch + 1] does not
+ * decrease; rows of the `num_tokens` outside [indptr[0], indptr[batch]) are left as they were.  A row whose page is missing
+ * (outside the table, or no page of the cache) becomes NaN.
+ */
+int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_table, int64_t page_table_stride,
+                     int64_t page_table_cols, const int32_t* indptr, const int32_t* starts, int64_t batch,
+                     const b200_heads* k_out, const b200_heads* v_out, int dtype, int64_t num_tokens, int num_kv_heads,
+                     int head_dim, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   out[t, n] = base[t, n] + scalings[a] * sum_r h[t, s, r] B[a, n, r],   h[t, s, r] = sum_k x[t, k] A[a, s * R + r, k]
+ * for token t with adapter a = token_adapters[t], r < ranks[a], and s the slice of column n.  A [L, num_slices * R, K] and
+ * B [L, N, R] are dense and hold every adapter in R = the largest rank; what lies behind an adapter's rank is not used.
+ * A token whose adapter is outside [0, L), or has rank <= 0, has none.
+ * Stands in for the sgemm_lora_a / sgemm_lora_b / qkv_lora_b / gate_up_lora_b kernels of python/sglang/srt/lora/triton_ops.
+ *
+ * b200_lora_plan groups the tokens by adapter into `plan` (16-byte aligned device memory of b200_lora_plan_bytes); shrink and
+ * expand take it, with the same num_tokens and L.  It has to be made again when ids or ranks change.
+ * b200_lora_shrink writes h [num_tokens, num_slices * R] in x's type (fp32 sums, rounded once; zero behind a rank, and for
+ * tokens without an adapter).  b200_lora_expand: base NULL counts as zeros; out may be base; tokens without an adapter get
+ * base.  slice_sizes (host) adds up to N, each a multiple of 8.  dtype (of x, A, h, B, base, out) bf16 or fp16; K and R
+ * multiples of 8, R <= 256, at most 8 slices, 1024 adapters and 1000000 tokens; leading dimensions multiples of 8, pointers
+ * 16-byte aligned.
+ */
+size_t b200_lora_plan_bytes(int64_t num_tokens, int num_adapters);
+int b200_lora_plan(const int32_t* token_adapters, int64_t num_tokens, const int32_t* ranks, int num_adapters, void* plan,
+                   size_t plan_bytes, void* stream);
+int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int dtype, const void* plan, size_t plan_bytes,
+                     int64_t num_tokens, int num_adapters, int64_t K, int R, int num_slices, void* h, int64_t h_ld,
+                     void* stream);
+int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes,
+                     const float* scalings, int64_t num_tokens, int num_adapters, int R, const int64_t* slice_sizes,
+                     int num_slices, const void* base, int64_t base_ld, void* out, int64_t out_ld, void* stream);
+
+/*
  * Device-side waits in the GEMM kernels are bounded (about a second of SM clocks).  A wait that gives up
  * makes its kernel drain and exit, and records a code that is STICKY for the device, like a CUDA error:
  *   - every later GEMM entry point on that device returns B200_ERR_DEVICE_TIMEOUT without launching

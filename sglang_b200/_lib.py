@@ -16,6 +16,21 @@ DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 _lib = None
 
 
+class Heads(ctypes.Structure):
+    """b200_heads"""
+    _fields_ = [("ptr", c_void_p), ("stride_token", c_int64), ("stride_head", c_int64)]
+
+
+class KVCache(ctypes.Structure):
+    """b200_kv_cache"""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("k_scale_stride", c_int64 * 3),
+                ("v_scale_stride", c_int64 * 3), ("num_pages", c_int64), ("page_size", c_int64)]
+
+
+_HEADS, _CACHE = ctypes.POINTER(Heads), ctypes.POINTER(KVCache)
+
+
 class B200Error(RuntimeError):
     """A C-ABI call returned a negative status."""
 
@@ -119,6 +134,20 @@ _SIGNATURES = {
     "b200_fp8_gate_up_silu_quant_pow2": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                                  c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64,
                                                  c_int64, c_int64, c_void_p]),
+    "b200_qk_norm_rope": (c_int, [_HEADS, _HEADS, _HEADS, _HEADS, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int,
+                                  c_void_p, c_void_p, c_float, c_int64, c_int, c_int, c_int, c_void_p]),
+    "b200_store_kv_fp8": (c_int, [_HEADS, _HEADS, c_int, _CACHE, c_void_p, c_int, c_int64, c_int, c_int, c_void_p]),
+    "b200_qk_norm_rope_store_kv_fp8": (c_int, [_HEADS, _HEADS, _HEADS, _HEADS, _HEADS, c_int, c_void_p, c_int, c_void_p, c_int64,
+                                               c_int, c_int, c_void_p, c_void_p, c_float, _CACHE, c_void_p, c_int, c_int64,
+                                               c_int, c_int, c_int, c_void_p]),
+    "b200_load_kv_fp8": (c_int, [_CACHE, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, _HEADS, _HEADS, c_int, c_int64,
+                                 c_int, c_int, c_void_p]),
+    "b200_lora_plan_bytes": (ctypes.c_size_t, [c_int64, c_int]),
+    "b200_lora_plan": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, ctypes.c_size_t, c_void_p]),
+    "b200_lora_shrink": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, ctypes.c_size_t, c_int64, c_int, c_int64, c_int,
+                                 c_int, c_void_p, c_int64, c_void_p]),
+    "b200_lora_expand": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, ctypes.c_size_t, c_void_p, c_int64, c_int, c_int,
+                                 ctypes.POINTER(c_int64), c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
 }
 
 

@@ -1,0 +1,207 @@
+"""CPU: what the adapter, head-norm and cache functions refuse, and the C ABI's codes for the same; nothing is launched."""
+import ctypes
+
+import pytest
+import torch
+
+BF, F16, F8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def _heads_call(**change):
+    from sglang_b200.layers.rotary_embedding import qk_norm_rope
+    a = dict(q=torch.zeros(3, 4, 64, dtype=BF), k=torch.zeros(3, 2, 64, dtype=BF), positions=torch.zeros(3, dtype=torch.int64),
+             cos_sin_cache=torch.zeros(10, 64), q_weight=torch.ones(64, dtype=BF), k_weight=torch.ones(64, dtype=BF))
+    a.update(change)
+    return qk_norm_rope(**a)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({}, "CUDA"),
+    (dict(q=torch.zeros(3, 4, 64)), "bfloat16 or float16"),
+    (dict(q=torch.zeros(3, 4, 64, dtype=F16)), "same type"),
+    (dict(q=torch.zeros(3, 256, dtype=BF)), "q must be"),
+    (dict(q=torch.zeros(2, 4, 64, dtype=BF)), "same number of tokens"),
+    (dict(k=torch.zeros(3, 2, 40, dtype=BF)), "multiple of 16"),
+    (dict(k=torch.zeros(3, 2, 272, dtype=BF)), "at most 256"),
+    (dict(k=torch.zeros(3, 64, 2, dtype=BF).transpose(1, 2)), "last dimension"),
+    (dict(k=torch.zeros(3, 2, 68, dtype=BF)[..., :64]), "multiples of 8"),
+    (dict(k=torch.zeros(3 * 128 + 4, dtype=BF)[4:].view(3, 2, 64)), "aligned"),
+    (dict(positions=None), "positions"),
+    (dict(positions=torch.zeros(3)), "int32 or int64"),
+    (dict(positions=torch.zeros(4, dtype=torch.int32)), "positions must have shape"),
+    (dict(cos_sin_cache=torch.zeros(10, 64, dtype=BF)), "float32"),
+    (dict(cos_sin_cache=torch.zeros(10, 24)), "rotary_dim"),
+    (dict(cos_sin_cache=torch.zeros(10, 80)), "rotary_dim"),
+    (dict(q_weight=torch.ones(32, dtype=BF)), "q_weight must have shape"),
+    (dict(k_weight=torch.ones(64)), "k_weight must have the type"),
+    (dict(q_out=torch.zeros(3, 4, 64, dtype=F16)), "q_out"),
+    (dict(k_out=torch.zeros(3, 1, 64, dtype=BF).expand(3, 2, 64)), "expanded"),
+    (dict(q="q"), "must be a tensor"),
+])
+def test_head_rows_refusals(change, message):
+    with pytest.raises(RuntimeError, match=message):
+        _heads_call(**change)
+
+
+def _store_call(**change):
+    from sglang_b200.layers.quantization.kv_cache import store_kv_fp8
+    a = dict(k=torch.zeros(3, 2, 64, dtype=BF), v=torch.zeros(3, 2, 64, dtype=BF), k_cache=torch.zeros(5, 4, 2, 64).to(F8),
+             v_cache=torch.zeros(5, 4, 2, 64).to(F8), k_scale=torch.zeros(5, 4, 2), v_scale=torch.zeros(5, 4, 2),
+             slots=torch.zeros(3, dtype=torch.int32))
+    a.update(change)
+    return store_kv_fp8(**a)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({}, "CUDA"),
+    (dict(v=torch.zeros(3, 1, 64, dtype=BF)), "v must have shape"),
+    (dict(v=torch.zeros(3, 2, 64, dtype=F16)), "same type"),
+    (dict(v=None), "v must be given"),
+    (dict(k_cache=torch.zeros(5, 4, 2, 64)), "float8_e4m3fn"),
+    (dict(k_cache=torch.zeros(20, 2, 64).to(F8)), "k_cache must be"),
+    (dict(v_cache=torch.zeros(5, 4, 2, 32).to(F8)), "v_cache must have shape"),
+    (dict(k_scale=torch.zeros(5, 4, 2, dtype=BF)), "float32"),
+    (dict(v_scale=torch.zeros(5, 4, 1)), "v_scale must have shape"),
+    (dict(v_scale=torch.zeros(5, 4, 1).expand(5, 4, 2)), "expanded"),
+    (dict(k=torch.zeros(3, 4, 64, dtype=BF), v=torch.zeros(3, 4, 64, dtype=BF)), "heads of k"),
+    (dict(slots=torch.zeros(2, dtype=torch.int32)), "slots must have shape"),
+    (dict(slots=torch.zeros(3)), "int32 or int64"),
+    (dict(slots=torch.zeros(6, dtype=torch.int32)[::2]), "contiguous"),
+])
+def test_store_refusals(change, message):
+    with pytest.raises(RuntimeError, match=message):
+        _store_call(**change)
+
+
+def _load_call(**change):
+    from sglang_b200.layers.quantization.kv_cache import load_kv_fp8
+    a = dict(k_cache=torch.zeros(5, 4, 2, 64).to(F8), v_cache=torch.zeros(5, 4, 2, 64).to(F8), k_scale=torch.zeros(5, 4, 2),
+             v_scale=torch.zeros(5, 4, 2), page_table=torch.zeros(2, 3, dtype=torch.int32),
+             kv_indptr=torch.zeros(3, dtype=torch.int32), num_tokens=7)
+    a.update(change)
+    return load_kv_fp8(**a)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({}, "CUDA"),
+    (dict(num_tokens=-1), "negative"),
+    (dict(page_table=torch.zeros(2, 3, dtype=torch.int64)), "int32"),
+    (dict(page_table=torch.zeros(2, 6, dtype=torch.int32)[:, ::2]), "last dimension"),
+    (dict(kv_indptr=torch.zeros(2, dtype=torch.int32)), "kv_indptr must have shape"),
+    (dict(kv_indptr=torch.zeros(3, dtype=torch.int64)), "int32"),
+    (dict(kv_start=torch.zeros(3, dtype=torch.int32)), "kv_start must have shape"),
+    (dict(out_dtype=torch.float32), "out_dtype"),
+    (dict(k_out=torch.zeros(6, 2, 64, dtype=BF)), "k_out must have shape"),
+    (dict(v_out=torch.zeros(7, 2, 64, dtype=F16)), "out_dtype"),
+    (dict(k_cache=torch.zeros(5, 4, 2, 40).to(F8), v_cache=torch.zeros(5, 4, 2, 40).to(F8)), "multiple"),
+])
+def test_load_refusals(change, message):
+    with pytest.raises(RuntimeError, match=message):
+        _load_call(**change)
+
+
+class _Batch:
+    """What LoRABatch holds, without its launch."""
+
+    def __init__(self, T, L):
+        from sglang_b200 import _lib
+        self.plan = torch.zeros(_lib.lib().b200_lora_plan_bytes(T, L), dtype=torch.uint8)
+        self.num_adapters, self.scalings = L, torch.ones(L)
+
+
+def _lora_call(**change):
+    from sglang_b200.layers.lora import apply_lora
+    a = dict(base_output=torch.zeros(5, 96, dtype=BF), x=torch.zeros(5, 64, dtype=BF), lora_a=torch.zeros(3, 32, 64, dtype=BF),
+             lora_b=torch.zeros(3, 96, 16, dtype=BF), batch=_Batch(5, 3), output_sizes=[64, 32])
+    a.update(change)
+    return apply_lora(**a)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({}, "CUDA"),
+    (dict(x=torch.zeros(5, 64)), "type of x|bfloat16"),
+    (dict(x=torch.zeros(1, 5, 64, dtype=BF)), "x must be"),
+    (dict(x=torch.zeros(5, 72, dtype=BF)), "lora_a must be"),
+    (dict(x=torch.zeros(5, 68, dtype=BF)[:, :64]), "multiples of 8"),
+    (dict(lora_a=torch.zeros(3, 16, 64, dtype=BF)), "lora_a must be"),
+    (dict(lora_a=torch.zeros(2, 32, 64, dtype=BF)), "adapters of the batch"),
+    (dict(lora_a=torch.zeros(3, 32, 128, dtype=BF)[..., :64]), "contiguous"),
+    (dict(lora_b=torch.zeros(3, 96, 16, dtype=F16)), "type of x"),
+    (dict(lora_a=torch.zeros(3, 24, 64, dtype=BF), lora_b=torch.zeros(3, 96, 12, dtype=BF)), "R must be"),
+    (dict(lora_a=torch.zeros(3, 528, 64, dtype=BF), lora_b=torch.zeros(3, 96, 264, dtype=BF)), "R must be"),
+    (dict(output_sizes=[64, 24]), "add up"),
+    (dict(output_sizes=[60, 36]), "multiples of 8"),
+    (dict(output_sizes=[8] * 9), "slices"),
+    (dict(base_output=torch.zeros(5, 88, dtype=BF)), "base_output must have shape"),
+    (dict(base_output=torch.zeros(1, 96, dtype=BF).expand(5, 96)), "overlap"),
+    (dict(out=torch.zeros(5, 96, dtype=F16)), "out must be"),
+    (dict(batch=_Batch(6, 3)), "another number of tokens"),
+])
+def test_lora_refusals(change, message):
+    with pytest.raises(RuntimeError, match=message):
+        _lora_call(**change)
+
+
+@pytest.mark.parametrize("ids,ranks,message", [
+    (torch.zeros(4, dtype=torch.int64), torch.zeros(2, dtype=torch.int32), "token_adapters"),
+    (torch.zeros(4, dtype=torch.int32), torch.zeros(2), "lora_ranks"),
+    (torch.zeros(4, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), "1024 adapters"),
+    (torch.zeros(4, dtype=torch.int32), torch.zeros(1025, dtype=torch.int32), "1024 adapters"),
+    (torch.zeros(1, dtype=torch.int32).expand(1000001), torch.zeros(2, dtype=torch.int32), "contiguous"),
+    (torch.zeros(4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), "CUDA"),
+])
+def test_lora_batch_refusals(ids, ranks, message):
+    from sglang_b200.layers.lora import LoRABatch
+    with pytest.raises(RuntimeError, match=message):
+        LoRABatch(ids, ranks, torch.ones(ranks.shape[0]))
+
+
+def test_c_abi_codes():
+    from sglang_b200 import _lib
+    L, P = _lib.lib(), ctypes.c_void_p
+    one, ref = P(16), ctypes.byref
+    rows = _lib.Heads(16, 512, 64)
+    cache = _lib.KVCache(16, 16, 16, 16, (512, 128, 64), (512, 128, 64), (8, 2, 1), (8, 2, 1), 5, 4)
+
+    def nr(q=rows, k=rows, dt=2, pos=one, cs=one, rot=64, T=3, D=64, eps=1e-6):
+        return L.b200_qk_norm_rope(ref(q), ref(k), ref(q), ref(k), dt, pos, 0, cs, 10, rot, 1, None, None, eps, T, 4, 2, D, None)
+    assert nr(T=0) == 0
+    assert nr(T=-1) == -3 and nr(D=40) == -3 and nr(rot=24) == -3 and nr(rot=80) == -3
+    assert nr(D=272, rot=16) == -9 and nr(dt=0) == -2 and nr(pos=None) == -1
+    assert nr(q=_lib.Heads(None, 512, 64)) == -1 and nr(q=_lib.Heads(8, 512, 64)) == -5 and nr(k=_lib.Heads(16, 516, 64)) == -5
+    assert nr(q=_lib.Heads(16, -512, 64)) == -4 and nr(cs=P(8)) == -5
+
+    def st(c=cache, v=ref(rows), slots=one, T=3):
+        return L.b200_store_kv_fp8(ref(rows), v, 2, ref(c) if c else None, slots, 0, T, 2, 64, None)
+
+    def changed(**kw):
+        c = _lib.KVCache.from_buffer_copy(cache)
+        for name, value in kw.items():
+            setattr(c, name, value)
+        return c
+    assert st(c=None) == -1 and st(T=0) == 0 and st(v=None) == -1 and st(slots=None) == -1
+    assert st(changed(page_size=0)) == -3 and st(changed(num_pages=1 << 29)) == -9 and st(changed(k=None)) == -1
+    assert st(changed(v=8)) == -5 and st(changed(k_stride=(512, 128, 72))) == -5 and st(changed(v_scale_stride=(8, -2, 1))) == -4
+
+    def ld(c=cache, table=one, T=7, batch=2, D=64, dt=2):
+        return L.b200_load_kv_fp8(ref(c), table, 3, 3, one, None, batch, ref(rows), ref(rows), dt, T, 2, D, None)
+    assert ld(T=0) == 0 and ld(batch=0) == 0 and ld(T=-1) == -3 and ld(D=24) == -3 and ld(dt=0) == -2 and ld(table=None) == -1
+    assert ld(changed(num_pages=-1)) == -3
+
+    plan = L.b200_lora_plan_bytes(5, 3)
+    assert plan >= 16 + 4 * 5 and L.b200_lora_plan_bytes(-1, 3) == 0
+    assert L.b200_lora_plan(one, 5, one, 0, one, plan, None) == -3
+    assert L.b200_lora_plan(one, 5, one, 2000, one, plan, None) == -9
+    assert L.b200_lora_plan(one, 5, one, 3, one, plan - 1, None) == -3
+    assert L.b200_lora_plan(None, 5, one, 3, one, plan, None) == -1
+
+    def sh(x=one, ld_=64, dt=2, T=5, K=64, R=16, S=2, hld=32, nbytes=plan):
+        return L.b200_lora_shrink(x, ld_, one, dt, one, nbytes, T, 3, K, R, S, one, hld, None)
+    assert sh(T=0) == 0 and sh(K=60) == -3 and sh(R=12) == -3 and sh(R=264) == -9 and sh(S=0) == -3 and sh(S=9, hld=144) == -9
+    assert sh(dt=0) == -2 and sh(ld_=56) == -4 and sh(hld=24) == -4 and sh(x=None) == -1 and sh(x=P(8)) == -5 and sh(nbytes=0) == -3
+
+    def ex(sizes=(64, 32), h=one, hld=32, old=96, bld=96, T=5):
+        return L.b200_lora_expand(h, hld, one, 2, one, plan, one, T, 3, 16, (ctypes.c_int64 * len(sizes))(*sizes), len(sizes), one, bld,
+                                  one, old, None)
+    assert ex(T=0) == 0 and ex(sizes=(64, 36)) == -3 and ex(old=88) == -4 and ex(bld=88) == -4 and ex(hld=24) == -4
+    assert ex(h=None) == -1 and ex(h=P(8)) == -5 and ex(sizes=(8,) * 9) == -9
