@@ -2,11 +2,11 @@
 // position embedding, keys and values quantised into a paged cache, and the cache read back.  All of it moves data: the
 // floor is the bytes read and written once, at the memory's rate.
 //
-// One head of one token ("row", D elements) belongs to a group of G lanes, G the power of two from D / 8 up, each lane
-// holding eight consecutive elements (one 16-byte load).  Everything that a row needs is a shuffle inside its group: the
-// sum of squares, the partner of a rotated pair, the largest magnitude.  A warp takes U x (32 / G) neighbouring rows of one
-// token, so its cosines and sines are loaded once for all of them, and all rows' loads are in flight before the first is
-// used.  All arithmetic is in 32 bits; a query is rounded once, when it is stored, and a key once, to e4m3.
+// One head of one token ("row", D elements) belongs to a group of G lanes, G the power of two from D / 16 up, each lane
+// holding sixteen elements in two 16-byte loads.  What a row needs beyond its lane is a shuffle inside its group: the sum of
+// squares and the largest magnitude.  A warp keeps to one token and to queries, keys or values: weights, cosines and sines
+// stay in registers while it walks over its rows, 32 / G at a time, the next ones on their way into shared memory.  All arithmetic is in 32 bits; a
+// query is rounded once, when it is stored, and a key once, to e4m3.
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w
 //   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)     neox: b = a + rot / 2; otherwise neighbours a = 2i, b = 2i + 1
@@ -31,7 +31,11 @@ struct HeadRowsParams {
   int64_t kc_s[3], vc_s[3], ks_s[3], vs_s[3];   // page, slot inside the page, head
   int64_t T, max_position;
   uint32_t num_slots, page_size;
-  int Hq, Hkv, Hv, D, rot, chunks;              // Hv: Hkv with a cache, else 0
+  int Hq, Hkv, Hv, D, rot;                      // Hv: Hkv with a cache, else 0
+  uint32_t chunks_magic;                        // 2^32 / chunks, rounded up
+  int page_shift;                               // page_size = 1 << page_shift, or -1
+  int chunks, chunks_q, chunks_kv;              // warps a token; of them for queries, and for keys (as many for values)
+  int heads_q, heads_kv;                        // of one warp
   int pos_i64, slots_i64;
   float eps;
 };
@@ -48,212 +52,365 @@ __device__ __forceinline__ uint32_t from_f2(float a, float b, __half*) {
   __half2 t = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&t);
 }
+// Two fp32 numbers in one 64-bit register pair: one instruction does both.
+struct f2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ f2 make_f2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f2 both(float a) { return make_f2(a, a); }
+__device__ __forceinline__ float2 split(f2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ f2 mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& v, f2* f) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 p = to_f2(w[i], static_cast<T*>(nullptr));
-    f[2 * i] = p.x;
-    f[2 * i + 1] = p.y;
+    f[i] = make_f2(p.x, p.y);
   }
 }
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  T* t = nullptr;
-  return make_uint4(from_f2(f[0], f[1], t), from_f2(f[2], f[3], t), from_f2(f[4], f[5], t), from_f2(f[6], f[7], t));
+__device__ __forceinline__ uint4 pack8(const f2* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = split(f[i]);
+    w[i] = from_f2(p.x, p.y, static_cast<T*>(nullptr));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ int64_t load_index(const void* p, int i64, int64_t i) {
   return i64 ? __ldg(static_cast<const long long*>(p) + i) : static_cast<int64_t>(__ldg(static_cast<const int*>(p) + i));
 }
 
-// The eight codes of one lane.  y / scale correctly rounded from the correctly rounded reciprocal (Markstein: exact for
-// every scale whose significand is not all ones); rows with such a scale, a non-finite one or a NaN among the lane's
-// elements take the literal fminf(fmaxf(y / scale, -448), 448), in which a NaN becomes -448.
-__device__ __forceinline__ uint2 quantise8(const float (&y)[8], float scale) {
+// amax / 448, correctly rounded: from the correctly rounded 1 / 448 and the exact remainder (Markstein).
+__device__ __forceinline__ float scale_of(float amax) {
+  const float r = 1.f / 448.f, q0 = __fmul_rn(amax, r);
+  const float q = fmaf(fmaf(-q0, 448.f, amax), r, q0);
+  return amax < __uint_as_float(0x7f800000u) ? q : amax;
+}
+
+// The sixteen codes of one lane.  y / scale correctly rounded from the correctly rounded reciprocal in the same way, which holds
+// for every scale whose significand is not all ones; with such a scale, a non-finite one or a NaN among the lane's elements the
+// quotients are taken literally.  Computed as -(y / scale), q0 = y (-r), q0 + (y + q0 scale)(-r), and the codes' signs flipped:
+// in this form a zero keeps its sign.
+__device__ __forceinline__ uint4 quantise16(const f2 (&y)[8], float scale) {
   const uint32_t bits = __float_as_uint(scale);
   bool literal = (bits & 0x007fffffu) == 0x007fffffu || (bits & 0x7f800000u) == 0x7f800000u;
-  const float r = __frcp_rn(scale);
-  float t[8];
+  const f2 nr = both(-__frcp_rn(scale)), s = both(scale);
+  uint32_t w[4], nan = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q0 = __fmul_rn(y[i], r);
-    const float rem = fmaf(q0, scale, -y[i]);
-    t[i] = fmaf(-rem, r, q0);
-    literal |= !(t[i] == t[i]);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t half[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f2 q0 = mul(y[2 * i + j], nr);
+      const float2 t = split(fma(fma(q0, s, y[2 * i + j]), nr, q0));
+      half[j] = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
+    }
+    w[i] = (half[0] | (half[1] << 16)) ^ 0x80808080u;
+    nan |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;               // bit 7 of a byte: its code was 0x7f or 0xff
   }
-  if (literal) {
+  literal |= (nan & 0x80808080u) != 0;
+  if (literal) {                                             // fminf(fmaxf(y / scale, -448), 448): a NaN becomes -448
+    float t[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = fminf(fmaxf(__fdiv_rn(y[i], scale), -448.f), 448.f);
+    for (int i = 0; i < 8; ++i) t[2 * i] = split(y[i]).x, t[2 * i + 1] = split(y[i]).y;
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) t[i] = fminf(fmaxf(__fdiv_rn(t[i], scale), -448.f), 448.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * i], t[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * i + 2], t[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+      w[i] = lo | (hi << 16);
+    }
   }
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __nv_cvt_float2_to_fp8x2(make_float2(t[2 * i], t[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// ROPE: 0 none, 1 neox, 2 neighbouring pairs.
-template <typename T, int G, int U, int ROPE>
-__global__ void __launch_bounds__(kThreads) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
-  pdl_start();
+constexpr int kStages = 4, kStageBytes = 32 * 32;            // row groups in flight for each warp
+
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// What differs between queries, keys and values, decided once for a warp.
+template <typename T>
+struct Rows {
+  const T* src;              // head 0 of the token
+  int64_t src_sh;
+  T* dst;                    // or nullptr
+  int64_t dst_sh;
+  const T* weight;           // or nullptr
+  uint8_t* codes;            // head 0 of the token's place in the cache
+  int64_t codes_sh;
+  float* scales;
+  int64_t scales_sh;
+  int first, last;           // the warp's heads
+  bool poisoned;
+};
+
+// ROPE: 0 none, 1 neox, 2 neighbouring pairs.  With neox pairs a lane of the rotated part holds elements 8l .. 8l + 7 and their
+// partners rot / 2 further on, so that a rotation stays inside the lane; otherwise elements 16l .. 16l + 15.
+// The weights are multiplied into the cosines and sines, once for all rows.
+template <typename T, int G, int ROPE, bool STORE, bool CODES>
+__device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lane, int D, int rot, float eps, const float* table_row) {
   constexpr int RPW = 32 / G;
-  const int lane = threadIdx.x & 31;
+  constexpr bool SPLIT = ROPE == 1;
   const int l = lane % G, sub = lane / G;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t tok = item / p.chunks;
-  if (tok >= p.T) return;
-  const int h0 = static_cast<int>(item - tok * p.chunks) * (RPW * U) + sub;
-  const int H = p.Hq + p.Hkv + p.Hv;
-  const bool in_row = l * 8 < p.D;
-
-  int64_t pos = 0;
-  if (ROPE != 0) {
-    pos = load_index(p.positions, p.pos_i64, tok);
-    if (pos < 0) return;                                    // padding: nothing of this token is read or written
-  }
-  int64_t slot = -1;
-  if (p.Hv != 0) slot = load_index(p.slots, p.slots_i64, tok);
-  const bool keep = slot >= 0 && slot < p.num_slots;
-
-  uint4 data[U];
+  const bool in_row = l * 16 < D;
+  const bool turned = ROPE != 0 && l * 16 < rot;
+  const int o0 = SPLIT && turned ? 8 * l : 16 * l, o1 = SPLIT && turned ? rot / 2 + 8 * l : 16 * l + 8;
+  const float inv_d = 1.f / static_cast<float>(D);
+  // ring: this lane's 32 bytes of each of the next kStages row groups; only the lane itself reads them
+  auto fetch = [&](int head, int stage) {
+    const int h = head + sub;
+    const bool live = h < r.last && in_row;
+    const T* row = r.src + (live ? h : 0) * r.src_sh;
+    const uint32_t to = ring + stage * kStageBytes;
+    sa::cp_async16(to, row + (live ? o0 : 0), live);
+    sa::cp_async16(to + kStageBytes / 2, row + (live ? o1 : 0), live);
+  };
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = h0 + u * RPW;
-    data[u] = make_uint4(0, 0, 0, 0);
-    const T* src = nullptr;
-    if (h < p.Hq) src = static_cast<const T*>(p.q) + tok * p.q_st + h * p.q_sh;
-    else if (h < p.Hq + p.Hkv) src = static_cast<const T*>(p.k) + tok * p.k_st + (h - p.Hq) * p.k_sh;
-    else if (h < H) src = static_cast<const T*>(p.v) + tok * p.v_st + (h - p.Hq - p.Hkv) * p.v_sh;
-    if (src != nullptr && in_row) data[u] = *reinterpret_cast<const uint4*>(src + l * 8);
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (r.first + i * RPW < r.last) fetch(r.first + i * RPW, i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // cosines and sines of this lane's elements
-  float c[8], s[8];
-  bool turned = false, second = false;
-  int partner = lane;
-  float poison = 1.f;
-  if (ROPE != 0) {
-    if (pos >= p.max_position) {                            // a position that the table lacks: NaN, not a read behind it
-      poison = __uint_as_float(0x7fc00000u);
-      pos = 0;
-    }
-    const float* row = p.cos_sin + pos * p.rot;
-    const int half = p.rot / 2;
-    turned = l * 8 < p.rot;
-    if (ROPE == 1) {
-      const int hl = half / 8;
-      second = l >= hl;
-      partner = turned ? lane + (second ? -hl : hl) : lane;
-      if (turned) {
-        const float4* cp = reinterpret_cast<const float4*>(row + (second ? l - hl : l) * 8);
-        const float4* sp = reinterpret_cast<const float4*>(row + half + (second ? l - hl : l) * 8);
-        const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-        c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-        s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+  f2 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = both(1.f);
+  if (r.weight != nullptr && in_row) {
+    unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o0)), w);
+    unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o1)), w + 4);
+  }
+  // the coefficients, two elements at a time: y' = y ca + partner sa (neox: pairs (e, e + 1) of the first run, then of the second;
+  // otherwise each pair is one that is rotated); elements that are not rotated keep w in ca
+  f2 ca[8], sa[8];
+  if (ROPE != 0 && turned) {
+    float cc[8] = {}, ss[8] = {};
+    if (!r.poisoned) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 c = __ldg(reinterpret_cast<const float4*>(table_row + 8 * l + 4 * i));
+        const float4 s = __ldg(reinterpret_cast<const float4*>(table_row + rot / 2 + 8 * l + 4 * i));
+        cc[4 * i] = c.x, cc[4 * i + 1] = c.y, cc[4 * i + 2] = c.z, cc[4 * i + 3] = c.w;
+        ss[4 * i] = s.x, ss[4 * i + 1] = s.y, ss[4 * i + 2] = s.z, ss[4 * i + 3] = s.w;
       }
-    } else if (turned) {
-      const float4 c0 = __ldg(reinterpret_cast<const float4*>(row + l * 4));
-      const float4 s0 = __ldg(reinterpret_cast<const float4*>(row + half + l * 4));
-      c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w;
-      s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w;
     }
-  }
-
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = h0 + u * RPW;
-    const bool is_q = h < p.Hq, is_k = !is_q && h < p.Hq + p.Hkv, is_v = !is_q && !is_k && h < H;
-    float y[8];
-    unpack8<T>(data[u], y);
-    const void* w = is_q ? p.q_w : is_k ? p.k_w : nullptr;
-    float sq = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sq = fmaf(y[i], y[i], sq);
-#pragma unroll
-    for (int off = G / 2; off >= 1; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-    if (w != nullptr && in_row) {
-      const float rinv = rsqrtf(sq / static_cast<float>(p.D) + p.eps);
-      float wf[8];
-      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w) + l * 8)), wf);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * rinv * wf[i];
-    }
-    if (ROPE == 1) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float o = __shfl_sync(0xffffffffu, y[i], partner);
-        if (turned && !is_v) y[i] = second ? fmaf(y[i], c[i], o * s[i]) : fmaf(y[i], c[i], -(o * s[i]));
+    for (int i = 0; i < 8; ++i) {
+      const float2 mine = split(w[i]);
+      if (ROPE == 1) {
+        const int j = 2 * (i % 4);
+        const float2 other = split(w[(i + 4) % 8]);
+        ca[i] = make_f2(cc[j] * mine.x, cc[j + 1] * mine.y);
+        sa[i] = i < 4 ? make_f2(-ss[j] * other.x, -ss[j + 1] * other.y) : make_f2(ss[j] * other.x, ss[j + 1] * other.y);
+      } else {
+        ca[i] = make_f2(cc[i] * mine.x, cc[i] * mine.y);
+        sa[i] = make_f2(-ss[i] * mine.y, ss[i] * mine.x);
       }
-    } else if (ROPE == 2) {
-      if (turned && !is_v) {
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ca[i] = w[i];
+  }
+  int stage = 0;
+#pragma unroll 1
+  for (int head = r.first; head < r.last; head += RPW) {
+    {
+      const int ahead = head + (kStages - 1) * RPW;
+      if (ahead < r.last) fetch(ahead, (stage + kStages - 1) % kStages);
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    }
+    const int h = head + sub;
+    const bool live = h < r.last && in_row;
+    f2 y[8];
+    {
+      const uint32_t from = ring + stage * kStageBytes;
+      unpack8<T>(ld_shared16(from), y);
+      unpack8<T>(ld_shared16(from + kStageBytes / 2), y + 4);
+      stage = (stage + 1) % kStages;
+    }
+    if (r.weight != nullptr) {
+      f2 sum = mul(y[0], y[0]);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) sum = fma(y[i], y[i], sum);
+      float sq = split(sum).x + split(sum).y;
+#pragma unroll
+      for (int off = G / 2; off >= 1; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
+      const f2 rinv = both(rsqrtf(fmaf(sq, inv_d, eps)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = mul(y[i], rinv);
+    }
+    if (ROPE != 0 && turned) {
+      if constexpr (ROPE == 1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float a = y[2 * i], b = y[2 * i + 1];
-          y[2 * i] = fmaf(a, c[i], -(b * s[i]));
-          y[2 * i + 1] = fmaf(b, c[i], a * s[i]);
+          const f2 a = y[i], b = y[i + 4];
+          y[i] = fma(a, ca[i], mul(b, sa[i]));
+          y[i + 4] = fma(b, ca[i + 4], mul(a, sa[i + 4]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 mine = split(y[i]);
+          y[i] = fma(y[i], ca[i], mul(make_f2(mine.y, mine.x), sa[i]));
         }
       }
-    }
-    if (ROPE != 0 && !is_v) {
+      if (r.poisoned) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= poison;
+        for (int i = 0; i < 8; ++i) y[i] = both(__uint_as_float(0x7fc00000u));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = mul(y[i], ca[i]);
+      if (ROPE != 0 && r.poisoned) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = both(__uint_as_float(0x7fc00000u));
+      }
     }
-    if (in_row) {
-      T* dst = nullptr;
-      if (is_q && p.q_out) dst = static_cast<T*>(p.q_out) + tok * p.qo_st + h * p.qo_sh;
-      if (is_k && p.k_out) dst = static_cast<T*>(p.k_out) + tok * p.ko_st + (h - p.Hq) * p.ko_sh;
-      if (dst != nullptr) *reinterpret_cast<uint4*>(dst + l * 8) = pack8<T>(y);
+    if (STORE && r.dst != nullptr && live) {
+      T* row = r.dst + h * r.dst_sh;
+      *reinterpret_cast<uint4*>(row + o0) = pack8<T>(y);
+      *reinterpret_cast<uint4*>(row + o1) = pack8<T>(y + 4);
     }
-    if (p.Hv != 0) {
+    if (CODES) {
       float amax = 1e-10f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[i]));
+      for (int i = 0; i < 8; ++i) {
+        const float2 v = split(y[i]);
+        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+      }
 #pragma unroll
       for (int off = G / 2; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-      if ((is_k || is_v) && keep && in_row) {
-        const float scale = __fdiv_rn(amax, 448.f);
-        const uint32_t page = static_cast<uint32_t>(slot) / p.page_size, at = static_cast<uint32_t>(slot) - page * p.page_size;
-        const int hh = is_k ? h - p.Hq : h - p.Hq - p.Hkv;
-        const int64_t* cs = is_k ? p.kc_s : p.vc_s;
-        const int64_t* ss = is_k ? p.ks_s : p.vs_s;
-        uint8_t* cache = (is_k ? p.kc : p.vc) + page * cs[0] + at * cs[1] + hh * cs[2];
-        *reinterpret_cast<uint2*>(cache + l * 8) = quantise8(y, scale);
-        if (l == 0) (is_k ? p.ks : p.vs)[page * ss[0] + at * ss[1] + hh * ss[2]] = is_k ? scale * poison : scale;
+      const float scale = scale_of(amax);
+      const uint4 q = quantise16(y, scale);
+      if (live) {
+        uint8_t* codes = r.codes + h * r.codes_sh;
+        if constexpr (SPLIT) {
+          *reinterpret_cast<uint2*>(codes + o0) = make_uint2(q.x, q.y);
+          *reinterpret_cast<uint2*>(codes + o1) = make_uint2(q.z, q.w);
+        } else {
+          *reinterpret_cast<uint4*>(codes + o0) = q;
+        }
+        if (l == 0) r.scales[h * r.scales_sh] = r.poisoned ? __uint_as_float(0x7fc00000u) : scale;
       }
     }
   }
 }
 
-template <typename T, int G, int U>
+template <typename T, int G, int ROPE>
+__global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
+  pdl_start();
+  __shared__ __align__(16) uint8_t rings[kThreads / 32 * kStages * kStageBytes];
+  const int lane = threadIdx.x & 31;
+  const uint32_t ring = smem_u32(rings) + (threadIdx.x >> 5) * (kStages * kStageBytes) + lane * 16;
+  const uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  uint32_t tok32 = p.chunks == 1 ? item : __umulhi(item, p.chunks_magic);      // item / chunks, or one more
+  if (tok32 * p.chunks > item) --tok32;
+  if (tok32 >= p.T) return;
+  const int64_t tok = tok32;
+  int chunk = static_cast<int>(item - tok32 * p.chunks);
+  Rows<T> r = {};
+  const float* table_row = nullptr;
+  if (ROPE != 0) {
+    const int64_t pos = load_index(p.positions, p.pos_i64, tok);
+    if (pos < 0) return;                                     // padding: nothing of this token is read or written
+    r.poisoned = pos >= p.max_position;                      // a position that the table lacks: NaN, not a read behind it
+    table_row = p.cos_sin + pos * p.rot;
+  }
+  if (chunk < p.chunks_q) {
+    r.first = chunk * p.heads_q, r.last = min(r.first + p.heads_q, p.Hq);
+    r.src = static_cast<const T*>(p.q) + tok * p.q_st, r.src_sh = p.q_sh;
+    r.dst = static_cast<T*>(p.q_out) + tok * p.qo_st, r.dst_sh = p.qo_sh;
+    r.weight = static_cast<const T*>(p.q_w);
+    do_rows<T, G, ROPE, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
+    return;
+  }
+  chunk -= p.chunks_q;
+  const bool keys = chunk < p.chunks_kv;
+  r.first = (keys ? chunk : chunk - p.chunks_kv) * p.heads_kv, r.last = min(r.first + p.heads_kv, p.Hkv);
+  if (keys) {
+    r.src = static_cast<const T*>(p.k) + tok * p.k_st, r.src_sh = p.k_sh;
+    if (p.k_out != nullptr) r.dst = static_cast<T*>(p.k_out) + tok * p.ko_st, r.dst_sh = p.ko_sh;
+    r.weight = static_cast<const T*>(p.k_w);
+  } else {
+    r.src = static_cast<const T*>(p.v) + tok * p.v_st, r.src_sh = p.v_sh;
+    r.poisoned = false;
+  }
+  bool keep = false;
+  if (p.Hv != 0) {
+    const int64_t slot = load_index(p.slots, p.slots_i64, tok);
+    keep = slot >= 0 && slot < p.num_slots;
+    const uint32_t page = p.page_shift >= 0 ? static_cast<uint32_t>(slot) >> p.page_shift : static_cast<uint32_t>(slot) / p.page_size;
+    const uint32_t place = static_cast<uint32_t>(slot) - page * p.page_size;
+    r.codes = keys ? p.kc + page * p.kc_s[0] + place * p.kc_s[1] : p.vc + page * p.vc_s[0] + place * p.vc_s[1];
+    r.codes_sh = keys ? p.kc_s[2] : p.vc_s[2];
+    r.scales = keys ? p.ks + page * p.ks_s[0] + place * p.ks_s[1] : p.vs + page * p.vs_s[0] + place * p.vs_s[1];
+    r.scales_sh = keys ? p.ks_s[2] : p.vs_s[2];
+  }
+  if (keys && !keep) {
+    if (r.dst != nullptr) do_rows<T, G, ROPE, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
+  } else if (keys) {
+    do_rows<T, G, ROPE, true, true>(r, ring, lane, p.D, p.rot, p.eps, table_row);
+  } else if (keep) {
+    do_rows<T, G, 0, false, true>(r, ring, lane, p.D, 0, 0.f, nullptr);
+  }
+}
+
+template <typename T, int G>
 cudaError_t launch_rows(const HeadRowsParams& p, int rope, unsigned grid, cudaStream_t st) {
   switch (rope) {
-    case 0: return launch_pdl(head_rows_kernel<T, G, U, 0>, dim3(grid), dim3(kThreads), 0, st, p);
-    case 1: return launch_pdl(head_rows_kernel<T, G, U, 1>, dim3(grid), dim3(kThreads), 0, st, p);
-    default: return launch_pdl(head_rows_kernel<T, G, U, 2>, dim3(grid), dim3(kThreads), 0, st, p);
+    case 0: return launch_pdl(head_rows_kernel<T, G, 0>, dim3(grid), dim3(kThreads), 0, st, p);
+    case 1: return launch_pdl(head_rows_kernel<T, G, 1>, dim3(grid), dim3(kThreads), 0, st, p);
+    default: return launch_pdl(head_rows_kernel<T, G, 2>, dim3(grid), dim3(kThreads), 0, st, p);
   }
 }
 
 template <typename T, int G>
 int go_rows(HeadRowsParams p, int rope, cudaStream_t st) {
-  const int H = p.Hq + p.Hkv + p.Hv, sms = sm_count();
+  const int sms = sm_count();
   if (sms <= 0) return B200_ERR_CUDA;
   constexpr int RPW = 32 / G, WPB = kThreads / 32;
-  auto chunks = [&](int u) { return (H + RPW * u - 1) / (RPW * u); };
-  // four rows a lane group where that still gives every SM sixteen warps; otherwise one, for latency
-  const bool wide = p.T * chunks(4) >= 16LL * sms;
-  p.chunks = chunks(wide ? 4 : 1);
+  auto chunks = [&](int heads, int u) { return (heads + RPW * u - 1) / (RPW * u); };
+  // Two rows a lane group at a time, and for queries four rounds of that, where every SM still gets sixteen warps; otherwise one
+  // row each, for latency.
+  const bool wide = p.T * (chunks(p.Hq, 8) + chunks(p.Hkv, 2)) >= 16LL * sms;
+  p.heads_q = RPW * (wide ? 8 : 1), p.heads_kv = RPW * (wide ? 2 : 1);
+  p.chunks_q = chunks(p.Hq, wide ? 8 : 1), p.chunks_kv = chunks(p.Hkv, wide ? 2 : 1);
+  p.chunks = p.chunks_q + p.chunks_kv + (p.Hv ? p.chunks_kv : 0);
+  p.chunks_magic = static_cast<uint32_t>((1ULL << 32) / p.chunks + 1);
   const int64_t blocks = (p.T * p.chunks + WPB - 1) / WPB;
-  if (blocks > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
-  B200_CUDA_TRY(wide ? (launch_rows<T, G, 4>(p, rope, static_cast<unsigned>(blocks), st))
-                     : (launch_rows<T, G, 1>(p, rope, static_cast<unsigned>(blocks), st)));
+  if (blocks * WPB > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
+  B200_CUDA_TRY((launch_rows<T, G>(p, rope, static_cast<unsigned>(blocks), st)));
   return B200_OK;
 }
 
 template <typename T>
 int dispatch_rows(const HeadRowsParams& p, int rope, cudaStream_t st) {
-  if (p.D <= 32) return go_rows<T, 4>(p, rope, st);
-  if (p.D <= 64) return go_rows<T, 8>(p, rope, st);
-  if (p.D <= 128) return go_rows<T, 16>(p, rope, st);
-  return go_rows<T, 32>(p, rope, st);
+  if (p.D <= 32) return go_rows<T, 2>(p, rope, st);
+  if (p.D <= 64) return go_rows<T, 4>(p, rope, st);
+  if (p.D <= 128) return go_rows<T, 8>(p, rope, st);
+  return go_rows<T, 16>(p, rope, st);
 }
 
 int take_heads(const b200_heads* h, int64_t T, int H, const void** ptr, int64_t* st, int64_t* sh) {
@@ -429,6 +586,9 @@ int rows_entry(const b200_heads* q, const b200_heads* k, const b200_heads* v, co
     p.page_size = static_cast<uint32_t>(cache->page_size);
     p.num_slots = static_cast<uint32_t>(cache->num_pages * cache->page_size);
   }
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.page_size == 1u << i) p.page_shift = i;
   const int rope = cos_sin ? (is_neox ? 1 : 2) : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == B200_DT_BF16 ? dispatch_rows<__nv_bfloat16>(p, rope, st) : dispatch_rows<__half>(p, rope, st);
