@@ -3,10 +3,12 @@
 //   h[t, s, r]  = sum_k x[t, k] A[a, s R + r, k]                      (shrink; a = the token's adapter, r < rank[a])
 //   out[t, n]   = base[t, n] + scaling[a] sum_r h[t, s(n), r] B[a, n, r]        (expand; s(n) = the slice of column n)
 //
-// The plan groups the tokens by adapter (a stable counting sort), so that a tile of up to kTileRows tokens shares one A and
-// one B; it is made once for a batch of tokens and used by every projection of every layer.
+// The plan groups the tokens by adapter (a stable counting sort), so that a tile of tokens shares one A and one B; it is made
+// once for a batch of tokens and used by every projection of every layer.  Tiles have up to 16 tokens in small batches, where
+// every adapter's weights are read for a few tokens each, and 128 in large ones.
 //
-// Both products are bound by memory: the shrink by x and A, the expand by base, out and B.  Operands go from global memory
+// Both products are bound by memory: the shrink by x and A, the expand by base, out and B.  The large shrink, whose products
+// would bind it on the older matrix instructions, runs on tcgen05 (lora_shrink_tiles_kernel).  In the others operands go from global memory
 // straight into the fragments of mma.m16n8k16: the order in which k is summed is free, so a lane's fragment of two
 // consecutive k16 steps is one 16-byte load (eight consecutive k), and no shared memory or transposition is needed.  The
 // weights are the 16-row operand, the tokens the 8-column one, so a single token wastes no weight traffic.
@@ -15,14 +17,16 @@
 // that adds at most half a step of h (2^-9 for bf16) to the adapter's part of the sum, less than the rounding of out adds.
 #include <cooperative_groups.h>
 
-#include "common.cuh"
+#include "gemm_common.cuh"
 
 namespace b200 {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kTileRows = 16;
+constexpr int kSmallRows = 16, kLargeRows = 128;
+constexpr int64_t kLargeFrom = 512;          // tokens
+__host__ __device__ inline int tile_rows(int64_t T) { return T >= kLargeFrom ? kLargeRows : kSmallRows; }
 constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
 constexpr int kMaxAdapters = 1024;
 constexpr int kMaxSlices = 8;
@@ -30,7 +34,7 @@ constexpr int64_t kMaxTokens = 1000000;     // max_tiles(kMaxTokens, kMaxAdapter
 
 // Device layout of a plan: int32 count[4] (tiles, -, -, -), int4 tiles[max_tiles] (adapter or -1, first, rows, rank), int32 perm[T]
 __host__ __device__ inline int64_t max_tiles(int64_t T, int64_t L) {
-  return T / kTileRows + (L + 1 < T ? L + 1 : T);
+  return T / tile_rows(T) + (L + 1 < T ? L + 1 : T);
 }
 
 struct PlanView {
@@ -48,7 +52,7 @@ inline PlanView view_plan(const void* plan, int64_t T, int64_t L) {
 // One block.  Warp w owns the tokens [w * per, ...); bins [kPlanWarps][L + 1] in shared memory count its tokens per adapter
 // (bin L: none), then hold where its next token of that adapter goes.  Stable: a token's place depends on nothing but the ids.
 __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const int32_t* __restrict__ ids, int64_t T,
-                                                                 const int32_t* __restrict__ ranks, int L,
+                                                                 const int32_t* __restrict__ ranks, int L, int rows,
                                                                  int* __restrict__ count, int4* __restrict__ tiles,
                                                                  int* __restrict__ perm) {
   pdl_start();
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const int32_t* 
       run += c;
     }
     first[a + 1] = run;
-    tile0[a + 1] = (run + kTileRows - 1) / kTileRows;
+    tile0[a + 1] = (run + rows - 1) / rows;
   }
   __syncthreads();
   if (warp == 0) {
@@ -122,8 +126,8 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const int32_t* 
   }
   for (int a = threadIdx.x; a < E; a += kPlanThreads)
     for (int i = tile0[a]; i < tile0[a + 1]; ++i) {
-      const int at = first[a] + (i - tile0[a]) * kTileRows;
-      tiles[i] = make_int4(a < L ? a : -1, at, min(kTileRows, first[a + 1] - at), rank_of[a]);
+      const int at = first[a] + (i - tile0[a]) * rows;
+      tiles[i] = make_int4(a < L ? a : -1, at, min(rows, first[a + 1] - at), rank_of[a]);
     }
 }
 
@@ -252,9 +256,198 @@ lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ 
   cluster.sync();
 }
 
+// A cluster of `splits` blocks computes up to n_alloc columns of h for one tile of up to 128 tokens, each block a part of K.
+// tcgen05: D [128 tokens x columns] += x [128 x 64] A^T [64 x columns], both operands K-major in shared memory with the
+// 128-byte swizzle.  Warps 0-3 copy rows of x and of A (any rows: tokens are gathered through the plan, and only the rows of A
+// below the adapter's rank are fetched, slices packed one behind the other) with 16-byte asynchronous copies, kStages k-blocks
+// ahead; warp 4 issues the products.  Then warps 0-3 read the sums out of tensor memory and, with several blocks, add them in
+// block order through distributed shared memory.
+constexpr int kTileThreads = 160, kBlockK = 64, kTileStages = 4, kMaxColumns = 256;
+constexpr uint32_t kXBytes = kLargeRows * kBlockK * 2;
+
+struct ShrinkTiles {
+  int64_t x_ld, K, h_ld;
+  int R, slices, n_alloc, splits;
+  int* status;
+};
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* status, int code) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = sa::wait(bar, parity, status, code);
+  return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+}
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc_f16(int n) {   // fp32 sums; both operands K-major, bf16 (1) or fp16 (0)
+  const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (static_cast<uint32_t>(n >> 3) << 17) | ((kLargeRows >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const T* __restrict__ x, const T* __restrict__ A,
+                                                                         PlanView plan, T* __restrict__ h,
+                                                                         const __grid_constant__ ShrinkTiles p) {
+  pdl_wait();
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t bars[2 * kTileStages + 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int64_t x_row[kLargeRows], a_row[kMaxColumns];     // element offsets, or -1
+  if (static_cast<int>(blockIdx.y) >= plan.count[0]) return;    // the whole cluster leaves together, here and below
+  const int4 tile = plan.tiles[blockIdx.y];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rows = tile.z, split = blockIdx.x;
+  const int rank = tile.x < 0 ? 0 : min(tile.w, p.R), rank8 = (rank + 7) / 8 * 8;
+  const int c0 = blockIdx.z * p.n_alloc, n = min(p.slices * rank8 - c0, p.n_alloc);      // packed columns of this block
+  if (blockIdx.z == 0 && split == 0) {                          // zeros behind the rank, 16 bytes at a time
+    const int vecs = (p.R - rank8) / 8, all = rows * p.slices * vecs;
+    for (int e = threadIdx.x; e < all; e += kTileThreads) {
+      const int v = e % vecs, s = e / vecs % p.slices, r = e / vecs / p.slices;
+      *reinterpret_cast<uint4*>(h + plan.perm[tile.y + r] * p.h_ld + s * p.R + rank8 + 8 * v) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  if (n <= 0) return;
+  const int n16 = (n + 15) / 16 * 16;
+  for (int r = threadIdx.x; r < kLargeRows; r += kTileThreads) x_row[r] = r < rows ? plan.perm[tile.y + r] * p.x_ld : -1;
+  for (int j = threadIdx.x; j < n16; j += kTileThreads) {
+    const int s = (c0 + j) / rank8, r = (c0 + j) % rank8;
+    a_row[j] = j < n && r < rank ? (static_cast<int64_t>(tile.x) * p.slices * p.R + s * p.R + r) * p.K : -1;
+  }
+  const uint32_t ring = (smem_u32(dyn) + 1023u) & ~1023u, stage_bytes = kXBytes + p.n_alloc * (kBlockK * 2);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kTileStages, done = empty + 8 * kTileStages;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kTileStages; ++i) {
+      sa::init(full + 8 * i, 128);
+      sa::init(empty + 8 * i, 1);
+    }
+    sa::init(done, 1);
+    fence_mbar_init();
+  }
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < static_cast<uint32_t>(n16)) tmem_cols *= 2;
+  if (warp == 4) {
+    tmem_alloc(&tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // Not before every block of this kernel that goes on has its tensor memory: a following kernel that takes all of it and then
+  // waits for this one would otherwise be waited for.
+  pdl_trigger();
+  const uint32_t tmem = tmem_slot;
+  const int64_t nkb = (p.K + kBlockK - 1) / kBlockK;
+  const int kb0 = static_cast<int>(nkb * split / p.splits), count = static_cast<int>(nkb * (split + 1) / p.splits) - kb0;
+  bool ok = true;
+  if (warp < 4) {
+    const int c8 = threadIdx.x % 8, r0 = threadIdx.x / 8;
+    for (int i = 0; i < count + kTileStages - 1; ++i) {
+      if (i < count) {
+        const int stage = i % kTileStages;
+        ok = warp_wait(empty + 8 * stage, ((i / kTileStages) & 1) ^ 1, p.status, 51);
+        if (!ok) break;
+        const int64_t k = static_cast<int64_t>(kb0 + i) * kBlockK + 8 * c8;
+        const uint32_t xs = ring + stage * stage_bytes, as = xs + kXBytes;
+#pragma unroll
+        for (int j = 0; j < kLargeRows / 16; ++j) {
+          const int r = r0 + 16 * j;
+          const int64_t off = x_row[r];
+          const bool in = off >= 0 && k < p.K;
+          sa::cp_async16(xs + r * 128 + ((c8 ^ (r & 7)) << 4), x + (in ? off + k : 0), in);
+        }
+        for (int r = r0; r < n16; r += 16) {
+          const int64_t off = a_row[r];
+          const bool in = off >= 0 && k < p.K;
+          sa::cp_async16(as + r * 128 + ((c8 ^ (r & 7)) << 4), A + (in ? off + k : 0), in);
+        }
+      }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group %0;" ::"n"(kTileStages - 1) : "memory");
+      if (i >= kTileStages - 1) {                               // block i - (kTileStages - 1) has landed
+        fence_proxy_async_smem();
+        sa::arrive(full + 8 * ((i - (kTileStages - 1)) % kTileStages));
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    const uint32_t idesc = idesc_f16<T>(n16);
+    for (int i = 0; i < count; ++i) {
+      const int stage = i % kTileStages;
+      ok = warp_wait(full + 8 * stage, (i / kTileStages) & 1, p.status, 52);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t xs = ring + stage * stage_bytes;
+        const uint64_t xd = umma_desc_k128(xs), ad = umma_desc_k128(xs + kXBytes);
+#pragma unroll
+        for (int k = 0; k < kBlockK / 16; ++k) umma_f16(tmem, xd + 2 * k, ad + 2 * k, idesc, i > 0 || k > 0);
+        sa::commit(empty + 8 * stage);
+        if (i + 1 == count) sa::commit(done);
+      }
+      __syncwarp();
+    }
+  }
+  // columns [j, j + 8) of token row `row`, packed column c0 + j on
+  auto put = [&](int row, int j, const float* v) {
+    const int s = (c0 + j) / rank8, r = (c0 + j) % rank8;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = pack2(static_cast<T*>(nullptr), r + 2 * i < rank ? v[2 * i] : 0.f, r + 2 * i + 1 < rank ? v[2 * i + 1] : 0.f);
+    *reinterpret_cast<uint4*>(h + plan.perm[tile.y + row] * p.h_ld + s * p.R + r) = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  float* partial = reinterpret_cast<float*>(dyn + (ring - smem_u32(dyn)));       // [columns][128], where the ring was
+  if (warp < 4) {
+    if (ok) ok = warp_wait(done, 0, p.status, 53);
+    tc_fence_after();
+    const int row = warp * 32 + lane;
+    for (int j = 0; j < n16; j += 16) {
+      float v[16];
+      tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + j, v);
+      tmem_ld_wait();
+      if (p.splits == 1) {
+        if (ok && row < rows) {
+          put(row, j, v);
+          if (j + 8 < n) put(row, j + 8, v + 8);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) partial[(j + i) * kLargeRows + row] = v[i];
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+  if (p.splits == 1) return;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int share = kLargeRows / p.splits;
+  for (int e = threadIdx.x; e < share * (n / 8); e += kTileThreads) {
+    const int row = split * share + e % share, j = e / share * 8;
+    if (row >= rows) continue;
+    float v[8] = {};
+    for (int b = 0; b < p.splits; ++b) {
+      const float* other = cluster.map_shared_rank(partial, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += other[(j + i) * kLargeRows + row];
+    }
+    if (*reinterpret_cast<volatile int*>(p.status) == 0) put(row, j, v);
+  }
+  cluster.sync();
+}
+
 // ------------------------------------------------------------------------------------------------------- expand
 struct Slices {
-  int n, first_col[kMaxSlices + 1], first_block[kMaxSlices + 1];     // columns; blocks of 64 columns
+  int n, first_col[kMaxSlices + 1], first_block[kMaxSlices + 1];     // columns; blocks of the columns of a warp
 };
 
 template <typename T>
@@ -267,15 +460,6 @@ template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-__device__ __forceinline__ uint32_t pack2_as(float a, float b, __nv_bfloat16*) {
-  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&t);
-}
-__device__ __forceinline__ uint32_t pack2_as(float a, float b, __half*) {
-  const __half2 t = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&t);
-}
-
 constexpr int kExpandThreads = 128;
 
 // A warp: 64 columns of one slice for one tile of up to 16 tokens.  Weight row (tile i, half f, lane / 4) of its four 16-row
@@ -345,11 +529,157 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* __
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           const float2 b = unpack2<T>(w[m]);
-          w[m] = pack2_as(fmaf(scaling, acc[i][m][j], b.x), fmaf(scaling, acc[i][m][j + 2], b.y), static_cast<T*>(nullptr));
+          w[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[i][m][j], b.x), fmaf(scaling, acc[i][m][j + 2], b.y));
         }
       }
       *reinterpret_cast<uint4*>(out + t * out_ld + n) = v;
     }
+}
+
+// Tiles of up to 128 tokens: a warp holds the B of NT x 8 columns of one slice in registers (tokens are the 16-row operand here)
+// and walks down the tile, 16 tokens at a time.  Row g of the 8-column operand i is column 2 NT (g / 2) + 2 i + g % 2, so that a
+// lane's 2 NT sums of a token are neighbours and base and out move 16 bytes at a time (8 with NT = 2).  RJ = ceil(R / 32).
+constexpr int kWalkThreads = 128;
+
+template <typename T, int RJ, int NT>
+__global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T* __restrict__ h, int64_t h_ld, const T* __restrict__ B,
+                                                                         int64_t N, int R, const float* __restrict__ scalings,
+                                                                         PlanView plan, const __grid_constant__ Slices sl,
+                                                                         const T* base, int64_t base_ld, T* out, int64_t out_ld) {
+  pdl_start();
+  if (static_cast<int>(blockIdx.y) >= plan.count[0]) return;
+  const int4 tile = plan.tiles[blockIdx.y];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+  const int block = blockIdx.x * (kWalkThreads / 32) + warp;
+  if (block >= sl.first_block[sl.n]) return;
+  int s = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxSlices; ++i) s += i < sl.n && block >= sl.first_block[i];
+  const int n0 = sl.first_col[s] + (block - sl.first_block[s]) * (8 * NT), n_end = sl.first_col[s + 1];
+  const int n = n0 + 2 * NT * c;                             // the first of this lane's 2 NT columns
+  const bool live = n < n_end;
+  const int rows = tile.z;
+  const bool none = tile.x < 0;
+  if (none && base == out) return;
+  const int rank = none ? 0 : min(tile.w, R);
+  const float scaling = none ? 0.f : __ldg(scalings + tile.x);
+  uint4 w[NT][RJ];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < RJ; ++j) {
+      const int col = n0 + 2 * NT * (g / 2) + 2 * i + g % 2, keep = rank - 32 * j - 8 * c;
+      w[i][j] = load_if(col < n_end && keep > 0, B + (static_cast<int64_t>(tile.x) * N + col) * R + 32 * j + 8 * c);
+      if (keep < 8) w[i][j] = first_of(w[i][j], keep);
+    }
+  const int* perm = plan.perm + tile.y;
+#pragma unroll 2
+  for (int r0 = 0; r0 < rows; r0 += 16) {
+    int64_t t[2];
+    bool in[2];
+    uint4 hv[2][RJ];
+    uint32_t v[2][NT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      in[i] = r0 + g + 8 * i < rows;
+      t[i] = in[i] ? __ldg(perm + r0 + g + 8 * i) : 0;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) v[i][j] = 0;
+      if (base != nullptr && in[i] && live) {
+        const T* src = base + t[i] * base_ld + n;
+        if constexpr (NT == 4) {
+          const uint4 q = *reinterpret_cast<const uint4*>(src);
+          v[i][0] = q.x, v[i][1] = q.y, v[i][2] = q.z, v[i][3] = q.w;
+        } else {
+          const uint2 q = *reinterpret_cast<const uint2*>(src);
+          v[i][0] = q.x, v[i][1] = q.y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < RJ; ++j)
+        hv[i][j] = load_if(in[i] && rank - 32 * j - 8 * c > 0, h + t[i] * h_ld + s * R + 32 * j + 8 * c);
+    }
+    float acc[NT][4] = {};
+#pragma unroll
+    for (int j = 0; j < RJ; ++j)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) mma_k32<T>(acc[i], hv[0][j], hv[1][j], w[i][j]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (!in[i] || !live) continue;
+      if (!none) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float2 b = unpack2<T>(v[i][j]);
+          v[i][j] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[j][2 * i], b.x), fmaf(scaling, acc[j][2 * i + 1], b.y));
+        }
+      }
+      T* dst = out + t[i] * out_ld + n;
+      if constexpr (NT == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(v[i][0], v[i][1]);
+    }
+  }
+}
+
+template <typename T>
+int shrink(const T* x, int64_t x_ld, const T* A, PlanView plan, int64_t tokens, int64_t tiles, int64_t K, int R, int slices, T* h,
+           int64_t h_ld, cudaStream_t st) {
+  const int cols = slices * R;
+  if (K == 0) {
+    B200_CUDA_TRY(cudaMemset2DAsync(h, h_ld * sizeof(T), 0, cols * sizeof(T), tokens, st));
+    return B200_OK;
+  }
+  if (tile_rows(tokens) == kSmallRows) {
+    const dim3 grid(kShrinkCluster, static_cast<unsigned>(tiles), static_cast<unsigned>((cols + 15) / 16));
+    B200_CUDA_TRY(launch_pdl(lora_shrink_kernel<T>, grid, dim3(kShrinkThreads), 0, st, x, x_ld, A, K, R, cols, plan, h, h_ld));
+    return B200_OK;
+  }
+  if (gemm_sticky_status() != 0) return B200_ERR_DEVICE_TIMEOUT;
+  ShrinkTiles p = {x_ld, K, h_ld, R, slices};
+  p.status = gemm_status_ptr();
+  const int sms = sm_count();
+  if (!p.status || sms <= 0) return B200_ERR_CUDA;
+  p.n_alloc = cols < kMaxColumns ? (cols + 15) / 16 * 16 : kMaxColumns;
+  const int passes = (cols + kMaxColumns - 1) / kMaxColumns;
+  // As many blocks a tile as give every SM at most one, the tiles being about as many as whole ones.
+  p.splits = 1;
+  while (p.splits < 8 && 2 * p.splits * passes * ((tokens + kLargeRows - 1) / kLargeRows) <= sms && 2 * p.splits * kBlockK <= K) p.splits *= 2;
+  const size_t smem = 1024 + kTileStages * (kXBytes + static_cast<size_t>(p.n_alloc) * kBlockK * 2);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(p.splits, static_cast<unsigned>(tiles), passes);
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_tiles_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, lora_shrink_tiles_kernel<T>, x, A, plan, h, static_cast<const ShrinkTiles&>(p)));
+  return B200_OK;
+}
+
+// Columns of a warp of the expand.
+int expand_columns(int64_t tokens, int R) { return tile_rows(tokens) == kSmallRows ? 64 : R <= 128 ? 32 : 16; }
+
+template <typename T>
+int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* scalings, PlanView plan, const Slices& sl, int64_t tokens,
+           int64_t tiles, const T* base, int64_t base_ld, T* out, int64_t out_ld, cudaStream_t st) {
+  static_assert(kExpandThreads == kWalkThreads, "one grid for both");
+  constexpr int kWarps = kExpandThreads / 32;
+  const dim3 grid(static_cast<unsigned>((sl.first_block[sl.n] + kWarps - 1) / kWarps), static_cast<unsigned>(tiles));
+  auto go = [&](auto kern) {
+    return launch_pdl(kern, grid, dim3(kExpandThreads), 0, st, h, h_ld, B, N, R, scalings, plan, sl, base, base_ld, out, out_ld);
+  };
+  if (tile_rows(tokens) == kSmallRows) B200_CUDA_TRY(go(lora_expand_kernel<T>));
+  else if (R <= 32) B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 1, 4>));
+  else if (R <= 64) B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 2, 4>));
+  else if (R <= 128) B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 4, 4>));
+  else B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 8, 2>));
+  return B200_OK;
 }
 
 int check_plan(const void* plan, size_t bytes, int64_t T, int64_t L) {
@@ -382,7 +712,7 @@ extern "C" int b200_lora_plan(const int32_t* token_adapters, int64_t T, const in
   const size_t smem = sizeof(int) * ((kPlanWarps + 1) * (L + 1) + 2 * (L + 2));
   if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   B200_CUDA_TRY(launch_pdl(lora_plan_kernel, dim3(1), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), token_adapters, T,
-                           ranks, L, const_cast<int*>(v.count), const_cast<int4*>(v.tiles), const_cast<int*>(v.perm)));
+                           ranks, L, tile_rows(T), const_cast<int*>(v.count), const_cast<int4*>(v.tiles), const_cast<int*>(v.perm)));
   return B200_OK;
 }
 
@@ -401,16 +731,13 @@ extern "C" int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int 
   if ((K > 0 && (!x || !A)) || !h) return B200_ERR_NULL_PTR;
   if (!aligned16(x) || !aligned16(A) || !aligned16(h)) return B200_ERR_MISALIGNED;
   const int64_t tiles = max_tiles(T, L);
-  const dim3 grid(kShrinkCluster, static_cast<unsigned>(tiles), static_cast<unsigned>((cols + 15) / 16));
   const PlanView v = view_plan(plan, T, L);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == B200_DT_BF16)
-    B200_CUDA_TRY(launch_pdl(lora_shrink_kernel<__nv_bfloat16>, grid, dim3(kShrinkThreads), 0, st, static_cast<const __nv_bfloat16*>(x),
-                             x_ld, static_cast<const __nv_bfloat16*>(A), K, R, cols, v, static_cast<__nv_bfloat16*>(h), h_ld));
-  else
-    B200_CUDA_TRY(launch_pdl(lora_shrink_kernel<__half>, grid, dim3(kShrinkThreads), 0, st, static_cast<const __half*>(x), x_ld,
-                             static_cast<const __half*>(A), K, R, cols, v, static_cast<__half*>(h), h_ld));
-  return B200_OK;
+    return shrink(static_cast<const __nv_bfloat16*>(x), x_ld, static_cast<const __nv_bfloat16*>(A), v, T, tiles, K, R, num_slices,
+                  static_cast<__nv_bfloat16*>(h), h_ld, st);
+  return shrink(static_cast<const __half*>(x), x_ld, static_cast<const __half*>(A), v, T, tiles, K, R, num_slices,
+                static_cast<__half*>(h), h_ld, st);
 }
 
 extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes,
@@ -422,6 +749,7 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
   if (num_slices <= 0 || !slice_sizes) return num_slices <= 0 ? B200_ERR_BAD_SHAPE : B200_ERR_NULL_PTR;
   if (num_slices > kMaxSlices) return B200_ERR_TOO_LARGE;
   if (dtype != B200_DT_BF16 && dtype != B200_DT_F16) return B200_ERR_BAD_DTYPE;
+  const int warp_cols = expand_columns(T, R);
   Slices sl = {};
   sl.n = num_slices;
   int64_t N = 0;
@@ -430,7 +758,7 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
     N += slice_sizes[i];
     if (N > (1 << 30)) return B200_ERR_TOO_LARGE;
     sl.first_col[i + 1] = static_cast<int>(N);
-    sl.first_block[i + 1] = sl.first_block[i] + static_cast<int>((slice_sizes[i] + 63) / 64);
+    sl.first_block[i + 1] = sl.first_block[i] + static_cast<int>((slice_sizes[i] + warp_cols - 1) / warp_cols);
   }
   if (h_ld < num_slices * static_cast<int64_t>(R) || h_ld % 8 != 0 || out_ld < N || out_ld % 8 != 0 ||
       (base && (base_ld < N || base_ld % 8 != 0)))
@@ -440,17 +768,11 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
   if (!h || !B || !scalings || !out) return B200_ERR_NULL_PTR;
   if (!aligned16(h) || !aligned16(B) || !aligned16(base) || !aligned16(out)) return B200_ERR_MISALIGNED;
   const int64_t tiles = max_tiles(T, L);
-  constexpr int kWarps = kExpandThreads / 32;
-  const dim3 grid(static_cast<unsigned>((sl.first_block[num_slices] + kWarps - 1) / kWarps), static_cast<unsigned>(tiles));
   const PlanView v = view_plan(plan, T, L);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == B200_DT_BF16)
-    B200_CUDA_TRY(launch_pdl(lora_expand_kernel<__nv_bfloat16>, grid, dim3(kExpandThreads), 0, st, static_cast<const __nv_bfloat16*>(h),
-                             h_ld, static_cast<const __nv_bfloat16*>(B), N, R, scalings, v, sl,
-                             static_cast<const __nv_bfloat16*>(base), base_ld, static_cast<__nv_bfloat16*>(out), out_ld));
-  else
-    B200_CUDA_TRY(launch_pdl(lora_expand_kernel<__half>, grid, dim3(kExpandThreads), 0, st, static_cast<const __half*>(h), h_ld,
-                             static_cast<const __half*>(B), N, R, scalings, v, sl, static_cast<const __half*>(base), base_ld,
-                             static_cast<__half*>(out), out_ld));
-  return B200_OK;
+    return expand(static_cast<const __nv_bfloat16*>(h), h_ld, static_cast<const __nv_bfloat16*>(B), N, R, scalings, v, sl, T, tiles,
+                  static_cast<const __nv_bfloat16*>(base), base_ld, static_cast<__nv_bfloat16*>(out), out_ld, st);
+  return expand(static_cast<const __half*>(h), h_ld, static_cast<const __half*>(B), N, R, scalings, v, sl, T, tiles,
+                static_cast<const __half*>(base), base_ld, static_cast<__half*>(out), out_ld, st);
 }
