@@ -46,6 +46,8 @@ int gemm_sticky_status();
 // 2-D tensor map over a row-major [rows, cols] byte matrix with leading dimension ld, box =
 // box_rows x 128 bytes, 128-byte swizzle, zero fill outside the matrix.
 int make_map_u8_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
+// The same over 16-bit elements (cols and ld in elements), box = box_rows x 64 elements.
+int make_map_u16_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
 
 // The dense fp32-promotion GEMM behind the C entry points (gemm.cu).  split_k 0: the library's own schedule, as far as the
 // workspace allows; sa_ue8m0: packed exponent activation scales; bias and prefetch_w as in GemmParams.

@@ -147,12 +147,6 @@ __device__ __forceinline__ uint4 quantise16(const f2 (&y)[8], float scale) {
 
 constexpr int kStages = 4, kStageBytes = 32 * 32;            // row groups in flight for each warp
 
-__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
 // What differs between queries, keys and values, decided once for a warp.
 template <typename T>
 struct Rows {
@@ -193,7 +187,7 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
     if (r.first + i * RPW < r.last) fetch(r.first + i * RPW, i);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    sa::cp_async_commit();
   }
   f2 w[8];
 #pragma unroll
@@ -239,15 +233,16 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
     {
       const int ahead = head + (kStages - 1) * RPW;
       if (ahead < r.last) fetch(ahead, (stage + kStages - 1) % kStages);
-      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      sa::cp_async_commit();
+      sa::cp_async_wait<kStages - 1>();
     }
     const int h = head + sub;
     const bool live = h < r.last && in_row;
     f2 y[8];
     {
       const uint32_t from = ring + stage * kStageBytes;
-      unpack8<T>(ld_shared16(from), y);
-      unpack8<T>(ld_shared16(from + kStageBytes / 2), y + 4);
+      unpack8<T>(sa::ld_v4(from), y);
+      unpack8<T>(sa::ld_v4(from + kStageBytes / 2), y + 4);
       stage = (stage + 1) % kStages;
     }
     if (r.weight != nullptr) {

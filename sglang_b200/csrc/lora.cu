@@ -258,16 +258,18 @@ lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ 
 
 // A cluster of `splits` blocks computes up to n_alloc columns of h for one tile of up to 128 tokens, each block a part of K.
 // tcgen05: D [128 tokens x columns] += x [128 x 64] A^T [64 x columns], both operands K-major in shared memory with the
-// 128-byte swizzle.  Warps 0-3 copy rows of x and of A (any rows: tokens are gathered through the plan, and only the rows of A
-// below the adapter's rank are fetched, slices packed one behind the other) with 16-byte asynchronous copies, kStages k-blocks
-// ahead; warp 4 issues the products.  Then warps 0-3 read the sums out of tensor memory and, with several blocks, add them in
-// block order through distributed shared memory.
-constexpr int kTileThreads = 160, kBlockK = 64, kTileStages = 4, kMaxColumns = 256;
+// 128-byte swizzle.  Warps 0 and 2 fetch half of the tile's x each, with one TMA box where its tokens are neighbours, else eight
+// rows at a time or gathered four by four; warp 3 fetches the rows of A below the adapter's rank, box by box, the slices packed
+// one behind the other; warp 1 issues the products.  Then all four warps read the sums out of tensor memory and, with several
+// blocks, add them in block order through distributed shared memory.  The number of TMA instructions counts: with one warp
+// issuing forty boxes of eight rows per k-block, a k-block took 2.2 us (8191 x 8192 and 192 columns: 141 us; rows copied by all
+// threads with 16-byte asynchronous copies: 174 us).
+constexpr int kTileThreads = 128, kBlockK = 64, kMaxTileStages = 8, kMaxColumns = 256;
 constexpr uint32_t kXBytes = kLargeRows * kBlockK * 2;
 
 struct ShrinkTiles {
-  int64_t x_ld, K, h_ld;
-  int R, slices, n_alloc, splits;
+  int64_t K, h_ld;
+  int R, slices, n_alloc, splits, stages, a_box;
   int* status;
 };
 
@@ -291,39 +293,37 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const T* __restrict__ x, const T* __restrict__ A,
+__global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap x1_map,
+                                                                         const __grid_constant__ CUtensorMap x8_map,
+                                                                         const __grid_constant__ CUtensorMap x64_map,
+                                                                         const __grid_constant__ CUtensorMap a_map,
                                                                          PlanView plan, T* __restrict__ h,
                                                                          const __grid_constant__ ShrinkTiles p) {
   pdl_wait();
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t bars[2 * kTileStages + 1];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxTileStages + 1];
   __shared__ uint32_t tmem_slot;
-  __shared__ int64_t x_row[kLargeRows], a_row[kMaxColumns];     // element offsets, or -1
-  if (static_cast<int>(blockIdx.y) >= plan.count[0]) return;    // the whole cluster leaves together, here and below
-  const int4 tile = plan.tiles[blockIdx.y];
+  const int tiles = plan.count[0];
+  const int4 tile = plan.tiles[blockIdx.y];                     // in bounds whether or not it is one
+  if (static_cast<int>(blockIdx.y) >= tiles) return;            // the whole cluster leaves together, here and below
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rows = tile.z, split = blockIdx.x;
-  const int rank = tile.x < 0 ? 0 : min(tile.w, p.R), rank8 = (rank + 7) / 8 * 8;
-  const int c0 = blockIdx.z * p.n_alloc, n = min(p.slices * rank8 - c0, p.n_alloc);      // packed columns of this block
+  const int rank = tile.x < 0 ? 0 : min(tile.w, p.R), width = (rank + p.a_box - 1) / p.a_box * p.a_box;    // of a slice
+  const int c0 = blockIdx.z * p.n_alloc, n = min(p.slices * width - c0, p.n_alloc);      // packed columns of this block
   if (blockIdx.z == 0 && split == 0) {                          // zeros behind the rank, 16 bytes at a time
-    const int vecs = (p.R - rank8) / 8, all = rows * p.slices * vecs;
+    const int vecs = (p.R - width) / 8, all = rows * p.slices * vecs;
     for (int e = threadIdx.x; e < all; e += kTileThreads) {
       const int v = e % vecs, s = e / vecs % p.slices, r = e / vecs / p.slices;
-      *reinterpret_cast<uint4*>(h + plan.perm[tile.y + r] * p.h_ld + s * p.R + rank8 + 8 * v) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(h + plan.perm[tile.y + r] * p.h_ld + s * p.R + width + 8 * v) = make_uint4(0, 0, 0, 0);
     }
   }
   if (n <= 0) return;
   const int n16 = (n + 15) / 16 * 16;
-  for (int r = threadIdx.x; r < kLargeRows; r += kTileThreads) x_row[r] = r < rows ? plan.perm[tile.y + r] * p.x_ld : -1;
-  for (int j = threadIdx.x; j < n16; j += kTileThreads) {
-    const int s = (c0 + j) / rank8, r = (c0 + j) % rank8;
-    a_row[j] = j < n && r < rank ? (static_cast<int64_t>(tile.x) * p.slices * p.R + s * p.R + r) * p.K : -1;
-  }
   const uint32_t ring = (smem_u32(dyn) + 1023u) & ~1023u, stage_bytes = kXBytes + p.n_alloc * (kBlockK * 2);
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kTileStages, done = empty + 8 * kTileStages;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxTileStages, done = empty + 8 * kMaxTileStages;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kTileStages; ++i) {
-      sa::init(full + 8 * i, 128);
+    for (int i = 0; i < p.stages; ++i) {
+      sa::init(full + 8 * i, 3);
       sa::init(empty + 8 * i, 1);
     }
     sa::init(done, 1);
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const T
   }
   uint32_t tmem_cols = 32;
   while (tmem_cols < static_cast<uint32_t>(n16)) tmem_cols *= 2;
-  if (warp == 4) {
+  if (warp == 1) {
     tmem_alloc(&tmem_slot, tmem_cols);
     tmem_relinquish();
   }
@@ -345,40 +345,55 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const T
   const int64_t nkb = (p.K + kBlockK - 1) / kBlockK;
   const int kb0 = static_cast<int>(nkb * split / p.splits), count = static_cast<int>(nkb * (split + 1) / p.splits) - kb0;
   bool ok = true;
-  if (warp < 4) {
-    const int c8 = threadIdx.x % 8, r0 = threadIdx.x / 8;
-    for (int i = 0; i < count + kTileStages - 1; ++i) {
-      if (i < count) {
-        const int stage = i % kTileStages;
-        ok = warp_wait(empty + 8 * stage, ((i / kTileStages) & 1) ^ 1, p.status, 51);
-        if (!ok) break;
-        const int64_t k = static_cast<int64_t>(kb0 + i) * kBlockK + 8 * c8;
-        const uint32_t xs = ring + stage * stage_bytes, as = xs + kXBytes;
+  if (warp != 1) {
+    // x: rows 64 half ... of the tile, lanes 0-7 with eight each (tokens are in ascending order, so the ends of a run tell whether
+    // it has gaps; rows behind the tile's last are any rows, their sums are not used).  A: lane by lane one box.
+    const int half = 64 * (warp / 2), first = half + 8 * (lane % 8);
+    int y[8], last = 0;
+    bool run64 = false, run8 = false;
+    if (warp != 3) {
 #pragma unroll
-        for (int j = 0; j < kLargeRows / 16; ++j) {
-          const int r = r0 + 16 * j;
-          const int64_t off = x_row[r];
-          const bool in = off >= 0 && k < p.K;
-          sa::cp_async16(xs + r * 128 + ((c8 ^ (r & 7)) << 4), x + (in ? off + k : 0), in);
-        }
-        for (int r = r0; r < n16; r += 16) {
-          const int64_t off = a_row[r];
-          const bool in = off >= 0 && k < p.K;
-          sa::cp_async16(as + r * 128 + ((c8 ^ (r & 7)) << 4), A + (in ? off + k : 0), in);
-        }
-      }
-      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group %0;" ::"n"(kTileStages - 1) : "memory");
-      if (i >= kTileStages - 1) {                               // block i - (kTileStages - 1) has landed
-        fence_proxy_async_smem();
-        sa::arrive(full + 8 * ((i - (kTileStages - 1)) % kTileStages));
-      }
+      for (int i = 0; i < 8; ++i) y[i] = __ldg(plan.perm + tile.y + min(first + i, rows - 1));
+      last = __ldg(plan.perm + tile.y + min(half + 63, rows - 1));
+      const int head = __shfl_sync(0xffffffffu, y[0], 0);
+      run64 = half >= rows || last - head == min(half + 63, rows - 1) - half;
+      run8 = first >= rows || y[7] - y[0] == min(first + 7, rows - 1) - first;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    const int boxes = n / p.a_box, j = c0 + lane * p.a_box;
+    const int ay = warp == 3 && lane < boxes ? tile.x * p.slices * p.R + j / width * p.R + j % width : 0;
+    const uint32_t bytes = warp == 3 ? n * (kBlockK * 2) : kXBytes / 2;
+    int stage = 0, phase = 1;
+    for (int i = 0; i < count; ++i) {
+      ok = warp_wait(empty + 8 * stage, phase, p.status, 51);
+      if (!ok) {                                                // let what is under way land before shared memory is given up
+        for (int b = 0; b < min(i, p.stages); ++b) {
+          if (stage-- == 0) stage = p.stages - 1, phase ^= 1;
+          warp_wait(full + 8 * stage, phase ^ 1, p.status, 54);
+        }
+        break;
+      }
+      const uint32_t bar = full + 8 * stage, to = ring + stage * stage_bytes + (warp == 3 ? kXBytes : half * 128);
+      const int k = (kb0 + i) * kBlockK;
+      if (lane == 0) sa::expect_tx(bar, bytes);
+      __syncwarp();
+      if (warp == 3) {
+        if (lane < boxes) sa::tma_load_2d(to + lane * p.a_box * 128, &a_map, bar, k, ay);
+      } else if (run64) {
+        if (lane == 0) sa::tma_load_2d(to, &x64_map, bar, k, y[0]);
+      } else if (lane < 8) {
+        if (run8) {
+          sa::tma_load_2d(to + lane * 1024, &x8_map, bar, k, y[0]);
+        } else {
+          sa::tma_gather4(to + lane * 1024, &x1_map, bar, k, y[0], y[1], y[2], y[3]);
+          sa::tma_gather4(to + lane * 1024 + 512, &x1_map, bar, k, y[4], y[5], y[6], y[7]);
+        }
+      }
+      if (++stage == p.stages) stage = 0, phase ^= 1;
+    }
   } else {
     const uint32_t idesc = idesc_f16<T>(n16);
-    for (int i = 0; i < count; ++i) {
-      const int stage = i % kTileStages;
-      ok = warp_wait(full + 8 * stage, (i / kTileStages) & 1, p.status, 52);
+    for (int i = 0, stage = 0, phase = 0; i < count; ++i) {
+      ok = warp_wait(full + 8 * stage, phase, p.status, 52);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -390,11 +405,12 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const T
         if (i + 1 == count) sa::commit(done);
       }
       __syncwarp();
+      if (++stage == p.stages) stage = 0, phase ^= 1;
     }
   }
   // columns [j, j + 8) of token row `row`, packed column c0 + j on
   auto put = [&](int row, int j, const float* v) {
-    const int s = (c0 + j) / rank8, r = (c0 + j) % rank8;
+    const int s = (c0 + j) / width, r = (c0 + j) % width;
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -402,9 +418,9 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const T
     *reinterpret_cast<uint4*>(h + plan.perm[tile.y + row] * p.h_ld + s * p.R + r) = make_uint4(w[0], w[1], w[2], w[3]);
   };
   float* partial = reinterpret_cast<float*>(dyn + (ring - smem_u32(dyn)));       // [columns][128], where the ring was
-  if (warp < 4) {
-    if (ok) ok = warp_wait(done, 0, p.status, 53);
-    tc_fence_after();
+  if (ok) ok = warp_wait(done, 0, p.status, 53);
+  tc_fence_after();
+  {
     const int row = warp * 32 + lane;
     for (int j = 0; j < n16; j += 16) {
       float v[16];
@@ -423,7 +439,7 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const T
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
   }
@@ -539,7 +555,11 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* __
 // Tiles of up to 128 tokens: a warp holds the B of NT x 8 columns of one slice in registers (tokens are the 16-row operand here)
 // and walks down the tile, 16 tokens at a time.  Row g of the 8-column operand i is column 2 NT (g / 2) + 2 i + g % 2, so that a
 // lane's 2 NT sums of a token are neighbours and base and out move 16 bytes at a time (8 with NT = 2).  RJ = ceil(R / 32).
-constexpr int kWalkThreads = 128;
+// The tile's h lies in shared memory, for all of the block's warps; base comes through a ring of kWalkStages steps in shared
+// memory in which each lane has its own place, so that three steps are under way without registers being held for them.
+constexpr int kWalkThreads = 128, kWalkStages = 4;
+template <int RJ, int NT>
+constexpr int walk_smem() { return kLargeRows * RJ * 64 + kWalkThreads * kWalkStages * 2 * NT * 4; }
 
 template <typename T, int RJ, int NT>
 __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T* __restrict__ h, int64_t h_ld, const T* __restrict__ B,
@@ -547,22 +567,28 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
                                                                          PlanView plan, const __grid_constant__ Slices sl,
                                                                          const T* base, int64_t base_ld, T* out, int64_t out_ld) {
   pdl_start();
-  if (static_cast<int>(blockIdx.y) >= plan.count[0]) return;
-  const int4 tile = plan.tiles[blockIdx.y];
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ int row_of[kLargeRows];
+  const int tiles = plan.count[0];
+  const int4 tile = plan.tiles[blockIdx.y];                  // in bounds whether or not it is one
+  if (static_cast<int>(blockIdx.y) >= tiles) return;
+  const int rows = tile.z;
+  const bool none = tile.x < 0;
+  if (none && base == out) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+  const int rank = none ? 0 : min(tile.w, R);
+  // a block's four warps have neighbouring columns, of one slice (Slices::first_block counts in fours)
   const int block = blockIdx.x * (kWalkThreads / 32) + warp;
-  if (block >= sl.first_block[sl.n]) return;
   int s = 0;
 #pragma unroll
   for (int i = 1; i < kMaxSlices; ++i) s += i < sl.n && block >= sl.first_block[i];
   const int n0 = sl.first_col[s] + (block - sl.first_block[s]) * (8 * NT), n_end = sl.first_col[s + 1];
   const int n = n0 + 2 * NT * c;                             // the first of this lane's 2 NT columns
   const bool live = n < n_end;
-  const int rows = tile.z;
-  const bool none = tile.x < 0;
-  if (none && base == out) return;
-  const int rank = none ? 0 : min(tile.w, R);
-  const float scaling = none ? 0.f : __ldg(scalings + tile.x);
+  const uint32_t hs = smem_u32(dyn);
+  const uint32_t ring = hs + kLargeRows * RJ * 64 + threadIdx.x * (4 * NT);
+  constexpr uint32_t kHalf = kWalkThreads * 4 * NT, kStage = 2 * kHalf;    // [stage][row half][thread]
+  row_of[threadIdx.x] = static_cast<int>(threadIdx.x) < rows ? __ldg(plan.perm + tile.y + threadIdx.x) : 0;
   uint4 w[NT][RJ];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -570,59 +596,87 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
     for (int j = 0; j < RJ; ++j) {
       const int col = n0 + 2 * NT * (g / 2) + 2 * i + g % 2, keep = rank - 32 * j - 8 * c;
       w[i][j] = load_if(col < n_end && keep > 0, B + (static_cast<int64_t>(tile.x) * N + col) * R + 32 * j + 8 * c);
+    }
+  const float scaling = none ? 0.f : __ldg(scalings + tile.x);
+  __syncthreads();
+  // the 16-byte vectors of a row of h, those of odd rows with halves of 64 bytes exchanged: eight lanes then read all banks
+  auto h_at = [&](int row, int v) { return hs + row * (RJ * 64) + ((RJ == 1 ? v : v ^ ((row & 1) << 2)) << 4); };
+  if (!none) {
+    for (int e = threadIdx.x; e < kLargeRows * RJ * 4; e += kWalkThreads) {
+      const int row = e / (RJ * 4), v = e % (RJ * 4);
+      const bool in = row < rows && v * 8 < rank;
+      sa::cp_async16(h_at(row, v), h + (in ? row_of[row] * h_ld + s * R + v * 8 : 0), in);
+    }
+  }
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = step * 16 + g + 8 * i;
+      const bool in = base != nullptr && r < rows && live;
+      const T* src = in ? base + row_of[r] * base_ld + n : h;
+      const uint32_t to = ring + step % kWalkStages * kStage + i * kHalf;
+      if constexpr (NT == 4) sa::cp_async16(to, src, in);
+      else sa::cp_async8(to, src, in);
+    }
+  };
+  const int steps = (rows + 15) / 16;
+  sa::cp_async_commit();
+#pragma unroll
+  for (int i = 0; i < kWalkStages - 1; ++i) {
+    if (i < steps) fetch(i);
+    sa::cp_async_commit();
+  }
+  sa::cp_async_wait<kWalkStages - 1>();                      // h
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < RJ; ++j) {
+      const int keep = rank - 32 * j - 8 * c;
       if (keep < 8) w[i][j] = first_of(w[i][j], keep);
     }
-  const int* perm = plan.perm + tile.y;
-#pragma unroll 2
-  for (int r0 = 0; r0 < rows; r0 += 16) {
-    int64_t t[2];
-    bool in[2];
-    uint4 hv[2][RJ];
-    uint32_t v[2][NT];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      in[i] = r0 + g + 8 * i < rows;
-      t[i] = in[i] ? __ldg(perm + r0 + g + 8 * i) : 0;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) v[i][j] = 0;
-      if (base != nullptr && in[i] && live) {
-        const T* src = base + t[i] * base_ld + n;
-        if constexpr (NT == 4) {
-          const uint4 q = *reinterpret_cast<const uint4*>(src);
-          v[i][0] = q.x, v[i][1] = q.y, v[i][2] = q.z, v[i][3] = q.w;
-        } else {
-          const uint2 q = *reinterpret_cast<const uint2*>(src);
-          v[i][0] = q.x, v[i][1] = q.y;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < RJ; ++j)
-        hv[i][j] = load_if(in[i] && rank - 32 * j - 8 * c > 0, h + t[i] * h_ld + s * R + 32 * j + 8 * c);
-    }
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    if (step + kWalkStages - 1 < steps) fetch(step + kWalkStages - 1);
+    sa::cp_async_commit();
     float acc[NT][4] = {};
+    if (!none) {
 #pragma unroll
-    for (int j = 0; j < RJ; ++j)
+      for (int j = 0; j < RJ; ++j) {
+        const uint4 lo = sa::ld_v4(h_at(step * 16 + g, 4 * j + c)), hi = sa::ld_v4(h_at(step * 16 + g + 8, 4 * j + c));
 #pragma unroll
-      for (int i = 0; i < NT; ++i) mma_k32<T>(acc[i], hv[0][j], hv[1][j], w[i][j]);
+        for (int i = 0; i < NT; ++i) mma_k32<T>(acc[i], lo, hi, w[i][j]);
+      }
+    }
+    sa::cp_async_wait<kWalkStages - 1>();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (!in[i] || !live) continue;
+      const int r = step * 16 + g + 8 * i;
+      uint32_t v[NT];
+      const uint32_t from = ring + step % kWalkStages * kStage + i * kHalf;
+      if constexpr (NT == 4) {
+        const uint4 q = sa::ld_v4(from);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+      } else {
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(from) : "memory");
+      }
+      if (r >= rows || !live) continue;
       if (!none) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float2 b = unpack2<T>(v[i][j]);
-          v[i][j] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[j][2 * i], b.x), fmaf(scaling, acc[j][2 * i + 1], b.y));
+          const float2 b = unpack2<T>(v[j]);
+          v[j] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[j][2 * i], b.x), fmaf(scaling, acc[j][2 * i + 1], b.y));
         }
       }
-      T* dst = out + t[i] * out_ld + n;
-      if constexpr (NT == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
-      else *reinterpret_cast<uint2*>(dst) = make_uint2(v[i][0], v[i][1]);
+      T* dst = out + row_of[r] * out_ld + n;
+      if constexpr (NT == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
     }
   }
 }
 
 template <typename T>
-int shrink(const T* x, int64_t x_ld, const T* A, PlanView plan, int64_t tokens, int64_t tiles, int64_t K, int R, int slices, T* h,
+int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, int64_t tokens, int64_t tiles, int64_t K, int R, int slices, T* h,
            int64_t h_ld, cudaStream_t st) {
   const int cols = slices * R;
   if (K == 0) {
@@ -635,16 +689,25 @@ int shrink(const T* x, int64_t x_ld, const T* A, PlanView plan, int64_t tokens, 
     return B200_OK;
   }
   if (gemm_sticky_status() != 0) return B200_ERR_DEVICE_TIMEOUT;
-  ShrinkTiles p = {x_ld, K, h_ld, R, slices};
+  ShrinkTiles p = {K, h_ld, R, slices};
   p.status = gemm_status_ptr();
   const int sms = sm_count();
   if (!p.status || sms <= 0) return B200_ERR_CUDA;
+  p.a_box = R % 32 == 0 ? 32 : R % 16 == 0 ? 16 : 8;       // rows of A that are fetched at a time; slices begin at multiples
   p.n_alloc = cols < kMaxColumns ? (cols + 15) / 16 * 16 : kMaxColumns;
   const int passes = (cols + kMaxColumns - 1) / kMaxColumns;
   // As many blocks a tile as give every SM at most one, the tiles being about as many as whole ones.
   p.splits = 1;
   while (p.splits < 8 && 2 * p.splits * passes * ((tokens + kLargeRows - 1) / kLargeRows) <= sms && 2 * p.splits * kBlockK <= K) p.splits *= 2;
-  const size_t smem = 1024 + kTileStages * (kXBytes + static_cast<size_t>(p.n_alloc) * kBlockK * 2);
+  const int stage_bytes = static_cast<int>(kXBytes) + p.n_alloc * kBlockK * 2;
+  p.stages = 200 * 1024 / stage_bytes < kMaxTileStages ? 200 * 1024 / stage_bytes : kMaxTileStages;
+  const size_t smem = 1024 + static_cast<size_t>(p.stages) * stage_bytes;
+  CUtensorMap x1_map, x8_map, x64_map, a_map;
+  int rc = make_map_u16_2d(&x1_map, x, tokens, K, x_ld, 1);
+  if (rc == B200_OK) rc = make_map_u16_2d(&x8_map, x, tokens, K, x_ld, 8);
+  if (rc == B200_OK) rc = make_map_u16_2d(&x64_map, x, tokens, K, x_ld, 64);
+  if (rc == B200_OK) rc = make_map_u16_2d(&a_map, A, static_cast<int64_t>(adapters) * cols, K, K, p.a_box);
+  if (rc != B200_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -658,7 +721,9 @@ int shrink(const T* x, int64_t x_ld, const T* A, PlanView plan, int64_t tokens, 
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_tiles_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, lora_shrink_tiles_kernel<T>, x, A, plan, h, static_cast<const ShrinkTiles&>(p)));
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, lora_shrink_tiles_kernel<T>, static_cast<const CUtensorMap&>(x1_map),
+                                   static_cast<const CUtensorMap&>(x8_map), static_cast<const CUtensorMap&>(x64_map),
+                                   static_cast<const CUtensorMap&>(a_map), plan, h, static_cast<const ShrinkTiles&>(p)));
   return B200_OK;
 }
 
@@ -671,15 +736,16 @@ int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* 
   static_assert(kExpandThreads == kWalkThreads, "one grid for both");
   constexpr int kWarps = kExpandThreads / 32;
   const dim3 grid(static_cast<unsigned>((sl.first_block[sl.n] + kWarps - 1) / kWarps), static_cast<unsigned>(tiles));
-  auto go = [&](auto kern) {
-    return launch_pdl(kern, grid, dim3(kExpandThreads), 0, st, h, h_ld, B, N, R, scalings, plan, sl, base, base_ld, out, out_ld);
+  auto go = [&](auto kern, int smem) -> int {
+    if (smem > 40 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    B200_CUDA_TRY(launch_pdl(kern, grid, dim3(kExpandThreads), smem, st, h, h_ld, B, N, R, scalings, plan, sl, base, base_ld, out, out_ld));
+    return B200_OK;
   };
-  if (tile_rows(tokens) == kSmallRows) B200_CUDA_TRY(go(lora_expand_kernel<T>));
-  else if (R <= 32) B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 1, 4>));
-  else if (R <= 64) B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 2, 4>));
-  else if (R <= 128) B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 4, 4>));
-  else B200_CUDA_TRY(go(lora_expand_tiles_kernel<T, 8, 2>));
-  return B200_OK;
+  if (tile_rows(tokens) == kSmallRows) return go(lora_expand_kernel<T>, 0);
+  if (R <= 32) return go(lora_expand_tiles_kernel<T, 1, 4>, walk_smem<1, 4>());
+  if (R <= 64) return go(lora_expand_tiles_kernel<T, 2, 4>, walk_smem<2, 4>());
+  if (R <= 128) return go(lora_expand_tiles_kernel<T, 4, 4>, walk_smem<4, 4>());
+  return go(lora_expand_tiles_kernel<T, 8, 2>, walk_smem<8, 2>());
 }
 
 int check_plan(const void* plan, size_t bytes, int64_t T, int64_t L) {
@@ -734,9 +800,9 @@ extern "C" int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int 
   const PlanView v = view_plan(plan, T, L);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == B200_DT_BF16)
-    return shrink(static_cast<const __nv_bfloat16*>(x), x_ld, static_cast<const __nv_bfloat16*>(A), v, T, tiles, K, R, num_slices,
+    return shrink(static_cast<const __nv_bfloat16*>(x), x_ld, static_cast<const __nv_bfloat16*>(A), L, v, T, tiles, K, R, num_slices,
                   static_cast<__nv_bfloat16*>(h), h_ld, st);
-  return shrink(static_cast<const __half*>(x), x_ld, static_cast<const __half*>(A), v, T, tiles, K, R, num_slices,
+  return shrink(static_cast<const __half*>(x), x_ld, static_cast<const __half*>(A), L, v, T, tiles, K, R, num_slices,
                 static_cast<__half*>(h), h_ld, st);
 }
 
@@ -749,7 +815,7 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
   if (num_slices <= 0 || !slice_sizes) return num_slices <= 0 ? B200_ERR_BAD_SHAPE : B200_ERR_NULL_PTR;
   if (num_slices > kMaxSlices) return B200_ERR_TOO_LARGE;
   if (dtype != B200_DT_BF16 && dtype != B200_DT_F16) return B200_ERR_BAD_DTYPE;
-  const int warp_cols = expand_columns(T, R);
+  const int warp_cols = expand_columns(T, R), block_cols = tile_rows(T) == kSmallRows ? warp_cols : 4 * warp_cols;
   Slices sl = {};
   sl.n = num_slices;
   int64_t N = 0;
@@ -758,7 +824,7 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
     N += slice_sizes[i];
     if (N > (1 << 30)) return B200_ERR_TOO_LARGE;
     sl.first_col[i + 1] = static_cast<int>(N);
-    sl.first_block[i + 1] = sl.first_block[i] + static_cast<int>((slice_sizes[i] + warp_cols - 1) / warp_cols);
+    sl.first_block[i + 1] = sl.first_block[i] + static_cast<int>((slice_sizes[i] + block_cols - 1) / block_cols) * (block_cols / warp_cols);
   }
   if (h_ld < num_slices * static_cast<int64_t>(R) || h_ld % 8 != 0 || out_ld < N || out_ld % 8 != 0 ||
       (base && (base_ld < N || base_ld % 8 != 0)))

@@ -65,7 +65,7 @@ CASES = [
     (1, 8, [8], 8, 1), (1, 8192, [8192], 16, 4), (2, 64, [64], 16, 3), (7, 72, [72, 8], 8, 2), (8, 1000, [200, 8, 8], 40, 5),
     (9, 256, [128, 0, 64], 24, 3), (16, 4096, [64, 64], 64, 2), (17, 520, [264], 128, 4), (33, 96, [40, 24, 16, 8], 256, 3),
     (129, 1024, [256, 64, 64], 64, 33), (300, 264, [136], 32, 1000), (515, 512, [320, 64, 64], 64, 3), (1000, 2048, [512, 512], 16, 2),
-    (2049, 320, [192], 8, 40), (700, 136, [72, 72], 128, 2), (640, 200, [48, 16], 256, 2),
+    (2049, 320, [192], 8, 40), (700, 136, [72, 72], 128, 2), (640, 200, [48, 16], 256, 2), (513, 8, [32, 8], 72, 2),
 ]
 
 
