@@ -151,8 +151,8 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 32 consecutive k at once: lo and hi are the 16-byte vectors (k = 8c .. 8c + 7, c = lane % 4) of the weight rows lane / 4 and
-// lane / 4 + 8, x the one of token lane / 4.
+// 32 consecutive k at once: lo and hi are the 16-byte vectors (k = 8c .. 8c + 7, c = lane % 4) of rows lane / 4 and lane / 4 + 8
+// of the 16-row operand, x the one of row lane / 4 of the other.
 template <typename T>
 __device__ __forceinline__ void mma_k32(float (&d)[4], const uint4& lo, const uint4& hi, const uint4& x) {
   mma16816<T>(d, lo.x, hi.x, lo.y, hi.y, x.x, x.y);
@@ -408,34 +408,56 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const _
       if (++stage == p.stages) stage = 0, phase ^= 1;
     }
   }
-  // columns [j, j + 8) of token row `row`, packed column c0 + j on
-  auto put = [&](int row, int j, const float* v) {
-    const int s = (c0 + j) / width, r = (c0 + j) % width;
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = pack2(static_cast<T*>(nullptr), r + 2 * i < rank ? v[2 * i] : 0.f, r + 2 * i + 1 < rank ? v[2 * i + 1] : 0.f);
-    *reinterpret_cast<uint4*>(h + plan.perm[tile.y + row] * p.h_ld + s * p.R + r) = make_uint4(w[0], w[1], w[2], w[3]);
-  };
-  float* partial = reinterpret_cast<float*>(dyn + (ring - smem_u32(dyn)));       // [columns][128], where the ring was
   if (ok) ok = warp_wait(done, 0, p.status, 53);
   tc_fence_after();
-  {
-    const int row = warp * 32 + lane;
-    for (int j = 0; j < n16; j += 16) {
-      float v[16];
-      tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + j, v);
-      tmem_ld_wait();
-      if (p.splits == 1) {
-        if (ok && row < rows) {
-          put(row, j, v);
-          if (j + 8 < n) put(row, j + 8, v + 8);
-        }
-      } else {
+  const uint32_t mine = tmem + (static_cast<uint32_t>(warp * 32) << 16);         // this thread's row of the sums
+  const int row = threadIdx.x;
+  // Each block of the cluster adds up a share of the columns, in groups of eight: the others' sums of them arrive in its shared
+  // memory, where the ring was, as [block][column][row].
+  const int groups = n / 8, share = (groups + p.splits - 1) / p.splits;
+  const int g0 = split * share, g1 = min(g0 + share, groups);
+  float* recv = reinterpret_cast<float*>(dyn + (ring - smem_u32(dyn))) + row;
+  if (p.splits > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();                                             // nobody's ring is in use any more
+    for (int b = 1; b < p.splits; ++b) {
+      const int to = (split + b) % p.splits;
+      float* theirs = cluster.map_shared_rank(recv, to) + split * share * (8 * kLargeRows);
+      for (int q = to * share; q < min(to * share + share, groups); ++q) {
+        float v[8];
+        tmem_ld8(mine + 8 * q, v);
+        tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) partial[(j + i) * kLargeRows + row] = v[i];
+        for (int i = 0; i < 8; ++i) theirs[((q - to * share) * 8 + i) * kLargeRows] = v[i];
       }
     }
+    cluster.sync();
+  }
+  const int64_t token = row < rows ? plan.perm[tile.y + row] : -1;
+  int s = (c0 + 8 * g0) / width, r = (c0 + 8 * g0) % width;
+  for (int q = g0; q < g1; ++q) {
+    float v[8];
+    tmem_ld8(mine + 8 * q, v);
+    tmem_ld_wait();
+    // in the order of the blocks, whoever adds
+    if (p.splits > 1) {
+      float sum[8] = {};
+      for (int b = 0; b < p.splits; ++b) {
+        const float* part = recv + (b * share + q - g0) * (8 * kLargeRows);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += b == split ? v[i] : part[i * kLargeRows];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = sum[i];
+    }
+    if (ok && token >= 0) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = pack2(static_cast<T*>(nullptr), r + 2 * i < rank ? v[2 * i] : 0.f, r + 2 * i + 1 < rank ? v[2 * i + 1] : 0.f);
+      *reinterpret_cast<uint4*>(h + token * p.h_ld + s * p.R + r) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if ((r += 8) == width) r = 0, ++s;
   }
   tc_fence_before();
   __syncthreads();
@@ -443,22 +465,6 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const _
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
   }
-  if (p.splits == 1) return;
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  const int share = kLargeRows / p.splits;
-  for (int e = threadIdx.x; e < share * (n / 8); e += kTileThreads) {
-    const int row = split * share + e % share, j = e / share * 8;
-    if (row >= rows) continue;
-    float v[8] = {};
-    for (int b = 0; b < p.splits; ++b) {
-      const float* other = cluster.map_shared_rank(partial, b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += other[(j + i) * kLargeRows + row];
-    }
-    if (*reinterpret_cast<volatile int*>(p.status) == 0) put(row, j, v);
-  }
-  cluster.sync();
 }
 
 // ------------------------------------------------------------------------------------------------------- expand
@@ -482,10 +488,10 @@ constexpr int kExpandThreads = 128;
 // operands is column 8 (lane / 4) + 2 i + f, so that the eight sums that a lane holds for a token are neighbours: base and out
 // move 16 bytes at a time.
 template <typename T>
-__global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* __restrict__ h, int64_t h_ld, const T* __restrict__ B,
+__global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* __restrict__ h, int h_ld, const T* __restrict__ B,
                                                                      int64_t N, int R, const float* __restrict__ scalings,
                                                                      PlanView plan, const __grid_constant__ Slices sl,
-                                                                     const T* base, int64_t base_ld, T* out, int64_t out_ld) {
+                                                                     const T* base, int base_ld, T* out, int out_ld) {
   pdl_start();
   if (static_cast<int>(blockIdx.y) >= plan.count[0]) return;
   const int4 tile = plan.tiles[blockIdx.y];
@@ -521,7 +527,7 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* __
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         w[i] = load_if(live && keep > 0, bp + i * R + r0);
-        if (keep < 8) w[i] = first_of(w[i], keep);
+        if (keep > 0 && keep < 8) w[i] = first_of(w[i], keep);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -562,10 +568,10 @@ template <int RJ, int NT>
 constexpr int walk_smem() { return kLargeRows * RJ * 64 + kWalkThreads * kWalkStages * 2 * NT * 4; }
 
 template <typename T, int RJ, int NT>
-__global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T* __restrict__ h, int64_t h_ld, const T* __restrict__ B,
+__global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T* __restrict__ h, int h_ld, const T* __restrict__ B,
                                                                          int64_t N, int R, const float* __restrict__ scalings,
                                                                          PlanView plan, const __grid_constant__ Slices sl,
-                                                                         const T* base, int64_t base_ld, T* out, int64_t out_ld) {
+                                                                         const T* base, int base_ld, T* out, int out_ld) {
   pdl_start();
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ int row_of[kLargeRows];
@@ -605,7 +611,7 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
     for (int e = threadIdx.x; e < kLargeRows * RJ * 4; e += kWalkThreads) {
       const int row = e / (RJ * 4), v = e % (RJ * 4);
       const bool in = row < rows && v * 8 < rank;
-      sa::cp_async16(h_at(row, v), h + (in ? row_of[row] * h_ld + s * R + v * 8 : 0), in);
+      sa::cp_async16(h_at(row, v), h + (in ? static_cast<int64_t>(row_of[row]) * h_ld + s * R + v * 8 : 0), in);
     }
   }
   auto fetch = [&](int step) {
@@ -613,7 +619,7 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
     for (int i = 0; i < 2; ++i) {
       const int r = step * 16 + g + 8 * i;
       const bool in = base != nullptr && r < rows && live;
-      const T* src = in ? base + row_of[r] * base_ld + n : h;
+      const T* src = in ? base + static_cast<int64_t>(row_of[r]) * base_ld + n : h;
       const uint32_t to = ring + step % kWalkStages * kStage + i * kHalf;
       if constexpr (NT == 4) sa::cp_async16(to, src, in);
       else sa::cp_async8(to, src, in);
@@ -633,7 +639,7 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
 #pragma unroll
     for (int j = 0; j < RJ; ++j) {
       const int keep = rank - 32 * j - 8 * c;
-      if (keep < 8) w[i][j] = first_of(w[i][j], keep);
+      if (keep > 0 && keep < 8) w[i][j] = first_of(w[i][j], keep);
     }
 #pragma unroll 1
   for (int step = 0; step < steps; ++step) {
@@ -643,6 +649,7 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
     if (!none) {
 #pragma unroll
       for (int j = 0; j < RJ; ++j) {
+        if (32 * j >= rank) break;                           // the same for the whole block
         const uint4 lo = sa::ld_v4(h_at(step * 16 + g, 4 * j + c)), hi = sa::ld_v4(h_at(step * 16 + g + 8, 4 * j + c));
 #pragma unroll
         for (int i = 0; i < NT; ++i) mma_k32<T>(acc[i], lo, hi, w[i][j]);
@@ -664,11 +671,11 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
       if (!none) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float2 b = unpack2<T>(v[j]);
-          v[j] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[j][2 * i], b.x), fmaf(scaling, acc[j][2 * i + 1], b.y));
+          const float2 y = __ffma2_rn(make_float2(scaling, scaling), make_float2(acc[j][2 * i], acc[j][2 * i + 1]), unpack2<T>(v[j]));
+          v[j] = pack2(static_cast<T*>(nullptr), y.x, y.y);
         }
       }
-      T* dst = out + row_of[r] * out_ld + n;
+      T* dst = out + static_cast<int64_t>(row_of[r]) * out_ld + n;
       if constexpr (NT == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
       else *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
     }
@@ -738,7 +745,8 @@ int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* 
   const dim3 grid(static_cast<unsigned>((sl.first_block[sl.n] + kWarps - 1) / kWarps), static_cast<unsigned>(tiles));
   auto go = [&](auto kern, int smem) -> int {
     if (smem > 40 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    B200_CUDA_TRY(launch_pdl(kern, grid, dim3(kExpandThreads), smem, st, h, h_ld, B, N, R, scalings, plan, sl, base, base_ld, out, out_ld));
+    B200_CUDA_TRY(launch_pdl(kern, grid, dim3(kExpandThreads), smem, st, h, static_cast<int>(h_ld), B, N, R, scalings, plan, sl, base,
+                             static_cast<int>(base_ld), out, static_cast<int>(out_ld)));
     return B200_OK;
   };
   if (tile_rows(tokens) == kSmallRows) return go(lora_expand_kernel<T>, 0);
@@ -829,6 +837,7 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
   if (h_ld < num_slices * static_cast<int64_t>(R) || h_ld % 8 != 0 || out_ld < N || out_ld % 8 != 0 ||
       (base && (base_ld < N || base_ld % 8 != 0)))
     return B200_ERR_BAD_STRIDE;
+  if (h_ld > 0x7fffffffLL || base_ld > 0x7fffffffLL || out_ld > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
   if (T == 0 || N == 0) return B200_OK;
   if ((rc = check_plan(plan, plan_bytes, T, L)) != B200_OK) return rc;
   if (!h || !B || !scalings || !out) return B200_ERR_NULL_PTR;
