@@ -647,7 +647,7 @@ int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_table, int6
  * tokens without an adapter).  b200_lora_expand: base NULL counts as zeros; out may be base; tokens without an adapter get
  * base.  slice_sizes (host) adds up to N, each a multiple of 8.  dtype (of x, A, h, B, base, out) bf16 or fp16; K and R
  * multiples of 8, R <= 256, at most 8 slices, 1024 adapters and 1000000 tokens; leading dimensions multiples of 8, pointers
- * 16-byte aligned.
+ * 16-byte aligned.  b200_lora_apply is both, h being scratch of num_tokens * num_slices * R elements.
  */
 size_t b200_lora_plan_bytes(int64_t num_tokens, int num_adapters);
 int b200_lora_plan(const int32_t* token_adapters, int64_t num_tokens, const int32_t* ranks, int num_adapters, void* plan,
@@ -658,6 +658,9 @@ int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int dtype, cons
 int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes,
                      const float* scalings, int64_t num_tokens, int num_adapters, int R, const int64_t* slice_sizes,
                      int num_slices, const void* base, int64_t base_ld, void* out, int64_t out_ld, void* stream);
+int b200_lora_apply(const void* x, int64_t x_ld, const void* A, const void* B, int dtype, const void* plan, size_t plan_bytes,
+                    const float* scalings, int64_t num_tokens, int num_adapters, int64_t K, int R, const int64_t* slice_sizes,
+                    int num_slices, const void* base, int64_t base_ld, void* out, int64_t out_ld, void* h, void* stream);
 
 /*
  * Device-side waits in the GEMM kernels are bounded (about a second of SM clocks).  A wait that gives up

@@ -148,6 +148,9 @@ _SIGNATURES = {
                                  c_int, c_void_p, c_int64, c_void_p]),
     "b200_lora_expand": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, ctypes.c_size_t, c_void_p, c_int64, c_int, c_int,
                                  ctypes.POINTER(c_int64), c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "b200_lora_apply": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, ctypes.c_size_t, c_void_p, c_int64, c_int,
+                                c_int64, c_int, ctypes.POINTER(c_int64), c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                c_void_p]),
 }
 
 

@@ -170,30 +170,29 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int keep) {
 }
 
 // ------------------------------------------------------------------------------------------------------- shrink
-constexpr int kShrinkThreads = 128, kShrinkCluster = 8;
+constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
 
-// A cluster of eight blocks computes 16 columns of h for one tile of up to 16 tokens, its 32 warps dividing K; the partial
+// A cluster of up to eight blocks computes 16 columns of h for one tile of up to 16 tokens, all its warps dividing K; the partial
 // sums are added in a fixed order, first over a block's warps, then over the blocks through distributed shared memory.
 template <typename T>
-__global__ void __cluster_dims__(kShrinkCluster, 1, 1) __launch_bounds__(kShrinkThreads)
-lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ A, int64_t K, int R, int cols,
-                   PlanView plan, T* __restrict__ h, int64_t h_ld) {
+__global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ A,
+                                                                     int64_t K, int R, int cols, PlanView plan,
+                                                                     T* __restrict__ h, int64_t h_ld) {
   pdl_start();
-  __shared__ float part[kShrinkThreads / 32][256];
+  __shared__ float part[kShrinkWarps][256];
   __shared__ float mine[256];
-  if (static_cast<int>(blockIdx.y) >= plan.count[0]) return;        // the whole cluster leaves together
-  const int4 tile = plan.tiles[blockIdx.y];
-  const int c0 = blockIdx.z * 16;
-  if (tile.x < 0) {                                                 // tokens without an adapter: zeros
-    if (blockIdx.x == 0)
-      for (int e = threadIdx.x; e < 256; e += kShrinkThreads)
-        if (e / 16 < tile.z && c0 + e % 16 < cols)
-          h[static_cast<int64_t>(plan.perm[tile.y + e / 16]) * h_ld + c0 + e % 16] = static_cast<T>(0.f);
+  const int tiles = plan.count[0];
+  const int4 tile = plan.tiles[blockIdx.y];                          // in bounds whether or not it is one
+  if (static_cast<int>(blockIdx.y) >= tiles) return;                 // the whole cluster leaves together, here and below
+  const int c0 = blockIdx.z * 16, splits = gridDim.x;
+  const int rows = tile.z, rank = tile.x < 0 ? 0 : min(tile.w, R);
+  if (c0 % R >= rank && (c0 + 8 >= cols || (c0 + 8) % R >= rank)) {  // behind the rank (R % 8 == 0), or no adapter: zeros
+    if (blockIdx.x == 0 && static_cast<int>(threadIdx.x) / 16 < rows && c0 + static_cast<int>(threadIdx.x) % 16 < cols)
+      h[static_cast<int64_t>(plan.perm[tile.y + threadIdx.x / 16]) * h_ld + c0 + threadIdx.x % 16] = static_cast<T>(0.f);
     return;
   }
-  const int rank = min(tile.w, R);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
-  const int rows = tile.z;
+  const int r0 = __ldg(plan.perm + tile.y + min(g, rows - 1)), r1 = __ldg(plan.perm + tile.y + min(g + 8, rows - 1));
   const T* wp[2];
   bool wok[2];
 #pragma unroll
@@ -202,27 +201,25 @@ lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ 
     wok[i] = col < cols && col % R < rank;
     wp[i] = A + (static_cast<int64_t>(tile.x) * cols + col) * K + 8 * c;
   }
-  const T* xp[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = g + 8 * i;
-    xp[i] = r < rows ? x + static_cast<int64_t>(__ldg(plan.perm + tile.y + r)) * x_ld + 8 * c : nullptr;
-  }
   const bool both = rows > 8;
   float acc[2][4] = {};
-  const int64_t chunks = (K + 31) / 32;
-  const int64_t per = (chunks + kShrinkCluster * (kShrinkThreads / 32) - 1) / (kShrinkCluster * (kShrinkThreads / 32));
-  const int64_t begin = (blockIdx.x * (kShrinkThreads / 32) + warp) * per, end = begin + per < chunks ? begin + per : chunks;
-  for (int64_t i = begin; i < end; i += 4) {
+  const int chunks = static_cast<int>((K + 31) / 32), per = (chunks + splits * kShrinkWarps - 1) / (splits * kShrinkWarps);
+  const int begin = (blockIdx.x * kShrinkWarps + warp) * per, end = min(begin + per, chunks);
+  for (int i = begin; i < end; i += 4) {
     uint4 w0[4], w1[4], x0[4], x1[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t k = (i + u) * 32;
+    for (int u = 0; u < 4; ++u) {                                    // the weights first: x waits for the plan's rows
+      const int64_t k = static_cast<int64_t>(i + u) * 32;
       const bool in = i + u < end && k + 8 * c < K;
       w0[u] = load_if(in && wok[0], wp[0] + k);
       w1[u] = load_if(in && wok[1], wp[1] + k);
-      x0[u] = load_if(in && xp[0] != nullptr, xp[0] + k);
-      x1[u] = load_if(both && in && xp[1] != nullptr, xp[1] + k);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t k = static_cast<int64_t>(i + u) * 32 + 8 * c;
+      const bool in = i + u < end && k < K;
+      x0[u] = load_if(in && g < rows, x + r0 * x_ld + k);
+      x1[u] = load_if(both && in && g + 8 < rows, x + r1 * x_ld + k);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -236,24 +233,28 @@ lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ 
 #pragma unroll
     for (int j = 0; j < 4; ++j) part[warp][(8 * i + 2 * c + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[i][j];
   __syncthreads();
-  for (int e = threadIdx.x; e < 256; e += kShrinkThreads) {
-    float s = 0.f;
+  float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kShrinkThreads / 32; ++w) s += part[w][e];
-    mine[e] = s;
+  for (int w = 0; w < kShrinkWarps; ++w) sum += part[w][threadIdx.x];
+  int e = threadIdx.x;
+  if (splits > 1) {
+    mine[e] = sum;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int share = 256 / splits;
+    e = static_cast<int>(blockIdx.x) * share + threadIdx.x;
+    sum = 0.f;
+    if (static_cast<int>(threadIdx.x) < share) {
+#pragma unroll 8
+      for (int b = 0; b < splits; ++b) sum += *cluster.map_shared_rank(mine + e, b);
+    } else {
+      e = 256;
+    }
+    cluster.sync();
   }
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  if (threadIdx.x < 256 / kShrinkCluster) {
-    const int e = static_cast<int>(cluster.block_rank()) * (256 / kShrinkCluster) + threadIdx.x;
-    float s = 0.f;
-#pragma unroll
-    for (int b = 0; b < kShrinkCluster; ++b) s += *cluster.map_shared_rank(mine + e, b);
-    const int row = e / 16, col = c0 + e % 16;
-    if (row < rows && col < cols)
-      h[static_cast<int64_t>(plan.perm[tile.y + row]) * h_ld + col] = static_cast<T>(col % R < rank ? s : 0.f);
-  }
-  cluster.sync();
+  const int row = e / 16, col = c0 + e % 16;
+  if (row < rows && col < cols)
+    h[static_cast<int64_t>(plan.perm[tile.y + row]) * h_ld + col] = static_cast<T>(col % R < rank ? sum : 0.f);
 }
 
 // A cluster of `splits` blocks computes up to n_alloc columns of h for one tile of up to 128 tokens, each block a part of K.
@@ -487,75 +488,83 @@ constexpr int kExpandThreads = 128;
 // A warp: 64 columns of one slice for one tile of up to 16 tokens.  Weight row (tile i, half f, lane / 4) of its four 16-row
 // operands is column 8 (lane / 4) + 2 i + f, so that the eight sums that a lane holds for a token are neighbours: base and out
 // move 16 bytes at a time.
+// early: the shrink before it is this library's own, launched in the same call, and triggered after its wait; what was there
+// before the shrink (the plan, B and base) may then be read ahead of the wait, which only h has to be behind.
 template <typename T>
-__global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* __restrict__ h, int h_ld, const T* __restrict__ B,
-                                                                     int64_t N, int R, const float* __restrict__ scalings,
+__global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h, int h_ld, const T* __restrict__ B, int64_t N, int R, const float* __restrict__ scalings,
                                                                      PlanView plan, const __grid_constant__ Slices sl,
-                                                                     const T* base, int base_ld, T* out, int out_ld) {
-  pdl_start();
-  if (static_cast<int>(blockIdx.y) >= plan.count[0]) return;
-  const int4 tile = plan.tiles[blockIdx.y];
+                                                                     const T* base, int base_ld, T* out, int out_ld, bool early) {
+  if (!early) pdl_wait();
+  const int tiles = plan.count[0];
+  const int4 tile = plan.tiles[blockIdx.y];                  // in bounds whether or not it is one
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
   const int block = blockIdx.x * (kExpandThreads / 32) + warp;
-  if (block >= sl.first_block[sl.n]) return;
+  const int rows = tile.z;
+  const bool none = tile.x < 0;
+  if (static_cast<int>(blockIdx.y) >= tiles || block >= sl.first_block[sl.n] || (none && base == out)) {
+    if (early) pdl_wait();                                   // no block ends before the shrink has: what follows relies on it
+    return;
+  }
   int s = 0;
 #pragma unroll
   for (int i = 1; i < kMaxSlices; ++i) s += i < sl.n && block >= sl.first_block[i];
   const int n = sl.first_col[s] + (block - sl.first_block[s]) * 64 + 8 * g;   // the first of this lane's eight columns
   const bool live = n < sl.first_col[s + 1];
-  const int rows = tile.z;
-  const bool none = tile.x < 0;
-  if (none && base == out) return;
   const bool both = rows > 8;
+  const int* perm = plan.perm + tile.y;
+  const int h_row[2] = {__ldg(perm + min(g, rows - 1)), __ldg(perm + min(g + 8, rows - 1))};
+  int token[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) token[i] = __ldg(perm + min(8 * (i / 2) + 2 * c + i % 2, rows - 1));
+  const int rank = none ? 0 : min(tile.w, R);
+  const float scaling = none ? 0.f : __ldg(scalings + tile.x);
+  const T* bp = B + (static_cast<int64_t>(tile.x) * N + n) * R + 8 * c;
+  auto load_b = [&](uint4 (&w)[8], int r0) {
+    const int keep = rank - r0 - 8 * c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = load_if(live && keep > 0, bp + i * R + r0);
+    if (keep > 0 && keep < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = first_of(w[i], keep);
+    }
+  };
+  uint4 w[8], v[4];
+  load_b(w, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = base != nullptr && live && 8 * (i / 2) + 2 * c + i % 2 < rows
+               ? *reinterpret_cast<const uint4*>(base + static_cast<int64_t>(token[i]) * base_ld + n) : make_uint4(0, 0, 0, 0);
+  if (early) pdl_wait();
+  pdl_trigger();
   float acc[2][4][4] = {};
-  float scaling = 0.f;
-  if (!none) {
-    const int rank = min(tile.w, R);
-    scaling = __ldg(scalings + tile.x);
-    const T* bp = B + (static_cast<int64_t>(tile.x) * N + n) * R + 8 * c;
-    const T* hp[2];
+  const T* hp[2] = {h + static_cast<int64_t>(h_row[0]) * h_ld + s * R + 8 * c, h + static_cast<int64_t>(h_row[1]) * h_ld + s * R + 8 * c};
+#pragma unroll 1
+  for (int r0 = 0; r0 < rank; r0 += 32) {
+    const bool in = rank - r0 - 8 * c > 0;
+    uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;              // coherent loads: h may be written while this kernel is resident
+    if (in && g < rows) x0 = __ldcg(reinterpret_cast<const uint4*>(hp[0] + r0));
+    if (in && g + 8 < rows) x1 = __ldcg(reinterpret_cast<const uint4*>(hp[1] + r0));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = g + 8 * i;
-      hp[i] = r < rows ? h + static_cast<int64_t>(__ldg(plan.perm + tile.y + r)) * h_ld + s * R + 8 * c : nullptr;
+    for (int i = 0; i < 4; ++i) {
+      mma_k32<T>(acc[0][i], w[2 * i], w[2 * i + 1], x0);
+      if (both) mma_k32<T>(acc[1][i], w[2 * i], w[2 * i + 1], x1);
     }
-    for (int r0 = 0; r0 < rank; r0 += 32) {
-      const int keep = rank - r0 - 8 * c;
-      const uint4 x0 = load_if(keep > 0 && hp[0] != nullptr, hp[0] + r0);
-      const uint4 x1 = load_if(both && keep > 0 && hp[1] != nullptr, hp[1] + r0);
-      uint4 w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = load_if(live && keep > 0, bp + i * R + r0);
-        if (keep > 0 && keep < 8) w[i] = first_of(w[i], keep);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mma_k32<T>(acc[0][i], w[2 * i], w[2 * i + 1], x0);
-        if (both) mma_k32<T>(acc[1][i], w[2 * i], w[2 * i + 1], x1);
-      }
-    }
+    if (r0 + 32 < rank) load_b(w, r0 + 32);
   }
   if (!live) return;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 4; ++i) {
+    if (8 * (i / 2) + 2 * c + i % 2 >= rows) continue;
+    if (!none) {
+      uint32_t* q = &v[i].x;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = 8 * i + 2 * c + j;
-      if (r >= rows) continue;
-      const int64_t t = __ldg(plan.perm + tile.y + r);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (base != nullptr) v = *reinterpret_cast<const uint4*>(base + t * base_ld + n);
-      if (!none) {
-        uint32_t* w = &v.x;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const float2 b = unpack2<T>(w[m]);
-          w[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[i][m][j], b.x), fmaf(scaling, acc[i][m][j + 2], b.y));
-        }
+      for (int m = 0; m < 4; ++m) {
+        const float2 b = unpack2<T>(q[m]);
+        q[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[i / 2][m][i % 2], b.x), fmaf(scaling, acc[i / 2][m][i % 2 + 2], b.y));
       }
-      *reinterpret_cast<uint4*>(out + t * out_ld + n) = v;
     }
+    *reinterpret_cast<uint4*>(out + static_cast<int64_t>(token[i]) * out_ld + n) = v[i];
+  }
 }
 
 // Tiles of up to 128 tokens: a warp holds the B of NT x 8 columns of one slice in registers (tokens are the 16-row operand here)
@@ -682,24 +691,46 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
   }
 }
 
+// launch_pdl with clusters of `blocks` blocks along x.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, int blocks, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = blocks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
 template <typename T>
 int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, int64_t tokens, int64_t tiles, int64_t K, int R, int slices, T* h,
            int64_t h_ld, cudaStream_t st) {
-  const int cols = slices * R;
+  const int cols = slices * R, sms = sm_count();
+  if (sms <= 0) return B200_ERR_CUDA;
   if (K == 0) {
     B200_CUDA_TRY(cudaMemset2DAsync(h, h_ld * sizeof(T), 0, cols * sizeof(T), tokens, st));
     return B200_OK;
   }
   if (tile_rows(tokens) == kSmallRows) {
-    const dim3 grid(kShrinkCluster, static_cast<unsigned>(tiles), static_cast<unsigned>((cols + 15) / 16));
-    B200_CUDA_TRY(launch_pdl(lora_shrink_kernel<T>, grid, dim3(kShrinkThreads), 0, st, x, x_ld, A, K, R, cols, plan, h, h_ld));
+    // Enough blocks for two on every SM, if K has a k32 step for each of their warps.
+    const int passes = (cols + 15) / 16;
+    int splits = 1;
+    while (splits < 8 && tiles * passes * splits < 2LL * sms && splits * 32 * kShrinkWarps < K) splits *= 2;
+    B200_CUDA_TRY(launch_cluster(lora_shrink_kernel<T>, dim3(splits, static_cast<unsigned>(tiles), passes), dim3(kShrinkThreads), 0, splits,
+                                 st, x, x_ld, A, K, R, cols, plan, h, h_ld));
     return B200_OK;
   }
   if (gemm_sticky_status() != 0) return B200_ERR_DEVICE_TIMEOUT;
   ShrinkTiles p = {K, h_ld, R, slices};
   p.status = gemm_status_ptr();
-  const int sms = sm_count();
-  if (!p.status || sms <= 0) return B200_ERR_CUDA;
+  if (!p.status) return B200_ERR_CUDA;
   p.a_box = R % 32 == 0 ? 32 : R % 16 == 0 ? 16 : 8;       // rows of A that are fetched at a time; slices begin at multiples
   p.n_alloc = cols < kMaxColumns ? (cols + 15) / 16 * 16 : kMaxColumns;
   const int passes = (cols + kMaxColumns - 1) / kMaxColumns;
@@ -715,22 +746,9 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
   if (rc == B200_OK) rc = make_map_u16_2d(&x64_map, x, tokens, K, x_ld, 64);
   if (rc == B200_OK) rc = make_map_u16_2d(&a_map, A, static_cast<int64_t>(adapters) * cols, K, K, p.a_box);
   if (rc != B200_OK) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.splits, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(p.splits, static_cast<unsigned>(tiles), passes);
-  cfg.blockDim = dim3(kTileThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
   B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_tiles_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, lora_shrink_tiles_kernel<T>, static_cast<const CUtensorMap&>(x1_map),
-                                   static_cast<const CUtensorMap&>(x8_map), static_cast<const CUtensorMap&>(x64_map),
-                                   static_cast<const CUtensorMap&>(a_map), plan, h, static_cast<const ShrinkTiles&>(p)));
+  B200_CUDA_TRY(launch_cluster(lora_shrink_tiles_kernel<T>, dim3(p.splits, static_cast<unsigned>(tiles), passes), dim3(kTileThreads), smem,
+                               p.splits, st, x1_map, x8_map, x64_map, a_map, plan, h, p));
   return B200_OK;
 }
 
@@ -739,17 +757,17 @@ int expand_columns(int64_t tokens, int R) { return tile_rows(tokens) == kSmallRo
 
 template <typename T>
 int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* scalings, PlanView plan, const Slices& sl, int64_t tokens,
-           int64_t tiles, const T* base, int64_t base_ld, T* out, int64_t out_ld, cudaStream_t st) {
+           int64_t tiles, const T* base, int64_t base_ld, T* out, int64_t out_ld, bool early, cudaStream_t st) {
   static_assert(kExpandThreads == kWalkThreads, "one grid for both");
   constexpr int kWarps = kExpandThreads / 32;
   const dim3 grid(static_cast<unsigned>((sl.first_block[sl.n] + kWarps - 1) / kWarps), static_cast<unsigned>(tiles));
-  auto go = [&](auto kern, int smem) -> int {
+  auto go = [&](auto kern, int smem, auto... more) -> int {
     if (smem > 40 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     B200_CUDA_TRY(launch_pdl(kern, grid, dim3(kExpandThreads), smem, st, h, static_cast<int>(h_ld), B, N, R, scalings, plan, sl, base,
-                             static_cast<int>(base_ld), out, static_cast<int>(out_ld)));
+                             static_cast<int>(base_ld), out, static_cast<int>(out_ld), more...));
     return B200_OK;
   };
-  if (tile_rows(tokens) == kSmallRows) return go(lora_expand_kernel<T>, 0);
+  if (tile_rows(tokens) == kSmallRows) return go(lora_expand_kernel<T>, 0, early);
   if (R <= 32) return go(lora_expand_tiles_kernel<T, 1, 4>, walk_smem<1, 4>());
   if (R <= 64) return go(lora_expand_tiles_kernel<T, 2, 4>, walk_smem<2, 4>());
   if (R <= 128) return go(lora_expand_tiles_kernel<T, 4, 4>, walk_smem<4, 4>());
@@ -790,9 +808,11 @@ extern "C" int b200_lora_plan(const int32_t* token_adapters, int64_t T, const in
   return B200_OK;
 }
 
-extern "C" int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int dtype, const void* plan, size_t plan_bytes,
-                                int64_t T, int L, int64_t K, int R, int num_slices, void* h, int64_t h_ld, void* stream) {
-  using namespace b200;
+namespace b200 {
+namespace {
+
+int shrink_entry(const void* x, int64_t x_ld, const void* A, int dtype, const void* plan, size_t plan_bytes, int64_t T, int L,
+                 int64_t K, int R, int num_slices, void* h, int64_t h_ld, void* stream) {
   int rc = check_sizes(T, L, R);
   if (rc != B200_OK) return rc;
   if (num_slices <= 0 || K < 0 || K % 8 != 0) return B200_ERR_BAD_SHAPE;
@@ -814,10 +834,10 @@ extern "C" int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int 
                 static_cast<__half*>(h), h_ld, st);
 }
 
-extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes,
-                                const float* scalings, int64_t T, int L, int R, const int64_t* slice_sizes, int num_slices,
-                                const void* base, int64_t base_ld, void* out, int64_t out_ld, void* stream) {
-  using namespace b200;
+// check_only: the arguments are looked at, nothing is launched.
+int expand_entry(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes, const float* scalings,
+                 int64_t T, int L, int R, const int64_t* slice_sizes, int num_slices, const void* base, int64_t base_ld, void* out,
+                 int64_t out_ld, bool early, bool check_only, void* stream) {
   int rc = check_sizes(T, L, R);
   if (rc != B200_OK) return rc;
   if (num_slices <= 0 || !slice_sizes) return num_slices <= 0 ? B200_ERR_BAD_SHAPE : B200_ERR_NULL_PTR;
@@ -829,8 +849,8 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
   int64_t N = 0;
   for (int i = 0; i < num_slices; ++i) {
     if (slice_sizes[i] < 0 || slice_sizes[i] % 8 != 0) return B200_ERR_BAD_SHAPE;
+    if (slice_sizes[i] > (1 << 30) || N + slice_sizes[i] > (1 << 30)) return B200_ERR_TOO_LARGE;
     N += slice_sizes[i];
-    if (N > (1 << 30)) return B200_ERR_TOO_LARGE;
     sl.first_col[i + 1] = static_cast<int>(N);
     sl.first_block[i + 1] = sl.first_block[i] + static_cast<int>((slice_sizes[i] + block_cols - 1) / block_cols) * (block_cols / warp_cols);
   }
@@ -842,12 +862,43 @@ extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int 
   if ((rc = check_plan(plan, plan_bytes, T, L)) != B200_OK) return rc;
   if (!h || !B || !scalings || !out) return B200_ERR_NULL_PTR;
   if (!aligned16(h) || !aligned16(B) || !aligned16(base) || !aligned16(out)) return B200_ERR_MISALIGNED;
+  if (check_only) return B200_OK;
   const int64_t tiles = max_tiles(T, L);
   const PlanView v = view_plan(plan, T, L);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == B200_DT_BF16)
     return expand(static_cast<const __nv_bfloat16*>(h), h_ld, static_cast<const __nv_bfloat16*>(B), N, R, scalings, v, sl, T, tiles,
-                  static_cast<const __nv_bfloat16*>(base), base_ld, static_cast<__nv_bfloat16*>(out), out_ld, st);
+                  static_cast<const __nv_bfloat16*>(base), base_ld, static_cast<__nv_bfloat16*>(out), out_ld, early, st);
   return expand(static_cast<const __half*>(h), h_ld, static_cast<const __half*>(B), N, R, scalings, v, sl, T, tiles,
-                static_cast<const __half*>(base), base_ld, static_cast<__half*>(out), out_ld, st);
+                static_cast<const __half*>(base), base_ld, static_cast<__half*>(out), out_ld, early, st);
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int dtype, const void* plan, size_t plan_bytes,
+                                int64_t T, int L, int64_t K, int R, int num_slices, void* h, int64_t h_ld, void* stream) {
+  return b200::shrink_entry(x, x_ld, A, dtype, plan, plan_bytes, T, L, K, R, num_slices, h, h_ld, stream);
+}
+
+extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes,
+                                const float* scalings, int64_t T, int L, int R, const int64_t* slice_sizes, int num_slices,
+                                const void* base, int64_t base_ld, void* out, int64_t out_ld, void* stream) {
+  return b200::expand_entry(h, h_ld, B, dtype, plan, plan_bytes, scalings, T, L, R, slice_sizes, num_slices, base, base_ld, out, out_ld,
+                            false, false, stream);
+}
+
+extern "C" int b200_lora_apply(const void* x, int64_t x_ld, const void* A, const void* B, int dtype, const void* plan,
+                               size_t plan_bytes, const float* scalings, int64_t T, int L, int64_t K, int R,
+                               const int64_t* slice_sizes, int num_slices, const void* base, int64_t base_ld, void* out,
+                               int64_t out_ld, void* h, void* stream) {
+  const int64_t h_ld = static_cast<int64_t>(num_slices) * R;
+  const int rc = b200::expand_entry(h, h_ld, B, dtype, plan, plan_bytes, scalings, T, L, R, slice_sizes, num_slices, base, base_ld, out,
+                                    out_ld, true, true, stream);
+  if (rc != B200_OK) return rc;
+  const int rc2 = b200::shrink_entry(x, x_ld, A, dtype, plan, plan_bytes, T, L, K, R, num_slices, h, h_ld, stream);
+  if (rc2 != B200_OK) return rc2;
+  // with K = 0 there is no kernel before the expand that would make reading ahead sound
+  return b200::expand_entry(h, h_ld, B, dtype, plan, plan_bytes, scalings, T, L, R, slice_sizes, num_slices, base, base_ld, out, out_ld,
+                            K > 0, false, stream);
 }

@@ -506,13 +506,15 @@ HOST_FN(experts) {
 HOST_END
 
 // ---- checked arguments of the functions below
-void need(bool ok, const std::string& message) {
-  if (!ok) throw std::runtime_error(message);
-}
+// The message is put together only for a call that is refused: sixty strings a call took 4 us.
+#define NEED(ok, message)                                        \
+  do {                                                           \
+    if (!(ok)) throw std::runtime_error(std::string() + message); \
+  } while (0)
 const Tensor& tensor_arg(PyObject* o, const char* name) {
-  need(THPVariable_Check(o), std::string(name) + " must be a tensor");
+  NEED(THPVariable_Check(o), std::string(name) + " must be a tensor");
   const Tensor& t = THPVariable_Unpack(o);
-  need(t.defined() && t.layout() == at::kStrided && !t.is_neg() && !t.is_conj() &&
+  NEED(t.defined() && t.layout() == at::kStrided && !t.is_neg() && !t.is_conj() &&
            !t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python),
        std::string(name) + " must be a plain strided tensor");
   return t;
@@ -523,39 +525,39 @@ void need_sizes(const Tensor& t, at::IntArrayRef sizes, const char* name) {
   std::string want, got;
   for (const int64_t n : sizes) want += (want.empty() ? "" : ", ") + std::to_string(n);
   for (const int64_t n : t.sizes()) got += (got.empty() ? "" : ", ") + std::to_string(n);
-  need(false, std::string(name) + " must have shape [" + want + "], got [" + got + "]");
+  NEED(false, std::string(name) + " must have shape [" + want + "], got [" + got + "]");
 }
 void need_type(const Tensor& t, at::ScalarType type, const char* name, const char* what) {
-  need(t.scalar_type() == type, std::string(name) + " must be " + what);
+  NEED(t.scalar_type() == type, std::string(name) + " must be " + what);
 }
 // The stride of a dimension; one that holds at most one element has none, nor has an empty tensor.
 int64_t stride_of(const Tensor& t, int d) { return t.size(d) > 1 && t.numel() > 0 ? t.stride(d) : 0; }
 // The leading dimension of a matrix.
 int64_t ld_of(const Tensor& t) { return stride_of(t, 0) != 0 ? t.stride(0) : t.size(1); }
 void need_rows(const Tensor& t, int64_t multiple, const char* name) {      // the last dimension dense, the others in whole vectors
-  need(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, std::string(name) + " must be contiguous in its last dimension");
+  NEED(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, std::string(name) + " must be contiguous in its last dimension");
   for (int d = 0; d + 1 < t.dim(); ++d)
-    need(stride_of(t, d) % multiple == 0,
+    NEED(stride_of(t, d) % multiple == 0,
          std::string(name) + ": strides must be multiples of " + std::to_string(multiple) + " elements");
 }
 void need_aligned(const Tensor& t, const char* name) {
-  need(!t.defined() || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0, std::string(name) + " must be 16-byte aligned");
+  NEED(!t.defined() || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0, std::string(name) + " must be 16-byte aligned");
 }
 void need_writable(const Tensor& t, const char* name) {     // no two elements in one place
   for (int d = 0; d < t.dim(); ++d)
-    need(t.size(d) <= 1 || t.stride(d) > 0, std::string(name) + " must not be an expanded tensor");
+    NEED(t.size(d) <= 1 || t.stride(d) > 0, std::string(name) + " must not be an expanded tensor");
 }
 void need_index(const Tensor& t, int64_t n, const char* name) {
-  need(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, std::string(name) + " must be int32 or int64");
+  NEED(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, std::string(name) + " must be int32 or int64");
   need_sizes(t, {n}, name);
-  need(n <= 1 || t.stride(0) == 1, std::string(name) + " must be contiguous");
+  NEED(n <= 1 || t.stride(0) == 1, std::string(name) + " must be contiguous");
 }
 at::Device one_device(std::initializer_list<const Tensor*> all) {
   const at::Device dev = (*all.begin())->device();
   for (const Tensor* t : all) {
     if (!t->defined()) continue;
-    need(t->is_cuda(), "all tensors must be CUDA tensors");
-    need(t->device() == dev, "all tensors must be on the same device");
+    NEED(t->is_cuda(), "all tensors must be CUDA tensors");
+    NEED(t->device() == dev, "all tensors must be on the same device");
   }
   return dev;
 }
@@ -567,10 +569,10 @@ struct CacheArgs {
 };
 CacheArgs cache_args(PyObject* const* a) {
   CacheArgs c{tensor_arg(a[0], "k_cache"), tensor_arg(a[1], "v_cache"), tensor_arg(a[2], "k_scale"), tensor_arg(a[3], "v_scale")};
-  need(c.k.dim() == 4, "k_cache must be [num_pages, page_size, num_kv_heads, head_dim]");
+  NEED(c.k.dim() == 4, "k_cache must be [num_pages, page_size, num_kv_heads, head_dim]");
   c.pages = c.k.size(0), c.page = c.k.size(1), c.heads = c.k.size(2), c.dim = c.k.size(3);
-  need(c.page > 0, "the pages of k_cache must hold at least one token");
-  need(c.page < (1LL << 31) && c.pages < (1LL << 31) / c.page, "num_pages * page_size must be below 2^31");
+  NEED(c.page > 0, "the pages of k_cache must hold at least one token");
+  NEED(c.page < (1LL << 31) && c.pages < (1LL << 31) / c.page, "num_pages * page_size must be below 2^31");
   need_type(c.k, at::kFloat8_e4m3fn, "k_cache", "float8_e4m3fn");
   need_type(c.v, at::kFloat8_e4m3fn, "v_cache", "float8_e4m3fn");
   need_type(c.ks, at::kFloat, "k_scale", "float32");
@@ -594,9 +596,9 @@ b200_kv_cache cache_of(const CacheArgs& c) {
   return r;
 }
 void need_heads(const Tensor& t, const char* name) {
-  need(t.dim() == 3, std::string(name) + " must be [num_tokens, num_heads, head_dim]");
-  need(is_16bit(t.scalar_type()), std::string(name) + " must be bfloat16 or float16");
-  need(t.size(2) > 0 && t.size(2) % 16 == 0 && t.size(2) <= 256, "head_dim must be a multiple of 16, at most 256");
+  NEED(t.dim() == 3, std::string(name) + " must be [num_tokens, num_heads, head_dim]");
+  NEED(is_16bit(t.scalar_type()), std::string(name) + " must be bfloat16 or float16");
+  NEED(t.size(2) > 0 && t.size(2) % 16 == 0 && t.size(2) <= 256, "head_dim must be a multiple of 16, at most 256");
   need_rows(t, 8, name);
   need_aligned(t, name);
 }
@@ -604,7 +606,7 @@ void need_heads(const Tensor& t, const char* name) {
 void need_out(const Tensor& t, const Tensor& like, const char* name) {
   need_heads(t, name);
   need_sizes(t, like.sizes(), name);
-  need(t.scalar_type() == like.scalar_type(), std::string(name) + " must have the type of its input");
+  NEED(t.scalar_type() == like.scalar_type(), std::string(name) + " must have the type of its input");
   need_writable(t, name);
 }
 
@@ -624,7 +626,7 @@ PyObject* pair_or_none(Tensor a, Tensor b) {
 // head_rows(name, q | None, k, v | None, positions | None, cos_sin | None, q_weight | None, k_weight | None, norm_eps, is_neox,
 //           q_out | None, k_out | None, want_k, k_cache | None, v_cache, k_scale, v_scale, slots) -> (q_out | None, k_out | None)
 HOST_FN(head_rows) {
-  need(n == 18, "head_rows takes 18 arguments");
+  NEED(n == 18, "head_rows takes 18 arguments");
   const char* name = PyUnicode_AsUTF8(a[0]);
   if (!name) return nullptr;
   const Tensor q = optional_arg(a[1], "q"), k = tensor_arg(a[2], "k"), v = optional_arg(a[3], "v");
@@ -639,34 +641,34 @@ HOST_FN(head_rows) {
   const at::ScalarType type = k.scalar_type();
   if (q.defined()) {
     need_heads(q, "q");
-    need(q.size(0) == T && q.size(2) == D, "q and k must have the same number of tokens and the same head_dim");
-    need(q.scalar_type() == type, "q and k must have the same type");
+    NEED(q.size(0) == T && q.size(2) == D, "q and k must have the same number of tokens and the same head_dim");
+    NEED(q.scalar_type() == type, "q and k must have the same type");
   }
   const int64_t Hq = q.defined() ? q.size(1) : 0;
   if (v.defined()) {
     need_heads(v, "v");
     need_sizes(v, k.sizes(), "v");
-    need(v.scalar_type() == type, "k and v must have the same type");
+    NEED(v.scalar_type() == type, "k and v must have the same type");
   }
   int64_t rot = 0, rows = 0;
   if (cs.defined()) {
-    need(pos.defined(), "positions must be given with cos_sin_cache");
+    NEED(pos.defined(), "positions must be given with cos_sin_cache");
     need_index(pos, T, "positions");
     need_type(cs, at::kFloat, "cos_sin_cache", "float32");
-    need(cs.dim() == 2 && cs.is_contiguous(), "cos_sin_cache must be a contiguous [max_position, rotary_dim] tensor");
+    NEED(cs.dim() == 2 && cs.is_contiguous(), "cos_sin_cache must be a contiguous [max_position, rotary_dim] tensor");
     rows = cs.size(0), rot = cs.size(1);
-    need(rot > 0 && rot % 16 == 0 && rot <= D, "rotary_dim must be a multiple of 16, at most head_dim");
+    NEED(rot > 0 && rot % 16 == 0 && rot <= D, "rotary_dim must be a multiple of 16, at most head_dim");
     need_aligned(cs, "cos_sin_cache");
   }
   for (const auto& [w, what] : {std::pair<const Tensor&, const char*>{qw, "q_weight"}, {kw, "k_weight"}}) {
     if (!w.defined()) continue;
     need_sizes(w, {D}, what);
-    need(w.scalar_type() == type, std::string(what) + " must have the type of k");
-    need(w.is_contiguous(), std::string(what) + " must be contiguous");
+    NEED(w.scalar_type() == type, std::string(what) + " must have the type of k");
+    NEED(w.is_contiguous(), std::string(what) + " must be contiguous");
     need_aligned(w, what);
   }
   if (qo.defined()) {
-    need(q.defined(), "q_out without q");
+    NEED(q.defined(), "q_out without q");
     need_out(qo, q, "q_out");
   }
   if (ko.defined()) need_out(ko, k, "k_out");
@@ -676,8 +678,8 @@ HOST_FN(head_rows) {
   if (store) {
     cache = cache_args(a + 13);
     slots = tensor_arg(a[17], "slots");
-    need(v.defined(), "v must be given with a cache");
-    need(cache.heads == Hkv && cache.dim == D, "the cache must have the heads of k: [num_pages, page_size, num_kv_heads, head_dim]");
+    NEED(v.defined(), "v must be given with a cache");
+    NEED(cache.heads == Hkv && cache.dim == D, "the cache must have the heads of k: [num_pages, page_size, num_kv_heads, head_dim]");
     need_index(slots, T, "slots");
     for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{cache.k, "k_cache"}, {cache.v, "v_cache"}, {cache.ks, "k_scale"}, {cache.vs, "v_scale"}})
       need_writable(t, what);
@@ -719,23 +721,23 @@ HOST_END
 
 // load_kv(k_cache, v_cache, k_scale, v_scale, page_table, indptr, starts | None, num_tokens, dtype, k_out | None, v_out | None)
 HOST_FN(load_kv) {
-  need(n == 11, "load_kv takes 11 arguments");
+  NEED(n == 11, "load_kv takes 11 arguments");
   const CacheArgs cache = cache_args(a);
   const Tensor table = tensor_arg(a[4], "page_table"), indptr = tensor_arg(a[5], "kv_indptr"), starts = optional_arg(a[6], "kv_start");
   const int64_t T = PyLong_AsLongLong(a[7]);
   if (PyErr_Occurred()) return nullptr;
-  need(THPDtype_Check(a[8]), "out_dtype must be a torch.dtype");
+  NEED(THPDtype_Check(a[8]), "out_dtype must be a torch.dtype");
   const at::ScalarType type = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
-  need(is_16bit(type), "out_dtype must be bfloat16 or float16");
-  need(T >= 0, "num_tokens must not be negative");
-  need(cache.dim > 0 && cache.dim % 16 == 0 && cache.dim <= 256, "head_dim must be a multiple of 16, at most 256");
-  need(table.dim() == 2 && table.scalar_type() == at::kInt, "page_table must be an int32 [batch, max_pages] tensor");
-  need(table.size(1) <= 1 || table.stride(1) == 1, "page_table must be contiguous in its last dimension");
+  NEED(is_16bit(type), "out_dtype must be bfloat16 or float16");
+  NEED(T >= 0, "num_tokens must not be negative");
+  NEED(cache.dim > 0 && cache.dim % 16 == 0 && cache.dim <= 256, "head_dim must be a multiple of 16, at most 256");
+  NEED(table.dim() == 2 && table.scalar_type() == at::kInt, "page_table must be an int32 [batch, max_pages] tensor");
+  NEED(table.size(1) <= 1 || table.stride(1) == 1, "page_table must be contiguous in its last dimension");
   const int64_t batch = table.size(0);
-  need(indptr.scalar_type() == at::kInt, "kv_indptr must be int32");
+  NEED(indptr.scalar_type() == at::kInt, "kv_indptr must be int32");
   need_index(indptr, batch + 1, "kv_indptr");
   if (starts.defined()) {
-    need(starts.scalar_type() == at::kInt, "kv_start must be int32");
+    NEED(starts.scalar_type() == at::kInt, "kv_start must be int32");
     need_index(starts, batch, "kv_start");
   }
   Tensor ko = optional_arg(a[9], "k_out"), vo = optional_arg(a[10], "v_out");
@@ -743,7 +745,7 @@ HOST_FN(load_kv) {
     if (!t.defined()) continue;
     need_heads(t, what);
     need_sizes(t, {T, cache.heads, cache.dim}, what);
-    need(t.scalar_type() == type, std::string(what) + " must be of out_dtype");
+    NEED(t.scalar_type() == type, std::string(what) + " must be of out_dtype");
     need_writable(t, what);
   }
   const at::Device dev = one_device({&cache.k, &cache.v, &cache.ks, &cache.vs, &table, &indptr, &starts, &ko, &vo});
@@ -767,20 +769,20 @@ HOST_END
 
 // lora_plan(token_adapters, ranks, plan | None) -> plan, written on the current stream
 HOST_FN(lora_plan) {
-  need(n == 3, "lora_plan takes 3 arguments");
+  NEED(n == 3, "lora_plan takes 3 arguments");
   const Tensor ids = tensor_arg(a[0], "token_adapters"), ranks = tensor_arg(a[1], "lora_ranks");
   Tensor plan = optional_arg(a[2], "plan");
-  need(ids.dim() == 1 && ids.scalar_type() == at::kInt, "token_adapters must be an int32 [num_tokens] tensor");
-  need(ranks.dim() == 1 && ranks.scalar_type() == at::kInt, "lora_ranks must be an int32 [num_adapters] tensor");
-  need(ids.is_contiguous() && ranks.is_contiguous(), "token_adapters and lora_ranks must be contiguous");
+  NEED(ids.dim() == 1 && ids.scalar_type() == at::kInt, "token_adapters must be an int32 [num_tokens] tensor");
+  NEED(ranks.dim() == 1 && ranks.scalar_type() == at::kInt, "lora_ranks must be an int32 [num_adapters] tensor");
+  NEED(ids.is_contiguous() && ranks.is_contiguous(), "token_adapters and lora_ranks must be contiguous");
   const int64_t T = ids.size(0), L = ranks.size(0);
-  need(L > 0 && L <= 1024, "between 1 and 1024 adapters");
-  need(T <= 1000000, "at most 1000000 tokens");
+  NEED(L > 0 && L <= 1024, "between 1 and 1024 adapters");
+  NEED(T <= 1000000, "at most 1000000 tokens");
   const int64_t bytes = static_cast<int64_t>(b200_lora_plan_bytes(T, static_cast<int>(L)));
   if (plan.defined()) {
     need_type(plan, at::kByte, "plan", "uint8");
     need_sizes(plan, {bytes}, "plan");
-    need(plan.is_contiguous(), "plan must be contiguous");
+    NEED(plan.is_contiguous(), "plan must be contiguous");
   }
   const at::Device dev = one_device({&ids, &ranks, &plan});
   int rc;
@@ -800,7 +802,7 @@ HOST_END
 //      scalings, sizes (a tuple of S) | None, num_slices, out | None) -> out [T, N]: shrink and expand; without lora_b only the
 // shrink, which returns h; without x only the expand.
 HOST_FN(lora) {
-  need(n == 11, "lora takes 11 arguments");
+  NEED(n == 11, "lora takes 11 arguments");
   const Tensor base = optional_arg(a[0], "base_output"), x = optional_arg(a[1], "x"), A = optional_arg(a[3], "lora_a"),
                B = optional_arg(a[4], "lora_b"), plan = tensor_arg(a[5], "plan"), scalings = tensor_arg(a[7], "scalings");
   Tensor h = optional_arg(a[2], "h"), out = optional_arg(a[10], "out");
@@ -811,62 +813,62 @@ HOST_FN(lora) {
   at::ScalarType type;
   std::vector<int64_t> sizes;
   if (a[8] != Py_None) {
-    need(PyTuple_Check(a[8]), "output_sizes must be a sequence of integers");
+    NEED(PyTuple_Check(a[8]), "output_sizes must be a sequence of integers");
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[8]); ++i) {
       sizes.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(a[8], i)));
       if (PyErr_Occurred()) return nullptr;
-      need(sizes.back() >= 0 && sizes.back() % 8 == 0, "output_sizes must be multiples of 8");
+      NEED(sizes.back() >= 0 && sizes.back() % 8 == 0, "output_sizes must be multiples of 8");
     }
     S = static_cast<int64_t>(sizes.size());
   }
-  need(S >= 1 && S <= 8, "between 1 and 8 slices");
+  NEED(S >= 1 && S <= 8, "between 1 and 8 slices");
   if (B.defined()) {
-    need(B.dim() == 3 && B.is_contiguous(), "lora_b must be a contiguous [num_adapters, N, R] tensor");
-    need(B.size(0) == L, "lora_b must hold the adapters of the batch");
+    NEED(B.dim() == 3 && B.is_contiguous(), "lora_b must be a contiguous [num_adapters, N, R] tensor");
+    NEED(B.size(0) == L, "lora_b must hold the adapters of the batch");
     N = B.size(1), R = B.size(2);
     if (sizes.empty()) sizes.push_back(N);
     int64_t sum = 0;
     for (const int64_t v : sizes) sum += v;
-    need(sum == N && N % 8 == 0 && static_cast<int64_t>(sizes.size()) == S, "output_sizes must add up to the rows of lora_b, multiples of 8");
+    NEED(sum == N && N % 8 == 0 && static_cast<int64_t>(sizes.size()) == S, "output_sizes must add up to the rows of lora_b, multiples of 8");
     need_aligned(B, "lora_b");
   }
   if (x.defined()) {
-    need(x.dim() == 2 && A.defined(), "x must be [num_tokens, K]");
+    NEED(x.dim() == 2 && A.defined(), "x must be [num_tokens, K]");
     T = x.size(0), K = x.size(1), type = x.scalar_type();
-    need(A.dim() == 3 && A.is_contiguous(), "lora_a must be a contiguous [num_adapters, num_slices * R, K] tensor");
-    need(A.size(0) == L, "lora_a must hold the adapters of the batch");
+    NEED(A.dim() == 3 && A.is_contiguous(), "lora_a must be a contiguous [num_adapters, num_slices * R, K] tensor");
+    NEED(A.size(0) == L, "lora_a must hold the adapters of the batch");
     if (!B.defined()) {
-      need(A.size(1) % S == 0, "the rows of lora_a must be num_slices * R");
+      NEED(A.size(1) % S == 0, "the rows of lora_a must be num_slices * R");
       R = A.size(1) / S;
     }
-    need(A.size(1) == S * R && A.size(2) == K, "lora_a must be [num_adapters, num_slices * R, K]");
-    need(K % 8 == 0, "K must be a multiple of 8");
+    NEED(A.size(1) == S * R && A.size(2) == K, "lora_a must be [num_adapters, num_slices * R, K]");
+    NEED(K % 8 == 0, "K must be a multiple of 8");
     need_rows(x, 8, "x");
     need_aligned(x, "x");
     need_aligned(A, "lora_a");
-    need(A.scalar_type() == type, "lora_a must have the type of x");
+    NEED(A.scalar_type() == type, "lora_a must have the type of x");
   } else {
-    need(h.defined() && B.defined() && h.dim() == 2, "h must be [num_tokens, num_slices * R]");
+    NEED(h.defined() && B.defined() && h.dim() == 2, "h must be [num_tokens, num_slices * R]");
     T = h.size(0), type = h.scalar_type();
     need_sizes(h, {T, S * R}, "h");
     need_rows(h, 8, "h");
     need_aligned(h, "h");
   }
-  need(is_16bit(type), "x must be bfloat16 or float16");
-  need(R > 0 && R % 8 == 0 && R <= 256, "R must be a multiple of 8, at most 256");
-  need(!B.defined() || B.scalar_type() == type, "lora_b must have the type of x");
+  NEED(is_16bit(type), "x must be bfloat16 or float16");
+  NEED(R > 0 && R % 8 == 0 && R <= 256, "R must be a multiple of 8, at most 256");
+  NEED(!B.defined() || B.scalar_type() == type, "lora_b must have the type of x");
   const int64_t bytes = static_cast<int64_t>(b200_lora_plan_bytes(T, static_cast<int>(L)));
-  need(plan.scalar_type() == at::kByte && plan.is_contiguous() && plan.numel() == bytes, "the batch was made for another number of tokens");
+  NEED(plan.scalar_type() == at::kByte && plan.is_contiguous() && plan.numel() == bytes, "the batch was made for another number of tokens");
   need_type(scalings, at::kFloat, "scalings", "float32");
   need_sizes(scalings, {L}, "scalings");
-  need(scalings.is_contiguous(), "scalings must be contiguous");
+  NEED(scalings.is_contiguous(), "scalings must be contiguous");
   for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{base, "base_output"}, {out, "out"}}) {
     if (!t.defined()) continue;
-    need(t.dim() == 2 && t.scalar_type() == type, std::string(what) + " must be [num_tokens, N] in the type of x");
+    NEED(t.dim() == 2 && t.scalar_type() == type, std::string(what) + " must be [num_tokens, N] in the type of x");
     need_sizes(t, {T, N}, what);
     need_rows(t, 8, what);
     need_aligned(t, what);
-    if (T > 1 && N > 0) need(t.stride(0) >= N, std::string(what) + " must not overlap itself");
+    if (T > 1 && N > 0) NEED(t.stride(0) >= N, std::string(what) + " must not overlap itself");
   }
   const at::Device dev = one_device({&plan, &base, &x, &h, &A, &B, &scalings, &out});
   int rc = 0;
@@ -875,20 +877,20 @@ HOST_FN(lora) {
     const c10::cuda::OptionalCUDAGuard guard(dev);
     void* st = stream_of(dev);
     const int dt = dt_of(type), iL = static_cast<int>(L), iR = static_cast<int>(R), iS = static_cast<int>(S);
-    if (x.defined()) {
-      h = empty({T, S * R}, type, dev);
-      if (T > 0)
-        rc = b200_lora_shrink(x.data_ptr(), ld_of(x), A.data_ptr(), dt, plan.data_ptr(), static_cast<size_t>(bytes), T,
-                              iL, K, iR, iS, h.data_ptr(), S * R, st);
-    }
-    if (rc == 0 && B.defined()) {
-      if (!out.defined()) out = empty({T, N}, type, dev);
-      if (T > 0 && N > 0)
-        rc = b200_lora_expand(h.data_ptr(), ld_of(h), B.data_ptr(), dt, plan.data_ptr(),
-                              static_cast<size_t>(bytes), static_cast<const float*>(scalings.data_ptr()), T, iL, iR, sizes.data(), iS,
-                              base.defined() ? base.data_ptr() : nullptr, base.defined() ? ld_of(base) : N,
-                              out.data_ptr(), ld_of(out), st);
-    }
+    if (x.defined()) h = empty({T, S * R}, type, dev);
+    if (B.defined() && !out.defined()) out = empty({T, N}, type, dev);
+    const size_t pb = static_cast<size_t>(bytes);
+    const float* sp = static_cast<const float*>(scalings.data_ptr());
+    const void* base_p = base.defined() ? base.data_ptr() : nullptr;
+    const int64_t base_ld = base.defined() ? ld_of(base) : N;
+    if (T > 0 && !B.defined())
+      rc = b200_lora_shrink(x.data_ptr(), ld_of(x), A.data_ptr(), dt, plan.data_ptr(), pb, T, iL, K, iR, iS, h.data_ptr(), S * R, st);
+    else if (T > 0 && N > 0 && x.defined())
+      rc = b200_lora_apply(x.data_ptr(), ld_of(x), A.data_ptr(), B.data_ptr(), dt, plan.data_ptr(), pb, sp, T, iL, K, iR, sizes.data(), iS,
+                           base_p, base_ld, out.data_ptr(), ld_of(out), h.data_ptr(), st);
+    else if (T > 0 && N > 0)
+      rc = b200_lora_expand(h.data_ptr(), ld_of(h), B.data_ptr(), dt, plan.data_ptr(), pb, sp, T, iL, iR, sizes.data(), iS, base_p,
+                            base_ld, out.data_ptr(), ld_of(out), st);
   }
   if (rc != 0) return raise_status("lora", rc);
   return THPVariable_Wrap(B.defined() ? std::move(out) : std::move(h));
