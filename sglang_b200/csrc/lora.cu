@@ -170,15 +170,19 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int keep) {
 }
 
 // ------------------------------------------------------------------------------------------------------- shrink
-constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
+constexpr int kShrinkThreads = 128, kShrinkWarps = kShrinkThreads / 32, kShrinkStages = 5;
+constexpr int kShrinkSmem = kShrinkWarps * kShrinkStages * 2048;
 
 // A cluster of up to eight blocks computes 16 columns of h for one tile of up to 16 tokens, all its warps dividing K; the partial
-// sums are added in a fixed order, first over a block's warps, then over the blocks through distributed shared memory.
+// sums are added in a fixed order, first over a block's warps, then over the blocks through distributed shared memory.  A warp's
+// operands come through a ring of k32 steps in shared memory in which each lane has its own place (nothing to synchronise):
+// with loads into registers instead, 128 tokens of 32 adapters over K = 8192 and three slices of 64 took 25.6 us.
 template <typename T>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ A,
                                                                      int64_t K, int R, int cols, PlanView plan,
                                                                      T* __restrict__ h, int64_t h_ld) {
   pdl_start();
+  extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ float part[kShrinkWarps][256];
   __shared__ float mine[256];
   const int tiles = plan.count[0];
@@ -187,45 +191,57 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __
   const int c0 = blockIdx.z * 16, splits = gridDim.x;
   const int rows = tile.z, rank = tile.x < 0 ? 0 : min(tile.w, R);
   if (c0 % R >= rank && (c0 + 8 >= cols || (c0 + 8) % R >= rank)) {  // behind the rank (R % 8 == 0), or no adapter: zeros
-    if (blockIdx.x == 0 && static_cast<int>(threadIdx.x) / 16 < rows && c0 + static_cast<int>(threadIdx.x) % 16 < cols)
-      h[static_cast<int64_t>(plan.perm[tile.y + threadIdx.x / 16]) * h_ld + c0 + threadIdx.x % 16] = static_cast<T>(0.f);
+    if (blockIdx.x == 0)
+      for (int e = threadIdx.x; e < 256; e += kShrinkThreads)
+        if (e / 16 < rows && c0 + e % 16 < cols) h[static_cast<int64_t>(plan.perm[tile.y + e / 16]) * h_ld + c0 + e % 16] = static_cast<T>(0.f);
     return;
   }
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
   const int r0 = __ldg(plan.perm + tile.y + min(g, rows - 1)), r1 = __ldg(plan.perm + tile.y + min(g + 8, rows - 1));
-  const T* wp[2];
-  bool wok[2];
+  const int chunks = static_cast<int>((K + 31) / 32), per = (chunks + splits * kShrinkWarps - 1) / (splits * kShrinkWarps);
+  const int begin = (blockIdx.x * kShrinkWarps + warp) * per, end = min(begin + per, chunks);
+  // this lane's four operands: rows lane / 4 and lane / 4 + 8 of A and of x; absent ones are zero-filled copies of nothing
+  const char* src[4];
+  uint32_t bytes[4], step[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int col = c0 + g + 8 * i;
-    wok[i] = col < cols && col % R < rank;
-    wp[i] = A + (static_cast<int64_t>(tile.x) * cols + col) * K + 8 * c;
+  for (int i = 0; i < 4; ++i) {
+    const int col = c0 + g + 8 * (i % 2);
+    const bool in = i < 2 ? col < cols && col % R < rank : g + 8 * (i % 2) < rows;
+    const T* row = i < 2 ? A + (static_cast<int64_t>(tile.x) * cols + col) * K : x + (i == 2 ? r0 : r1) * x_ld;
+    src[i] = reinterpret_cast<const char*>(in ? row + static_cast<int64_t>(begin) * 32 + 8 * c : A);
+    bytes[i] = in ? 16 : 0, step[i] = in ? 64 : 0;
   }
   const bool both = rows > 8;
   float acc[2][4] = {};
-  const int chunks = static_cast<int>((K + 31) / 32), per = (chunks + splits * kShrinkWarps - 1) / (splits * kShrinkWarps);
-  const int begin = (blockIdx.x * kShrinkWarps + warp) * per, end = min(begin + per, chunks);
-  for (int i = begin; i < end; i += 4) {
-    uint4 w0[4], w1[4], x0[4], x1[4];
+  const uint32_t ring = smem_u32(dyn) + warp * (kShrinkStages * 2048) + lane * 16, ring_end = ring + kShrinkStages * 2048;
+  const int ragged = K % 32 != 0 && 8 * c >= K % 32 ? chunks - 1 : -1;       // the step of which this lane has nothing
+  uint32_t to = ring, from = ring;
+  auto fetch = [&](int i) {                                          // a stage: [A lo, A hi, x lo, x hi][lane]
+    if (i == ragged) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {                                    // the weights first: x waits for the plan's rows
-      const int64_t k = static_cast<int64_t>(i + u) * 32;
-      const bool in = i + u < end && k + 8 * c < K;
-      w0[u] = load_if(in && wok[0], wp[0] + k);
-      w1[u] = load_if(in && wok[1], wp[1] + k);
+      for (int j = 0; j < 4; ++j) bytes[j] = 0, src[j] = reinterpret_cast<const char*>(A);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t k = static_cast<int64_t>(i + u) * 32 + 8 * c;
-      const bool in = i + u < end && k < K;
-      x0[u] = load_if(in && g < rows, x + r0 * x_ld + k);
-      x1[u] = load_if(both && in && g + 8 < rows, x + r1 * x_ld + k);
+    for (int j = 0; j < 4; ++j) {
+      if (j < 3 || both) sa::cp_async16_n(to + 512 * j, src[j], bytes[j]);
+      src[j] += step[j];
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      mma_k32<T>(acc[0], w0[u], w1[u], x0[u]);
-      if (both) mma_k32<T>(acc[1], w0[u], w1[u], x1[u]);
-    }
+    to = to + 2048 == ring_end ? ring : to + 2048;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kShrinkStages - 1; ++i) {
+    if (begin + i < end) fetch(begin + i);
+    sa::cp_async_commit();
+  }
+#pragma unroll 2
+  for (int i = begin; i < end; ++i) {
+    if (i + kShrinkStages - 1 < end) fetch(i + kShrinkStages - 1);
+    sa::cp_async_commit();
+    sa::cp_async_wait<kShrinkStages - 1>();
+    const uint4 lo = sa::ld_v4(from), hi = sa::ld_v4(from + 512);
+    mma_k32<T>(acc[0], lo, hi, sa::ld_v4(from + 1024));
+    if (both) mma_k32<T>(acc[1], lo, hi, sa::ld_v4(from + 1536));
+    from = from + 2048 == ring_end ? ring : from + 2048;
   }
   // part[warp][token][column]
 #pragma unroll
@@ -233,28 +249,28 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __
 #pragma unroll
     for (int j = 0; j < 4; ++j) part[warp][(8 * i + 2 * c + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[i][j];
   __syncthreads();
-  float sum = 0.f;
+  for (int e = threadIdx.x; e < 256; e += kShrinkThreads) {
+    float sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kShrinkWarps; ++w) sum += part[w][threadIdx.x];
-  int e = threadIdx.x;
-  if (splits > 1) {
+    for (int w = 0; w < kShrinkWarps; ++w) sum += part[w][e];
     mine[e] = sum;
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const int share = 256 / splits;
-    e = static_cast<int>(blockIdx.x) * share + threadIdx.x;
-    sum = 0.f;
-    if (static_cast<int>(threadIdx.x) < share) {
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (splits > 1) cluster.sync();
+  const int share = 256 / splits;                                    // one block: each thread reads what it has written
+  for (int i = threadIdx.x; i < share; i += kShrinkThreads) {
+    const int e = static_cast<int>(blockIdx.x) * share + i, row = e / 16, col = c0 + e % 16;
+    float sum = 0.f;
+    if (splits == 1) {
+      sum = mine[e];
+    } else {
 #pragma unroll 8
       for (int b = 0; b < splits; ++b) sum += *cluster.map_shared_rank(mine + e, b);
-    } else {
-      e = 256;
     }
-    cluster.sync();
+    if (row < rows && col < cols)
+      h[static_cast<int64_t>(plan.perm[tile.y + row]) * h_ld + col] = static_cast<T>(col % R < rank ? sum : 0.f);
   }
-  const int row = e / 16, col = c0 + e % 16;
-  if (row < rows && col < cols)
-    h[static_cast<int64_t>(plan.perm[tile.y + row]) * h_ld + col] = static_cast<T>(col % R < rank ? sum : 0.f);
+  if (splits > 1) cluster.sync();
 }
 
 // A cluster of `splits` blocks computes up to n_alloc columns of h for one tile of up to 128 tokens, each block a part of K.
@@ -485,85 +501,150 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
 }
 constexpr int kExpandThreads = 128;
 
-// A warp: 64 columns of one slice for one tile of up to 16 tokens.  Weight row (tile i, half f, lane / 4) of its four 16-row
-// operands is column 8 (lane / 4) + 2 i + f, so that the eight sums that a lane holds for a token are neighbours: base and out
-// move 16 bytes at a time.
+// A warp takes `per` neighbouring blocks of 64 columns (each within a slice) for one tile of up to 16 tokens.  Weight row (tile i,
+// half f, lane / 4) of its four 16-row operands is column 8 (lane / 4) + 2 i + f, so that the eight sums that a lane holds for a
+// token are neighbours: base and out move 16 bytes at a time.  Operands come through a ring of (block, 32 ranks) steps in shared
+// memory in which each lane has its own places: [B: 8][base: 4][h: 2] vectors.
 // early: the shrink before it is this library's own, launched in the same call, and triggered after its wait; what was there
 // before the shrink (the plan, B and base) may then be read ahead of the wait, which only h has to be behind.
+constexpr int kExpandStages = 3, kExpandStageBytes = 14 * 512;
+constexpr int kExpandSmem = kExpandThreads / 32 * kExpandStages * kExpandStageBytes;
+
 template <typename T>
-__global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h, int h_ld, const T* __restrict__ B, int64_t N, int R, const float* __restrict__ scalings,
-                                                                     PlanView plan, const __grid_constant__ Slices sl,
-                                                                     const T* base, int base_ld, T* out, int out_ld, bool early) {
+__global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h, int h_ld, const T* __restrict__ B, int64_t N, int R,
+                                                                     const float* __restrict__ scalings, PlanView plan,
+                                                                     const __grid_constant__ Slices sl, const T* base, int base_ld,
+                                                                     T* out, int out_ld, int per, bool early) {
   if (!early) pdl_wait();
+  extern __shared__ __align__(128) uint8_t dyn[];
   const int tiles = plan.count[0];
   const int4 tile = plan.tiles[blockIdx.y];                  // in bounds whether or not it is one
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
-  const int block = blockIdx.x * (kExpandThreads / 32) + warp;
+  const int first = (blockIdx.x * (kExpandThreads / 32) + warp) * per, blocks = min(per, sl.first_block[sl.n] - first);
   const int rows = tile.z;
   const bool none = tile.x < 0;
-  if (static_cast<int>(blockIdx.y) >= tiles || block >= sl.first_block[sl.n] || (none && base == out)) {
+  if (static_cast<int>(blockIdx.y) >= tiles || blocks <= 0 || (none && base == out)) {
     if (early) pdl_wait();                                   // no block ends before the shrink has: what follows relies on it
     return;
   }
-  int s = 0;
-#pragma unroll
-  for (int i = 1; i < kMaxSlices; ++i) s += i < sl.n && block >= sl.first_block[i];
-  const int n = sl.first_col[s] + (block - sl.first_block[s]) * 64 + 8 * g;   // the first of this lane's eight columns
-  const bool live = n < sl.first_col[s + 1];
   const bool both = rows > 8;
   const int* perm = plan.perm + tile.y;
   const int h_row[2] = {__ldg(perm + min(g, rows - 1)), __ldg(perm + min(g + 8, rows - 1))};
   int token[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) token[i] = __ldg(perm + min(8 * (i / 2) + 2 * c + i % 2, rows - 1));
-  const int rank = none ? 0 : min(tile.w, R);
+  const int rank = none ? 0 : min(tile.w, R), chunks = max(1, (rank + 31) / 32), steps = blocks * chunks;
   const float scaling = none ? 0.f : __ldg(scalings + tile.x);
-  const T* bp = B + (static_cast<int64_t>(tile.x) * N + n) * R + 8 * c;
-  auto load_b = [&](uint4 (&w)[8], int r0) {
-    const int keep = rank - r0 - 8 * c;
+  const uint32_t ring = smem_u32(dyn) + warp * (kExpandStages * kExpandStageBytes) + lane * 16;
+  // Where a walk over the steps (block, 32 ranks) stands: once for the copies, once for the products.
+  struct At {
+    int block, j, s, n;
+    bool live;
+    uint32_t place;
+  };
+  auto enter = [&](At& p) {                                  // slice and first column (of this lane's eight) of its block
+    p.s = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = load_if(live && keep > 0, bp + i * R + r0);
-    if (keep > 0 && keep < 8) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = first_of(w[i], keep);
+    for (int i = 1; i < kMaxSlices; ++i) p.s += i < sl.n && p.block >= sl.first_block[i];
+    p.n = sl.first_col[p.s] + (p.block - sl.first_block[p.s]) * 64 + 8 * g;
+    p.live = p.n < sl.first_col[p.s + 1];
+  };
+  auto advance = [&](At& p) {
+    p.place = p.place + kExpandStageBytes == ring + kExpandStages * kExpandStageBytes ? ring : p.place + kExpandStageBytes;
+    if (++p.j == chunks) {
+      p.j = 0;
+      ++p.block;
+      enter(p);
     }
   };
-  uint4 w[8], v[4];
-  load_b(w, 0);
+  At in_flight = {first, 0, 0, 0, false, ring}, at = in_flight;
+  enter(in_flight);
+  at = in_flight;
+  const int64_t row_bytes = static_cast<int64_t>(R) * sizeof(T);
+  const char* b0 = reinterpret_cast<const char*>(B + static_cast<int64_t>(none ? 0 : tile.x) * N * R + 8 * c);
+  auto fetch_weights = [&](const At& p) {
+    const bool in = p.live && rank - 32 * p.j - 8 * c > 0;
+    const char* src = in ? b0 + p.n * row_bytes + p.j * (32 * sizeof(T)) : b0 - 8 * c * sizeof(T);
+    const uint32_t bytes = in ? 16 : 0, ld = in ? static_cast<uint32_t>(row_bytes) : 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = base != nullptr && live && 8 * (i / 2) + 2 * c + i % 2 < rows
-               ? *reinterpret_cast<const uint4*>(base + static_cast<int64_t>(token[i]) * base_ld + n) : make_uint4(0, 0, 0, 0);
-  if (early) pdl_wait();
-  pdl_trigger();
-  float acc[2][4][4] = {};
-  const T* hp[2] = {h + static_cast<int64_t>(h_row[0]) * h_ld + s * R + 8 * c, h + static_cast<int64_t>(h_row[1]) * h_ld + s * R + 8 * c};
-#pragma unroll 1
-  for (int r0 = 0; r0 < rank; r0 += 32) {
-    const bool in = rank - r0 - 8 * c > 0;
-    uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;              // coherent loads: h may be written while this kernel is resident
-    if (in && g < rows) x0 = __ldcg(reinterpret_cast<const uint4*>(hp[0] + r0));
-    if (in && g + 8 < rows) x1 = __ldcg(reinterpret_cast<const uint4*>(hp[1] + r0));
+    for (int i = 0; i < 8; ++i) sa::cp_async16_n(p.place + i * 512, src + i * ld, bytes);
+    if (base != nullptr && p.j + 1 == chunks) {              // with the block's last step, which stores
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      mma_k32<T>(acc[0][i], w[2 * i], w[2 * i + 1], x0);
-      if (both) mma_k32<T>(acc[1][i], w[2 * i], w[2 * i + 1], x1);
-    }
-    if (r0 + 32 < rank) load_b(w, r0 + 32);
-  }
-  if (!live) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (8 * (i / 2) + 2 * c + i % 2 >= rows) continue;
-    if (!none) {
-      uint32_t* q = &v[i].x;
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const float2 b = unpack2<T>(q[m]);
-        q[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[i / 2][m][i % 2], b.x), fmaf(scaling, acc[i / 2][m][i % 2 + 2], b.y));
+      for (int i = 0; i < 4; ++i) {
+        if (i >= 2 && !both) continue;
+        const bool mine = p.live && 8 * (i / 2) + 2 * c + i % 2 < rows;
+        sa::cp_async16_n(p.place + (8 + i) * 512, mine ? base + static_cast<int64_t>(token[i]) * base_ld + p.n : base, mine ? 16 : 0);
       }
     }
-    *reinterpret_cast<uint4*>(out + static_cast<int64_t>(token[i]) * out_ld + n) = v[i];
+  };
+  const T* h0[2] = {h + static_cast<int64_t>(h_row[0]) * h_ld + 8 * c, h + static_cast<int64_t>(h_row[1]) * h_ld + 8 * c};
+  auto fetch_h = [&](const At& p) {
+    const bool in = rank - 32 * p.j - 8 * c > 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool mine = in && g + 8 * i < rows;
+      if (i == 0 || both) sa::cp_async16_n(p.place + (12 + i) * 512, mine ? h0[i] + p.s * R + 32 * p.j : h, mine ? 16 : 0);
+    }
+  };
+  static_assert(kExpandStages == 3, "two steps ahead");
+  fetch_weights(in_flight);
+  At second = in_flight;
+  if (steps > 1) {
+    advance(second);
+    fetch_weights(second);
+  }
+  if (early) pdl_wait();
+  pdl_trigger();
+  fetch_h(in_flight);
+  sa::cp_async_commit();
+  if (steps > 1) fetch_h(second);
+  sa::cp_async_commit();
+  in_flight = second;
+  float acc[2][4][4];
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step, advance(at)) {
+    if (step + 2 < steps) {
+      advance(in_flight);
+      fetch_weights(in_flight);
+      fetch_h(in_flight);
+    }
+    sa::cp_async_commit();
+    sa::cp_async_wait<2>();
+    const uint32_t from = at.place;
+    const int j = at.j;
+    if (j == 0) {
+#pragma unroll
+      for (int m = 0; m < 32; ++m) acc[m / 16][m / 4 % 4][m % 4] = 0.f;
+    }
+    if (!none) {
+      const int keep = rank - 32 * j - 8 * c;
+      const uint4 x0 = sa::ld_v4(from + 12 * 512);
+      uint4 x1 = make_uint4(0, 0, 0, 0);
+      if (both) x1 = sa::ld_v4(from + 13 * 512);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 lo = sa::ld_v4(from + 2 * i * 512), hi = sa::ld_v4(from + (2 * i + 1) * 512);
+        if (keep > 0 && keep < 8) lo = first_of(lo, keep), hi = first_of(hi, keep);
+        mma_k32<T>(acc[0][i], lo, hi, x0);
+        if (both) mma_k32<T>(acc[1][i], lo, hi, x1);
+      }
+    }
+    if (j + 1 < chunks || !at.live) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (8 * (i / 2) + 2 * c + i % 2 >= rows) continue;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (base != nullptr) v = sa::ld_v4(from + (8 + i) * 512);
+      if (!none) {
+        uint32_t* q = &v.x;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const float2 b = unpack2<T>(q[m]);
+          q[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[i / 2][m][i % 2], b.x), fmaf(scaling, acc[i / 2][m][i % 2 + 2], b.y));
+        }
+      }
+      *reinterpret_cast<uint4*>(out + static_cast<int64_t>(token[i]) * out_ld + at.n) = v;
+    }
   }
 }
 
@@ -719,12 +800,14 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
     return B200_OK;
   }
   if (tile_rows(tokens) == kSmallRows) {
-    // Enough blocks for two on every SM, if K has a k32 step for each of their warps.
+    // Enough blocks for six on every SM (of the tiles that a plan may have about half are used, and five blocks are resident), if
+    // K has a k32 step for each of their warps.
     const int passes = (cols + 15) / 16;
     int splits = 1;
-    while (splits < 8 && tiles * passes * splits < 2LL * sms && splits * 32 * kShrinkWarps < K) splits *= 2;
-    B200_CUDA_TRY(launch_cluster(lora_shrink_kernel<T>, dim3(splits, static_cast<unsigned>(tiles), passes), dim3(kShrinkThreads), 0, splits,
-                                 st, x, x_ld, A, K, R, cols, plan, h, h_ld));
+    while (splits < 8 && tiles * passes * splits < 6LL * sms && splits * 32 * kShrinkWarps < K) splits *= 2;
+    B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShrinkSmem));
+    B200_CUDA_TRY(launch_cluster(lora_shrink_kernel<T>, dim3(splits, static_cast<unsigned>(tiles), passes), dim3(kShrinkThreads),
+                                 kShrinkSmem, splits, st, x, x_ld, A, K, R, cols, plan, h, h_ld));
     return B200_OK;
   }
   if (gemm_sticky_status() != 0) return B200_ERR_DEVICE_TIMEOUT;
@@ -759,15 +842,23 @@ template <typename T>
 int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* scalings, PlanView plan, const Slices& sl, int64_t tokens,
            int64_t tiles, const T* base, int64_t base_ld, T* out, int64_t out_ld, bool early, cudaStream_t st) {
   static_assert(kExpandThreads == kWalkThreads, "one grid for both");
+  const int sms = sm_count();
+  if (sms <= 0) return B200_ERR_CUDA;
   constexpr int kWarps = kExpandThreads / 32;
-  const dim3 grid(static_cast<unsigned>((sl.first_block[sl.n] + kWarps - 1) / kWarps), static_cast<unsigned>(tiles));
+  // small batches: as many blocks of columns a warp as leave eight warps for each SM, at most eight
+  int per = 1;
+  if (tile_rows(tokens) == kSmallRows) {
+    const int64_t most = tiles * sl.first_block[sl.n] / (8LL * sms);
+    per = static_cast<int>(most < 1 ? 1 : most < 8 ? most : 8);
+  }
+  const dim3 grid(static_cast<unsigned>((sl.first_block[sl.n] + kWarps * per - 1) / (kWarps * per)), static_cast<unsigned>(tiles));
   auto go = [&](auto kern, int smem, auto... more) -> int {
     if (smem > 40 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     B200_CUDA_TRY(launch_pdl(kern, grid, dim3(kExpandThreads), smem, st, h, static_cast<int>(h_ld), B, N, R, scalings, plan, sl, base,
                              static_cast<int>(base_ld), out, static_cast<int>(out_ld), more...));
     return B200_OK;
   };
-  if (tile_rows(tokens) == kSmallRows) return go(lora_expand_kernel<T>, 0, early);
+  if (tile_rows(tokens) == kSmallRows) return go(lora_expand_kernel<T>, kExpandSmem, per, early);
   if (R <= 32) return go(lora_expand_tiles_kernel<T, 1, 4>, walk_smem<1, 4>());
   if (R <= 64) return go(lora_expand_tiles_kernel<T, 2, 4>, walk_smem<2, 4>());
   if (R <= 128) return go(lora_expand_tiles_kernel<T, 4, 4>, walk_smem<4, 4>());
