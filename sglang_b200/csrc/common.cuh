@@ -277,20 +277,24 @@ __device__ __forceinline__ float ld_f32(uint32_t addr) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-// Asynchronous 4-, 8- and 16-byte copies global -> shared (zero-filled when !in), and the arrival on `bar` once all of this
+// Asynchronous 4- and 16-byte copies global -> shared (zero-filled when !in), and the arrival on `bar` once all of this
 // thread's earlier ones have landed (counted in the barrier's init count).
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(in ? 8 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
-// `bytes` (0 .. 16) of 16 copied, the rest zero-filled.
-__device__ __forceinline__ void cp_async16_n(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// 8 or 16 bytes copied, or zeros written and the source not read.
+template <int BYTES>
+__device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, bool in) {
+  static_assert(BYTES == 8 || BYTES == 16, "");
+  if constexpr (BYTES == 16)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %2, 0;\n\tcp.async.cg.shared.global [%0], [%1], 16, p;\n\t}\n"
+                 ::"r"(dst), "l"(src), "r"(in ? 1u : 0u) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %2, 0;\n\tcp.async.ca.shared.global [%0], [%1], 8, p;\n\t}\n"
+                 ::"r"(dst), "l"(src), "r"(in ? 1u : 0u) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>   // until at most the PENDING youngest groups of this thread are under way

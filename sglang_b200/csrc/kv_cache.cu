@@ -181,8 +181,8 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
     const bool live = h < r.last && in_row;
     const T* row = r.src + (live ? h : 0) * r.src_sh;
     const uint32_t to = ring + stage * kStageBytes;
-    sa::cp_async16(to, row + (live ? o0 : 0), live);
-    sa::cp_async16(to + kStageBytes / 2, row + (live ? o1 : 0), live);
+    sa::cp_async_or_zero<16>(to, row + (live ? o0 : 0), live);
+    sa::cp_async_or_zero<16>(to + kStageBytes / 2, row + (live ? o1 : 0), live);
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {

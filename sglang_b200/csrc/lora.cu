@@ -202,14 +202,14 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __
   const int begin = (blockIdx.x * kShrinkWarps + warp) * per, end = min(begin + per, chunks);
   // this lane's four operands: rows lane / 4 and lane / 4 + 8 of A and of x; absent ones are zero-filled copies of nothing
   const char* src[4];
-  uint32_t bytes[4], step[4];
+  bool there[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int col = c0 + g + 8 * (i % 2);
     const bool in = i < 2 ? col < cols && col % R < rank : g + 8 * (i % 2) < rows;
     const T* row = i < 2 ? A + (static_cast<int64_t>(tile.x) * cols + col) * K : x + (i == 2 ? r0 : r1) * x_ld;
     src[i] = reinterpret_cast<const char*>(in ? row + static_cast<int64_t>(begin) * 32 + 8 * c : A);
-    bytes[i] = in ? 16 : 0, step[i] = in ? 64 : 0;
+    there[i] = in;
   }
   const bool both = rows > 8;
   float acc[2][4] = {};
@@ -219,12 +219,12 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __
   auto fetch = [&](int i) {                                          // a stage: [A lo, A hi, x lo, x hi][lane]
     if (i == ragged) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bytes[j] = 0, src[j] = reinterpret_cast<const char*>(A);
+      for (int j = 0; j < 4; ++j) there[j] = false, src[j] = reinterpret_cast<const char*>(A);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (j < 3 || both) sa::cp_async16_n(to + 512 * j, src[j], bytes[j]);
-      src[j] += step[j];
+      if (j < 3 || both) sa::cp_async_or_zero<16>(to + 512 * j, src[j], there[j]);
+      src[j] += 64;
     }
     to = to + 2048 == ring_end ? ring : to + 2048;
   };
@@ -565,15 +565,15 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h,
   auto fetch_weights = [&](const At& p) {
     const bool in = p.live && rank - 32 * p.j - 8 * c > 0;
     const char* src = in ? b0 + p.n * row_bytes + p.j * (32 * sizeof(T)) : b0 - 8 * c * sizeof(T);
-    const uint32_t bytes = in ? 16 : 0, ld = in ? static_cast<uint32_t>(row_bytes) : 0;
+    const uint32_t ld = static_cast<uint32_t>(row_bytes);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sa::cp_async16_n(p.place + i * 512, src + i * ld, bytes);
+    for (int i = 0; i < 8; ++i) sa::cp_async_or_zero<16>(p.place + i * 512, src + i * ld, in);
     if (base != nullptr && p.j + 1 == chunks) {              // with the block's last step, which stores
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= 2 && !both) continue;
         const bool mine = p.live && 8 * (i / 2) + 2 * c + i % 2 < rows;
-        sa::cp_async16_n(p.place + (8 + i) * 512, mine ? base + static_cast<int64_t>(token[i]) * base_ld + p.n : base, mine ? 16 : 0);
+        sa::cp_async_or_zero<16>(p.place + (8 + i) * 512, mine ? base + static_cast<int64_t>(token[i]) * base_ld + p.n : base, mine);
       }
     }
   };
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h,
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const bool mine = in && g + 8 * i < rows;
-      if (i == 0 || both) sa::cp_async16_n(p.place + (12 + i) * 512, mine ? h0[i] + p.s * R + 32 * p.j : h, mine ? 16 : 0);
+      if (i == 0 || both) sa::cp_async_or_zero<16>(p.place + (12 + i) * 512, mine ? h0[i] + p.s * R + 32 * p.j : h, mine);
     }
   };
   static_assert(kExpandStages == 3, "two steps ahead");
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
     for (int e = threadIdx.x; e < kLargeRows * RJ * 4; e += kWalkThreads) {
       const int row = e / (RJ * 4), v = e % (RJ * 4);
       const bool in = row < rows && v * 8 < rank;
-      sa::cp_async16(h_at(row, v), h + (in ? static_cast<int64_t>(row_of[row]) * h_ld + s * R + v * 8 : 0), in);
+      sa::cp_async_or_zero<16>(h_at(row, v), h + (in ? static_cast<int64_t>(row_of[row]) * h_ld + s * R + v * 8 : 0), in);
     }
   }
   auto fetch = [&](int step) {
@@ -711,8 +711,8 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
       const bool in = base != nullptr && r < rows && live;
       const T* src = in ? base + static_cast<int64_t>(row_of[r]) * base_ld + n : h;
       const uint32_t to = ring + step % kWalkStages * kStage + i * kHalf;
-      if constexpr (NT == 4) sa::cp_async16(to, src, in);
-      else sa::cp_async8(to, src, in);
+      if constexpr (NT == 4) sa::cp_async_or_zero<16>(to, src, in);
+      else sa::cp_async_or_zero<8>(to, src, in);
     }
   };
   const int steps = (rows + 15) / 16;
