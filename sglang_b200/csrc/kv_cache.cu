@@ -163,136 +163,142 @@ struct Rows {
   bool poisoned;
 };
 
-// ROPE: 0 none, 1 neox, 2 neighbouring pairs.  With neox pairs a lane of the rotated part holds elements 8l .. 8l + 7 and their
-// partners rot / 2 further on, so that a rotation stays inside the lane; otherwise elements 16l .. 16l + 15.
-// The weights are multiplied into the cosines and sines, once for all rows.
-template <typename T, int G, int ROPE, bool STORE, bool CODES>
+// How a row is treated: taken as it is, normalised (if there is a weight) and not rotated, rotated as neox pairs, rotated as
+// neighbouring pairs.
+enum { kRaw = -1, kNorm = 0, kNeox = 1, kPairs = 2 };
+
+// With neox pairs a lane of the rotated part holds elements 8l .. 8l + 7 and their partners rot / 2 further on, so that a rotation
+// stays inside the lane; otherwise elements 16l .. 16l + 15.  The weights are multiplied into the cosines and sines, once for all
+// rows; where the position is not in the table, all of these factors are NaN.
+template <typename T, int G, int KIND, bool STORE, bool CODES>
 __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lane, int D, int rot, float eps, const float* table_row) {
   constexpr int RPW = 32 / G;
-  constexpr bool SPLIT = ROPE == 1;
+  constexpr bool SPLIT = KIND == kNeox, ROPE = KIND == kNeox || KIND == kPairs;
   const int l = lane % G, sub = lane / G;
   const bool in_row = l * 16 < D;
-  const bool turned = ROPE != 0 && l * 16 < rot;
+  const bool turned = ROPE && l * 16 < rot;
   const int o0 = SPLIT && turned ? 8 * l : 16 * l, o1 = SPLIT && turned ? rot / 2 + 8 * l : 16 * l + 8;
   const float inv_d = 1.f / static_cast<float>(D);
   // ring: this lane's 32 bytes of each of the next kStages row groups; only the lane itself reads them
-  auto fetch = [&](int head, int stage) {
-    const int h = head + sub;
-    const bool live = h < r.last && in_row;
-    const T* row = r.src + (live ? h : 0) * r.src_sh;
-    const uint32_t to = ring + stage * kStageBytes;
-    sa::cp_async_or_zero<16>(to, row + (live ? o0 : 0), live);
-    sa::cp_async_or_zero<16>(to + kStageBytes / 2, row + (live ? o1 : 0), live);
+  const uint32_t ring_end = ring + kStages * kStageBytes;
+  const int heads = in_row ? r.last - r.first - sub : 0;      // of this lane's, counted by RPW
+  const T* src = r.src + (r.first + sub) * r.src_sh;
+  const int64_t src_step = RPW * r.src_sh;
+  uint32_t to = ring;
+  auto fetch = [&](int i) {                                   // row group i / RPW
+    const bool live = i < heads;
+    sa::cp_async_or_zero<16>(to, live ? src + o0 : r.src, live);
+    sa::cp_async_or_zero<16>(to + kStageBytes / 2, live ? src + o1 : r.src, live);
+    src += src_step;
+    to = to + kStageBytes == ring_end ? ring : to + kStageBytes;
   };
+  const int count = r.last - r.first;
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
-    if (r.first + i * RPW < r.last) fetch(r.first + i * RPW, i);
+    if (i * RPW < count) fetch(i * RPW);
     sa::cp_async_commit();
   }
-  f2 w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = both(1.f);
-  if (r.weight != nullptr && in_row) {
-    unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o0)), w);
-    unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o1)), w + 4);
-  }
   // the coefficients, two elements at a time: y' = y ca + partner sa (neox: pairs (e, e + 1) of the first run, then of the second;
-  // otherwise each pair is one that is rotated); elements that are not rotated keep w in ca
+  // otherwise each pair is one that is rotated); elements that are not rotated have their weight in ca
   f2 ca[8], sa[8];
-  if (ROPE != 0 && turned) {
-    float cc[8] = {}, ss[8] = {};
-    if (!r.poisoned) {
+  if (KIND != kRaw) {
+    f2 w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = both(r.poisoned ? __uint_as_float(0x7fc00000u) : 1.f);
+    if (r.weight != nullptr && in_row && !r.poisoned) {
+      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o0)), w);
+      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o1)), w + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ca[i] = w[i];
+    if (turned) {
+      float cc[8], ss[8];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float4 c = __ldg(reinterpret_cast<const float4*>(table_row + 8 * l + 4 * i));
-        const float4 s = __ldg(reinterpret_cast<const float4*>(table_row + rot / 2 + 8 * l + 4 * i));
+        float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = c;
+        if (!r.poisoned) {
+          c = __ldg(reinterpret_cast<const float4*>(table_row + 8 * l + 4 * i));
+          s = __ldg(reinterpret_cast<const float4*>(table_row + rot / 2 + 8 * l + 4 * i));
+        }
         cc[4 * i] = c.x, cc[4 * i + 1] = c.y, cc[4 * i + 2] = c.z, cc[4 * i + 3] = c.w;
         ss[4 * i] = s.x, ss[4 * i + 1] = s.y, ss[4 * i + 2] = s.z, ss[4 * i + 3] = s.w;
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 mine = split(w[i]);
-      if (ROPE == 1) {
-        const int j = 2 * (i % 4);
-        const float2 other = split(w[(i + 4) % 8]);
-        ca[i] = make_f2(cc[j] * mine.x, cc[j + 1] * mine.y);
-        sa[i] = i < 4 ? make_f2(-ss[j] * other.x, -ss[j + 1] * other.y) : make_f2(ss[j] * other.x, ss[j + 1] * other.y);
-      } else {
-        ca[i] = make_f2(cc[i] * mine.x, cc[i] * mine.y);
-        sa[i] = make_f2(-ss[i] * mine.y, ss[i] * mine.x);
+      for (int i = 0; i < 8; ++i) {
+        const float2 mine = split(w[i]);
+        if (SPLIT) {
+          const int j = 2 * (i % 4);
+          const float2 other = split(w[(i + 4) % 8]);
+          ca[i] = make_f2(cc[j] * mine.x, cc[j + 1] * mine.y);
+          sa[i] = i < 4 ? make_f2(-ss[j] * other.x, -ss[j + 1] * other.y) : make_f2(ss[j] * other.x, ss[j + 1] * other.y);
+        } else {
+          ca[i] = make_f2(cc[i] * mine.x, cc[i] * mine.y);
+          sa[i] = make_f2(-ss[i] * mine.y, ss[i] * mine.x);
+        }
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ca[i] = w[i];
   }
-  int stage = 0;
+  T* dst = STORE && r.dst != nullptr ? r.dst + (r.first + sub) * r.dst_sh : nullptr;
+  const int64_t dst_step = RPW * r.dst_sh;
+  uint8_t* codes = CODES ? r.codes + (r.first + sub) * r.codes_sh : nullptr;
+  const int64_t codes_step = RPW * r.codes_sh;
+  float* scales = CODES ? r.scales + (r.first + sub) * r.scales_sh : nullptr;
+  const int64_t scales_step = RPW * r.scales_sh;
+  uint32_t from = ring;
 #pragma unroll 1
-  for (int head = r.first; head < r.last; head += RPW) {
-    {
-      const int ahead = head + (kStages - 1) * RPW;
-      if (ahead < r.last) fetch(ahead, (stage + kStages - 1) % kStages);
-      sa::cp_async_commit();
-      sa::cp_async_wait<kStages - 1>();
-    }
-    const int h = head + sub;
-    const bool live = h < r.last && in_row;
+  for (int i = 0; i < count; i += RPW) {
+    if (i + (kStages - 1) * RPW < count) fetch(i + (kStages - 1) * RPW);
+    sa::cp_async_commit();
+    sa::cp_async_wait<kStages - 1>();
+    const bool live = i < heads;
     f2 y[8];
-    {
-      const uint32_t from = ring + stage * kStageBytes;
-      unpack8<T>(sa::ld_v4(from), y);
-      unpack8<T>(sa::ld_v4(from + kStageBytes / 2), y + 4);
-      stage = (stage + 1) % kStages;
-    }
-    if (r.weight != nullptr) {
-      f2 sum = mul(y[0], y[0]);
+    unpack8<T>(sa::ld_v4(from), y);
+    unpack8<T>(sa::ld_v4(from + kStageBytes / 2), y + 4);
+    from = from + kStageBytes == ring_end ? ring : from + kStageBytes;
+    if (KIND != kRaw) {
+      if (r.weight != nullptr) {
+        f2 sum = mul(y[0], y[0]);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) sum = fma(y[i], y[i], sum);
-      float sq = split(sum).x + split(sum).y;
+        for (int e = 1; e < 8; ++e) sum = fma(y[e], y[e], sum);
+        float sq = split(sum).x + split(sum).y;
 #pragma unroll
-      for (int off = G / 2; off >= 1; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-      const f2 rinv = both(rsqrtf(fmaf(sq, inv_d, eps)));
+        for (int off = G / 2; off >= 1; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
+        const f2 rinv = both(rsqrtf(fmaf(sq, inv_d, eps)));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = mul(y[i], rinv);
-    }
-    if (ROPE != 0 && turned) {
-      if constexpr (ROPE == 1) {
+        for (int e = 0; e < 8; ++e) y[e] = mul(y[e], rinv);
+      }
+      if (turned) {
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f2 a = y[i], b = y[i + 4];
-          y[i] = fma(a, ca[i], mul(b, sa[i]));
-          y[i + 4] = fma(b, ca[i + 4], mul(a, sa[i + 4]));
+          for (int e = 0; e < 4; ++e) {
+            const f2 a = y[e], b = y[e + 4];
+            y[e] = fma(a, ca[e], mul(b, sa[e]));
+            y[e + 4] = fma(b, ca[e + 4], mul(a, sa[e + 4]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 mine = split(y[e]);
+            y[e] = fma(y[e], ca[e], mul(make_f2(mine.y, mine.x), sa[e]));
+          }
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 mine = split(y[i]);
-          y[i] = fma(y[i], ca[i], mul(make_f2(mine.y, mine.x), sa[i]));
-        }
-      }
-      if (r.poisoned) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = both(__uint_as_float(0x7fc00000u));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = mul(y[i], ca[i]);
-      if (ROPE != 0 && r.poisoned) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = both(__uint_as_float(0x7fc00000u));
+        for (int e = 0; e < 8; ++e) y[e] = mul(y[e], ca[e]);
       }
     }
-    if (STORE && r.dst != nullptr && live) {
-      T* row = r.dst + h * r.dst_sh;
-      *reinterpret_cast<uint4*>(row + o0) = pack8<T>(y);
-      *reinterpret_cast<uint4*>(row + o1) = pack8<T>(y + 4);
+    if (STORE && dst != nullptr) {
+      if (live) {
+        *reinterpret_cast<uint4*>(dst + o0) = pack8<T>(y);
+        *reinterpret_cast<uint4*>(dst + o1) = pack8<T>(y + 4);
+      }
+      dst += dst_step;
     }
     if (CODES) {
       float amax = 1e-10f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 v = split(y[i]);
+      for (int e = 0; e < 8; ++e) {
+        const float2 v = split(y[e]);
         amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
       }
 #pragma unroll
@@ -300,22 +306,24 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
       const float scale = scale_of(amax);
       const uint4 q = quantise16(y, scale);
       if (live) {
-        uint8_t* codes = r.codes + h * r.codes_sh;
         if constexpr (SPLIT) {
           *reinterpret_cast<uint2*>(codes + o0) = make_uint2(q.x, q.y);
           *reinterpret_cast<uint2*>(codes + o1) = make_uint2(q.z, q.w);
         } else {
           *reinterpret_cast<uint4*>(codes + o0) = q;
         }
-        if (l == 0) r.scales[h * r.scales_sh] = r.poisoned ? __uint_as_float(0x7fc00000u) : scale;
+        if (l == 0) *scales = KIND != kRaw && r.poisoned ? __uint_as_float(0x7fc00000u) : scale;
       }
+      codes += codes_step;
+      scales += scales_step;
     }
   }
 }
 
-template <typename T, int G, int ROPE>
+template <typename T, int G, int KIND>
 __global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
   pdl_start();
+  constexpr bool ROPE = KIND == kNeox || KIND == kPairs;
   __shared__ __align__(16) uint8_t rings[kThreads / 32 * kStages * kStageBytes];
   const int lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(rings) + (threadIdx.x >> 5) * (kStages * kStageBytes) + lane * 16;
@@ -327,7 +335,9 @@ __global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_con
   int chunk = static_cast<int>(item - tok32 * p.chunks);
   Rows<T> r = {};
   const float* table_row = nullptr;
-  if (ROPE != 0) {
+  int64_t slot = -1;
+  if (p.Hv != 0 && chunk >= p.chunks_q) slot = load_index(p.slots, p.slots_i64, tok);
+  if (ROPE) {
     const int64_t pos = load_index(p.positions, p.pos_i64, tok);
     if (pos < 0) return;                                     // padding: nothing of this token is read or written
     r.poisoned = pos >= p.max_position;                      // a position that the table lacks: NaN, not a read behind it
@@ -338,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_con
     r.src = static_cast<const T*>(p.q) + tok * p.q_st, r.src_sh = p.q_sh;
     r.dst = static_cast<T*>(p.q_out) + tok * p.qo_st, r.dst_sh = p.qo_sh;
     r.weight = static_cast<const T*>(p.q_w);
-    do_rows<T, G, ROPE, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
+    do_rows<T, G, KIND, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
     return;
   }
   chunk -= p.chunks_q;
@@ -350,12 +360,9 @@ __global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_con
     r.weight = static_cast<const T*>(p.k_w);
   } else {
     r.src = static_cast<const T*>(p.v) + tok * p.v_st, r.src_sh = p.v_sh;
-    r.poisoned = false;
   }
-  bool keep = false;
-  if (p.Hv != 0) {
-    const int64_t slot = load_index(p.slots, p.slots_i64, tok);
-    keep = slot >= 0 && slot < p.num_slots;
+  const bool keep = slot >= 0 && slot < p.num_slots;
+  if (keep) {
     const uint32_t page = p.page_shift >= 0 ? static_cast<uint32_t>(slot) >> p.page_shift : static_cast<uint32_t>(slot) / p.page_size;
     const uint32_t place = static_cast<uint32_t>(slot) - page * p.page_size;
     r.codes = keys ? p.kc + page * p.kc_s[0] + place * p.kc_s[1] : p.vc + page * p.vc_s[0] + place * p.vc_s[1];
@@ -363,26 +370,31 @@ __global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_con
     r.scales = keys ? p.ks + page * p.ks_s[0] + place * p.ks_s[1] : p.vs + page * p.vs_s[0] + place * p.vs_s[1];
     r.scales_sh = keys ? p.ks_s[2] : p.vs_s[2];
   }
-  if (keys && !keep) {
-    if (r.dst != nullptr) do_rows<T, G, ROPE, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
-  } else if (keys) {
-    do_rows<T, G, ROPE, true, true>(r, ring, lane, p.D, p.rot, p.eps, table_row);
-  } else if (keep) {
-    do_rows<T, G, 0, false, true>(r, ring, lane, p.D, 0, 0.f, nullptr);
+  if constexpr (KIND == kRaw) {
+    if (keep) do_rows<T, G, kRaw, false, true>(r, ring, lane, p.D, 0, 0.f, nullptr);
+  } else {
+    if (!keys) {
+      if (keep) do_rows<T, G, kRaw, false, true>(r, ring, lane, p.D, 0, 0.f, nullptr);
+    } else if (keep) {
+      do_rows<T, G, KIND, true, true>(r, ring, lane, p.D, p.rot, p.eps, table_row);
+    } else if (r.dst != nullptr) {
+      do_rows<T, G, KIND, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
+    }
   }
 }
 
 template <typename T, int G>
-cudaError_t launch_rows(const HeadRowsParams& p, int rope, unsigned grid, cudaStream_t st) {
-  switch (rope) {
-    case 0: return launch_pdl(head_rows_kernel<T, G, 0>, dim3(grid), dim3(kThreads), 0, st, p);
-    case 1: return launch_pdl(head_rows_kernel<T, G, 1>, dim3(grid), dim3(kThreads), 0, st, p);
-    default: return launch_pdl(head_rows_kernel<T, G, 2>, dim3(grid), dim3(kThreads), 0, st, p);
+cudaError_t launch_rows(const HeadRowsParams& p, int kind, unsigned grid, cudaStream_t st) {
+  switch (kind) {
+    case kRaw: return launch_pdl(head_rows_kernel<T, G, kRaw>, dim3(grid), dim3(kThreads), 0, st, p);
+    case kNorm: return launch_pdl(head_rows_kernel<T, G, kNorm>, dim3(grid), dim3(kThreads), 0, st, p);
+    case kNeox: return launch_pdl(head_rows_kernel<T, G, kNeox>, dim3(grid), dim3(kThreads), 0, st, p);
+    default: return launch_pdl(head_rows_kernel<T, G, kPairs>, dim3(grid), dim3(kThreads), 0, st, p);
   }
 }
 
 template <typename T, int G>
-int go_rows(HeadRowsParams p, int rope, cudaStream_t st) {
+int go_rows(HeadRowsParams p, int kind, cudaStream_t st) {
   const int sms = sm_count();
   if (sms <= 0) return B200_ERR_CUDA;
   constexpr int RPW = 32 / G, WPB = kThreads / 32;
@@ -396,16 +408,16 @@ int go_rows(HeadRowsParams p, int rope, cudaStream_t st) {
   p.chunks_magic = static_cast<uint32_t>((1ULL << 32) / p.chunks + 1);
   const int64_t blocks = (p.T * p.chunks + WPB - 1) / WPB;
   if (blocks * WPB > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
-  B200_CUDA_TRY((launch_rows<T, G>(p, rope, static_cast<unsigned>(blocks), st)));
+  B200_CUDA_TRY((launch_rows<T, G>(p, kind, static_cast<unsigned>(blocks), st)));
   return B200_OK;
 }
 
 template <typename T>
-int dispatch_rows(const HeadRowsParams& p, int rope, cudaStream_t st) {
-  if (p.D <= 32) return go_rows<T, 2>(p, rope, st);
-  if (p.D <= 64) return go_rows<T, 4>(p, rope, st);
-  if (p.D <= 128) return go_rows<T, 8>(p, rope, st);
-  return go_rows<T, 16>(p, rope, st);
+int dispatch_rows(const HeadRowsParams& p, int kind, cudaStream_t st) {
+  if (p.D <= 32) return go_rows<T, 2>(p, kind, st);
+  if (p.D <= 64) return go_rows<T, 4>(p, kind, st);
+  if (p.D <= 128) return go_rows<T, 8>(p, kind, st);
+  return go_rows<T, 16>(p, kind, st);
 }
 
 int take_heads(const b200_heads* h, int64_t T, int H, const void** ptr, int64_t* st, int64_t* sh) {
@@ -584,9 +596,10 @@ int rows_entry(const b200_heads* q, const b200_heads* k, const b200_heads* v, co
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (p.page_size == 1u << i) p.page_shift = i;
-  const int rope = cos_sin ? (is_neox ? 1 : 2) : 0;
+  // only a store alone takes its rows as they are: k_out without a rotation or a weight is a copy, which kNorm makes
+  const int kind = cos_sin ? (is_neox ? kNeox : kPairs) : Hq == 0 && !k_weight && !k_out ? kRaw : kNorm;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == B200_DT_BF16 ? dispatch_rows<__nv_bfloat16>(p, rope, st) : dispatch_rows<__half>(p, rope, st);
+  return dtype == B200_DT_BF16 ? dispatch_rows<__nv_bfloat16>(p, kind, st) : dispatch_rows<__half>(p, kind, st);
 }
 
 }  // namespace
