@@ -590,7 +590,7 @@ typedef struct {
  *   (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)            for rotary_dim / 2 pairs, the other elements stay
  * is_neox: pair i is (i, i + rotary_dim / 2), otherwise (2 i, 2 i + 1).  c and s are elements i and rotary_dim / 2 + i of
  * row positions[t] of cos_sin [max_position, rotary_dim] (NULL: no rotation).  positions are int32, or int64 with
- * positions_i64.  A token whose position is negative is padding: nothing of it is read or written.  One whose position
+ * positions_i64.  A token whose position is negative is padding: nothing of it is written.  One whose position
  * is >= max_position becomes NaN.  q_out / k_out may be q / k themselves.  dtype bf16 or fp16; head_dim a multiple of 16 up
  * to 256, rotary_dim a multiple of 16.  num_q_heads or num_kv_heads may be 0.
  * Stands in for RMSNorm on the heads (python/sglang/srt/layers/layernorm.py) followed by

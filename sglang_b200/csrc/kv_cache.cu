@@ -147,7 +147,7 @@ __device__ __forceinline__ uint4 quantise16(const f2 (&y)[8], float scale) {
 
 constexpr int kStages = 4, kStageBytes = 32 * 32;            // row groups in flight for each warp
 
-// What differs between queries, keys and values, decided once for a warp.
+// The rows of a warp: heads first ... last - 1 of one token's queries, keys or values.
 template <typename T>
 struct Rows {
   const T* src;              // head 0 of the token
@@ -155,12 +155,7 @@ struct Rows {
   T* dst;                    // or nullptr
   int64_t dst_sh;
   const T* weight;           // or nullptr
-  uint8_t* codes;            // head 0 of the token's place in the cache
-  int64_t codes_sh;
-  float* scales;
-  int64_t scales_sh;
-  int first, last;           // the warp's heads
-  bool poisoned;
+  int first, last;
 };
 
 // How a row is treated: taken as it is, normalised (if there is a weight) and not rotated, rotated as neox pairs, rotated as
@@ -170,9 +165,13 @@ enum { kRaw = -1, kNorm = 0, kNeox = 1, kPairs = 2 };
 // With neox pairs a lane of the rotated part holds elements 8l .. 8l + 7 and their partners rot / 2 further on, so that a rotation
 // stays inside the lane; otherwise elements 16l .. 16l + 15.  The weights are multiplied into the cosines and sines, once for all
 // rows; where the position is not in the table, all of these factors are NaN.
+// pos: the token's position (no rotation: 0); slot: its place in the cache (CODES); both were loaded ahead and are looked at only
+// when the first rows are under way.
 template <typename T, int G, int KIND, bool STORE, bool CODES>
-__device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lane, int D, int rot, float eps, const float* table_row) {
+__device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& r, uint32_t ring, int lane, int64_t pos, int64_t slot,
+                                        bool keys) {
   constexpr int RPW = 32 / G;
+  const int D = p.D, rot = p.rot;
   constexpr bool SPLIT = KIND == kNeox, ROPE = KIND == kNeox || KIND == kPairs;
   const int l = lane % G, sub = lane / G;
   const bool in_row = l * 16 < D;
@@ -198,14 +197,21 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
     if (i * RPW < count) fetch(i * RPW);
     sa::cp_async_commit();
   }
+  const bool poisoned = ROPE && pos >= p.max_position;         // a position that the table lacks: NaN, not a read behind it
+  const bool keep = CODES && slot >= 0 && slot < p.num_slots;
+  if ((ROPE && pos < 0) || !(keep || (STORE && r.dst != nullptr))) {     // padding, or nowhere to go: nothing is written
+    sa::cp_async_wait<0>();
+    return;
+  }
+  const float* table_row = ROPE ? p.cos_sin + pos * rot : nullptr;
   // the coefficients, two elements at a time: y' = y ca + partner sa (neox: pairs (e, e + 1) of the first run, then of the second;
   // otherwise each pair is one that is rotated); elements that are not rotated have their weight in ca
   f2 ca[8], sa[8];
   if (KIND != kRaw) {
     f2 w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = both(r.poisoned ? __uint_as_float(0x7fc00000u) : 1.f);
-    if (r.weight != nullptr && in_row && !r.poisoned) {
+    for (int i = 0; i < 8; ++i) w[i] = both(poisoned ? __uint_as_float(0x7fc00000u) : 1.f);
+    if (r.weight != nullptr && in_row && !poisoned) {
       unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o0)), w);
       unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o1)), w + 4);
     }
@@ -216,7 +222,7 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = c;
-        if (!r.poisoned) {
+        if (!poisoned) {
           c = __ldg(reinterpret_cast<const float4*>(table_row + 8 * l + 4 * i));
           s = __ldg(reinterpret_cast<const float4*>(table_row + rot / 2 + 8 * l + 4 * i));
         }
@@ -240,10 +246,17 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
   }
   T* dst = STORE && r.dst != nullptr ? r.dst + (r.first + sub) * r.dst_sh : nullptr;
   const int64_t dst_step = RPW * r.dst_sh;
-  uint8_t* codes = CODES ? r.codes + (r.first + sub) * r.codes_sh : nullptr;
-  const int64_t codes_step = RPW * r.codes_sh;
-  float* scales = CODES ? r.scales + (r.first + sub) * r.scales_sh : nullptr;
-  const int64_t scales_step = RPW * r.scales_sh;
+  uint8_t* codes = nullptr;
+  float* scales = nullptr;
+  int64_t codes_step = 0, scales_step = 0;
+  if (CODES && keep) {
+    const uint32_t page = p.page_shift >= 0 ? static_cast<uint32_t>(slot) >> p.page_shift : static_cast<uint32_t>(slot) / p.page_size;
+    const uint32_t place = static_cast<uint32_t>(slot) - page * p.page_size;
+    const int64_t *cs = keys ? p.kc_s : p.vc_s, *ss = keys ? p.ks_s : p.vs_s;
+    codes = (keys ? p.kc : p.vc) + page * cs[0] + place * cs[1] + (r.first + sub) * cs[2];
+    scales = (keys ? p.ks : p.vs) + page * ss[0] + place * ss[1] + (r.first + sub) * ss[2];
+    codes_step = RPW * cs[2], scales_step = RPW * ss[2];
+  }
   uint32_t from = ring;
 #pragma unroll 1
   for (int i = 0; i < count; i += RPW) {
@@ -263,7 +276,7 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
         float sq = split(sum).x + split(sum).y;
 #pragma unroll
         for (int off = G / 2; off >= 1; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-        const f2 rinv = both(rsqrtf(fmaf(sq, inv_d, eps)));
+        const f2 rinv = both(rsqrtf(fmaf(sq, inv_d, p.eps)));
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = mul(y[e], rinv);
       }
@@ -305,14 +318,14 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
       for (int off = G / 2; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
       const float scale = scale_of(amax);
       const uint4 q = quantise16(y, scale);
-      if (live) {
+      if (live && keep) {
         if constexpr (SPLIT) {
           *reinterpret_cast<uint2*>(codes + o0) = make_uint2(q.x, q.y);
           *reinterpret_cast<uint2*>(codes + o1) = make_uint2(q.z, q.w);
         } else {
           *reinterpret_cast<uint4*>(codes + o0) = q;
         }
-        if (l == 0) *scales = KIND != kRaw && r.poisoned ? __uint_as_float(0x7fc00000u) : scale;
+        if (l == 0) *scales = KIND != kRaw && poisoned ? __uint_as_float(0x7fc00000u) : scale;
       }
       codes += codes_step;
       scales += scales_step;
@@ -321,7 +334,7 @@ __device__ __forceinline__ void do_rows(const Rows<T>& r, uint32_t ring, int lan
 }
 
 template <typename T, int G, int KIND>
-__global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
+__global__ void __launch_bounds__(kThreads, 6) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
   pdl_start();
   constexpr bool ROPE = KIND == kNeox || KIND == kPairs;
   __shared__ __align__(16) uint8_t rings[kThreads / 32 * kStages * kStageBytes];
@@ -333,53 +346,31 @@ __global__ void __launch_bounds__(kThreads, 5) head_rows_kernel(const __grid_con
   if (tok32 >= p.T) return;
   const int64_t tok = tok32;
   int chunk = static_cast<int>(item - tok32 * p.chunks);
+  const int64_t pos = ROPE ? load_index(p.positions, p.pos_i64, tok) : 0;
+  const int64_t slot = p.Hv != 0 && chunk >= p.chunks_q ? load_index(p.slots, p.slots_i64, tok) : -1;
   Rows<T> r = {};
-  const float* table_row = nullptr;
-  int64_t slot = -1;
-  if (p.Hv != 0 && chunk >= p.chunks_q) slot = load_index(p.slots, p.slots_i64, tok);
-  if (ROPE) {
-    const int64_t pos = load_index(p.positions, p.pos_i64, tok);
-    if (pos < 0) return;                                     // padding: nothing of this token is read or written
-    r.poisoned = pos >= p.max_position;                      // a position that the table lacks: NaN, not a read behind it
-    table_row = p.cos_sin + pos * p.rot;
-  }
   if (chunk < p.chunks_q) {
     r.first = chunk * p.heads_q, r.last = min(r.first + p.heads_q, p.Hq);
     r.src = static_cast<const T*>(p.q) + tok * p.q_st, r.src_sh = p.q_sh;
     r.dst = static_cast<T*>(p.q_out) + tok * p.qo_st, r.dst_sh = p.qo_sh;
     r.weight = static_cast<const T*>(p.q_w);
-    do_rows<T, G, KIND, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
+    do_rows<T, G, KIND, true, false>(p, r, ring, lane, pos, -1, false);
     return;
   }
   chunk -= p.chunks_q;
   const bool keys = chunk < p.chunks_kv;
   r.first = (keys ? chunk : chunk - p.chunks_kv) * p.heads_kv, r.last = min(r.first + p.heads_kv, p.Hkv);
-  if (keys) {
-    r.src = static_cast<const T*>(p.k) + tok * p.k_st, r.src_sh = p.k_sh;
+  r.src = keys ? static_cast<const T*>(p.k) + tok * p.k_st : static_cast<const T*>(p.v) + tok * p.v_st;
+  r.src_sh = keys ? p.k_sh : p.v_sh;
+  if constexpr (KIND == kRaw) {
+    do_rows<T, G, kRaw, false, true>(p, r, ring, lane, 0, slot, keys);
+  } else if (keys) {
     if (p.k_out != nullptr) r.dst = static_cast<T*>(p.k_out) + tok * p.ko_st, r.dst_sh = p.ko_sh;
     r.weight = static_cast<const T*>(p.k_w);
-  } else {
-    r.src = static_cast<const T*>(p.v) + tok * p.v_st, r.src_sh = p.v_sh;
-  }
-  const bool keep = slot >= 0 && slot < p.num_slots;
-  if (keep) {
-    const uint32_t page = p.page_shift >= 0 ? static_cast<uint32_t>(slot) >> p.page_shift : static_cast<uint32_t>(slot) / p.page_size;
-    const uint32_t place = static_cast<uint32_t>(slot) - page * p.page_size;
-    r.codes = keys ? p.kc + page * p.kc_s[0] + place * p.kc_s[1] : p.vc + page * p.vc_s[0] + place * p.vc_s[1];
-    r.codes_sh = keys ? p.kc_s[2] : p.vc_s[2];
-    r.scales = keys ? p.ks + page * p.ks_s[0] + place * p.ks_s[1] : p.vs + page * p.vs_s[0] + place * p.vs_s[1];
-    r.scales_sh = keys ? p.ks_s[2] : p.vs_s[2];
-  }
-  if constexpr (KIND == kRaw) {
-    if (keep) do_rows<T, G, kRaw, false, true>(r, ring, lane, p.D, 0, 0.f, nullptr);
-  } else {
-    if (!keys) {
-      if (keep) do_rows<T, G, kRaw, false, true>(r, ring, lane, p.D, 0, 0.f, nullptr);
-    } else if (keep) {
-      do_rows<T, G, KIND, true, true>(r, ring, lane, p.D, p.rot, p.eps, table_row);
-    } else if (r.dst != nullptr) {
-      do_rows<T, G, KIND, true, false>(r, ring, lane, p.D, p.rot, p.eps, table_row);
-    }
+    if (p.Hv != 0) do_rows<T, G, KIND, true, true>(p, r, ring, lane, pos, slot, true);
+    else do_rows<T, G, KIND, true, false>(p, r, ring, lane, pos, -1, true);
+  } else if (pos >= 0) {
+    do_rows<T, G, kRaw, false, true>(p, r, ring, lane, 0, slot, false);
   }
 }
 

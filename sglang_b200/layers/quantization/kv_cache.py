@@ -37,7 +37,7 @@ def qk_norm_rope_store_kv_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """qk_norm_rope (layers/rotary_embedding.py) and store_kv_fp8 of the rotated keys and of v, one pass over the qkv output.
     Returns q_out (new and contiguous unless given; may be q itself).  The keys are quantised from fp32, without a rounding to
     16 bits in between; k_out, if given, receives them in k's type as well.  A token with a negative position is padding:
-    nothing of it is read or written, whatever its slot."""
+    nothing of it is written, whatever its slot."""
     return _lib.host().head_rows("qk_norm_rope_store_kv_fp8", q, k, v, positions, cos_sin_cache, q_weight, k_weight, norm_eps,
                                  is_neox, q_out, k_out, False, k_cache, v_cache, k_scale, v_scale, slots)[0]
 
