@@ -285,6 +285,10 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool in
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool in) {   // otherwise nothing happens
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}\n"
+               ::"r"(dst), "l"(src), "r"(in ? 1u : 0u) : "memory");
+}
 // 8 or 16 bytes copied, or zeros written and the source not read.
 template <int BYTES>
 __device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, bool in) {

@@ -16,7 +16,7 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 64;
 
 struct HeadRowsParams {
   const void *q, *k, *v;
@@ -77,21 +77,31 @@ __device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& v, f2* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// The sixteen elements of two vectors as eight pairs: (2e, 2e + 1); or, TURNED, first elements 4e and 4e + 2, then elements 4e + 1
+// and 4e + 3, so that neighbours which are rotated with one another lie in the same half of two pairs.
+template <typename T, bool TURNED>
+__device__ __forceinline__ void unpack16(const uint4& lo, const uint4& hi, f2 (&f)[8]) {
+  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = to_f2(w[i], static_cast<T*>(nullptr));
-    f[i] = make_f2(p.x, p.y);
+  for (int i = 0; i < 8; i += 2) {
+    const float2 p = to_f2(w[i], static_cast<T*>(nullptr)), q = to_f2(w[i + 1], static_cast<T*>(nullptr));
+    f[TURNED ? i / 2 : i] = TURNED ? make_f2(p.x, q.x) : make_f2(p.x, p.y);
+    f[TURNED ? i / 2 + 4 : i + 1] = TURNED ? make_f2(p.y, q.y) : make_f2(q.x, q.y);
   }
 }
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const f2* f) {
+// Back in order: pair i of the elements.
+template <bool TURNED>
+__device__ __forceinline__ float2 pair_of(const f2 (&f)[8], int i) {
+  if (!TURNED) return split(f[i]);
+  const float2 a = split(f[i / 2]), b = split(f[i / 2 + 4]);
+  return i % 2 == 0 ? make_float2(a.x, b.x) : make_float2(a.y, b.y);
+}
+template <typename T, bool TURNED>
+__device__ __forceinline__ uint4 pack8(const f2 (&f)[8], int half) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 p = split(f[i]);
+    const float2 p = pair_of<TURNED>(f, 4 * half + i);
     w[i] = from_f2(p.x, p.y, static_cast<T*>(nullptr));
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -111,34 +121,36 @@ __device__ __forceinline__ float scale_of(float amax) {
 // for every scale whose significand is not all ones; with such a scale, a non-finite one or a NaN among the lane's elements the
 // quotients are taken literally.  Computed as -(y / scale), q0 = y (-r), q0 + (y + q0 scale)(-r), and the codes' signs flipped:
 // in this form a zero keeps its sign.
+template <bool TURNED>
 __device__ __forceinline__ uint4 quantise16(const f2 (&y)[8], float scale) {
   const uint32_t bits = __float_as_uint(scale);
   bool literal = (bits & 0x007fffffu) == 0x007fffffu || (bits & 0x7f800000u) == 0x7f800000u;
   const f2 nr = both(-__frcp_rn(scale)), s = both(scale);
+  f2 t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const f2 q0 = mul(y[i], nr);
+    t[i] = fma(fma(q0, s, y[i]), nr, q0);
+  }
   uint32_t w[4], nan = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t half[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f2 q0 = mul(y[2 * i + j], nr);
-      const float2 t = split(fma(fma(q0, s, y[2 * i + j]), nr, q0));
-      half[j] = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
-    }
-    w[i] = (half[0] | (half[1] << 16)) ^ 0x80808080u;
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(pair_of<TURNED>(t, 2 * i), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(pair_of<TURNED>(t, 2 * i + 1), __NV_SATFINITE, __NV_E4M3);
+    w[i] = (lo | (hi << 16)) ^ 0x80808080u;
     nan |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;               // bit 7 of a byte: its code was 0x7f or 0xff
   }
   literal |= (nan & 0x80808080u) != 0;
   if (literal) {                                             // fminf(fmaxf(y / scale, -448), 448): a NaN becomes -448
-    float t[16];
+    float v[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[2 * i] = split(y[i]).x, t[2 * i + 1] = split(y[i]).y;
+    for (int i = 0; i < 8; ++i) v[2 * i] = pair_of<TURNED>(y, i).x, v[2 * i + 1] = pair_of<TURNED>(y, i).y;
 #pragma unroll 1
-    for (int i = 0; i < 16; ++i) t[i] = fminf(fmaxf(__fdiv_rn(t[i], scale), -448.f), 448.f);
+    for (int i = 0; i < 16; ++i) v[i] = fminf(fmaxf(__fdiv_rn(v[i], scale), -448.f), 448.f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * i], t[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * i + 2], t[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
       w[i] = lo | (hi << 16);
     }
   }
@@ -172,22 +184,26 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
                                         bool keys) {
   constexpr int RPW = 32 / G;
   const int D = p.D, rot = p.rot;
-  constexpr bool SPLIT = KIND == kNeox, ROPE = KIND == kNeox || KIND == kPairs;
+  constexpr bool SPLIT = KIND == kNeox, TURNED = KIND == kPairs, ROPE = SPLIT || TURNED;
   const int l = lane % G, sub = lane / G;
   const bool in_row = l * 16 < D;
   const bool turned = ROPE && l * 16 < rot;
   const int o0 = SPLIT && turned ? 8 * l : 16 * l, o1 = SPLIT && turned ? rot / 2 + 8 * l : 16 * l + 8;
   const float inv_d = 1.f / static_cast<float>(D);
-  // ring: this lane's 32 bytes of each of the next kStages row groups; only the lane itself reads them
+  // ring: this lane's 32 bytes of each of the next kStages row groups; only the lane itself reads them.  A lane behind the end of
+  // its rows has zeros there from the start.
   const uint32_t ring_end = ring + kStages * kStageBytes;
   const int heads = in_row ? r.last - r.first - sub : 0;      // of this lane's, counted by RPW
-  const T* src = r.src + (r.first + sub) * r.src_sh;
+  if (!in_row)
+    for (uint32_t at = ring; at != ring_end; at += kStageBytes / 2)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+  const T* src = r.src + (r.first + sub) * r.src_sh + o0;
   const int64_t src_step = RPW * r.src_sh;
+  const int run = SPLIT ? o1 - o0 : 8;
   uint32_t to = ring;
   auto fetch = [&](int i) {                                   // row group i / RPW
-    const bool live = i < heads;
-    sa::cp_async_or_zero<16>(to, live ? src + o0 : r.src, live);
-    sa::cp_async_or_zero<16>(to + kStageBytes / 2, live ? src + o1 : r.src, live);
+    sa::cp_async16_if(to, src, i < heads);
+    sa::cp_async16_if(to + kStageBytes / 2, src + run, i < heads);
     src += src_step;
     to = to + kStageBytes == ring_end ? ring : to + kStageBytes;
   };
@@ -204,16 +220,15 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
     return;
   }
   const float* table_row = ROPE ? p.cos_sin + pos * rot : nullptr;
-  // the coefficients, two elements at a time: y' = y ca + partner sa (neox: pairs (e, e + 1) of the first run, then of the second;
-  // otherwise each pair is one that is rotated); elements that are not rotated have their weight in ca
+  // the coefficients: y' = y ca + partner sa, the partner of the i-th pair of elements being the (i + 4)-th; elements that are not
+  // rotated have their weight in ca
   f2 ca[8], sa[8];
   if (KIND != kRaw) {
     f2 w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = both(poisoned ? __uint_as_float(0x7fc00000u) : 1.f);
     if (r.weight != nullptr && in_row && !poisoned) {
-      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o0)), w);
-      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.weight + o1)), w + 4);
+      unpack16<T, TURNED>(__ldg(reinterpret_cast<const uint4*>(r.weight + o0)), __ldg(reinterpret_cast<const uint4*>(r.weight + o1)), w);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) ca[i] = w[i];
@@ -231,16 +246,10 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 mine = split(w[i]);
-        if (SPLIT) {
-          const int j = 2 * (i % 4);
-          const float2 other = split(w[(i + 4) % 8]);
-          ca[i] = make_f2(cc[j] * mine.x, cc[j + 1] * mine.y);
-          sa[i] = i < 4 ? make_f2(-ss[j] * other.x, -ss[j + 1] * other.y) : make_f2(ss[j] * other.x, ss[j + 1] * other.y);
-        } else {
-          ca[i] = make_f2(cc[i] * mine.x, cc[i] * mine.y);
-          sa[i] = make_f2(-ss[i] * mine.y, ss[i] * mine.x);
-        }
+        const int j = 2 * (i % 4);
+        const float2 mine = split(w[i]), other = split(w[(i + 4) % 8]);
+        ca[i] = make_f2(cc[j] * mine.x, cc[j + 1] * mine.y);
+        sa[i] = i < 4 ? make_f2(-ss[j] * other.x, -ss[j + 1] * other.y) : make_f2(ss[j] * other.x, ss[j + 1] * other.y);
       }
     }
   }
@@ -265,8 +274,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
     sa::cp_async_wait<kStages - 1>();
     const bool live = i < heads;
     f2 y[8];
-    unpack8<T>(sa::ld_v4(from), y);
-    unpack8<T>(sa::ld_v4(from + kStageBytes / 2), y + 4);
+    unpack16<T, TURNED>(sa::ld_v4(from), sa::ld_v4(from + kStageBytes / 2), y);
     from = from + kStageBytes == ring_end ? ring : from + kStageBytes;
     if (KIND != kRaw) {
       if (r.weight != nullptr) {
@@ -281,19 +289,11 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
         for (int e = 0; e < 8; ++e) y[e] = mul(y[e], rinv);
       }
       if (turned) {
-        if constexpr (SPLIT) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f2 a = y[e], b = y[e + 4];
-            y[e] = fma(a, ca[e], mul(b, sa[e]));
-            y[e + 4] = fma(b, ca[e + 4], mul(a, sa[e + 4]));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 mine = split(y[e]);
-            y[e] = fma(y[e], ca[e], mul(make_f2(mine.y, mine.x), sa[e]));
-          }
+        for (int e = 0; e < 4; ++e) {
+          const f2 a = y[e], b = y[e + 4];
+          y[e] = fma(a, ca[e], mul(b, sa[e]));
+          y[e + 4] = fma(b, ca[e + 4], mul(a, sa[e + 4]));
         }
       } else {
 #pragma unroll
@@ -302,8 +302,8 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
     }
     if (STORE && dst != nullptr) {
       if (live) {
-        *reinterpret_cast<uint4*>(dst + o0) = pack8<T>(y);
-        *reinterpret_cast<uint4*>(dst + o1) = pack8<T>(y + 4);
+        *reinterpret_cast<uint4*>(dst + o0) = pack8<T, TURNED>(y, 0);
+        *reinterpret_cast<uint4*>(dst + o1) = pack8<T, TURNED>(y, 1);
       }
       dst += dst_step;
     }
@@ -317,7 +317,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
 #pragma unroll
       for (int off = G / 2; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
       const float scale = scale_of(amax);
-      const uint4 q = quantise16(y, scale);
+      const uint4 q = quantise16<TURNED>(y, scale);
       if (live && keep) {
         if constexpr (SPLIT) {
           *reinterpret_cast<uint2*>(codes + o0) = make_uint2(q.x, q.y);
@@ -334,7 +334,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
 }
 
 template <typename T, int G, int KIND>
-__global__ void __launch_bounds__(kThreads, 6) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
+__global__ void __launch_bounds__(kThreads, 12) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
   pdl_start();
   constexpr bool ROPE = KIND == kNeox || KIND == kPairs;
   __shared__ __align__(16) uint8_t rings[kThreads / 32 * kStages * kStageBytes];
