@@ -11,7 +11,7 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w
 //   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)     neox: b = a + rot / 2; otherwise neighbours a = 2i, b = 2i + 1
 //   scale = max(1e-10, max|y|) / 448,  code = e4m3(y / scale)     correctly rounded quotient, as in the group quantiser
-#include "common.cuh"
+#include "gemm_common.cuh"
 
 namespace b200 {
 namespace {
@@ -174,8 +174,9 @@ struct Rows {
 // neighbouring pairs.
 enum { kRaw = -1, kNorm = 0, kNeox = 1, kPairs = 2 };
 
-// With neox pairs a lane of the rotated part holds elements 8l .. 8l + 7 and their partners rot / 2 further on, so that a rotation
-// stays inside the lane; otherwise elements 16l .. 16l + 15.  The weights are multiplied into the cosines and sines, once for all
+// A lane holds two runs of eight elements, half of the row apart: a group's 16-byte accesses are then neighbours (with sixteen
+// elements in one run every access took half of a sector, and 8192 tokens of 36 heads 36.8 us).  With neox pairs the runs are half
+// of the rotated part apart, so that a rotation stays inside the lane, and half of the rest in the rest.  The weights are multiplied into the cosines and sines, once for all
 // rows; where the position is not in the table, all of these factors are NaN.
 // pos: the token's position (no rotation: 0); slot: its place in the cache (CODES); both were loaded ahead and are looked at only
 // when the first rows are under way.
@@ -187,8 +188,11 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
   constexpr bool SPLIT = KIND == kNeox, TURNED = KIND == kPairs, ROPE = SPLIT || TURNED;
   const int l = lane % G, sub = lane / G;
   const bool in_row = l * 16 < D;
-  const bool turned = ROPE && l * 16 < rot;
-  const int o0 = SPLIT && turned ? 8 * l : 16 * l, o1 = SPLIT && turned ? rot / 2 + 8 * l : 16 * l + 8;
+  // the lane's two runs of eight, and whether each is rotated
+  const bool tail = SPLIT && l * 16 >= rot;
+  const int o0 = tail ? rot + 8 * (l - rot / 16) : 8 * l;
+  const int o1 = o0 + (SPLIT ? (tail ? D - rot : rot) / 2 : D / 2);
+  const bool turn0 = ROPE && (SPLIT ? !tail : o0 < rot), turn1 = ROPE && (SPLIT ? !tail : o1 < rot);
   const float inv_d = 1.f / static_cast<float>(D);
   // ring: this lane's 32 bytes of each of the next kStages row groups; only the lane itself reads them.  A lane behind the end of
   // its rows has zeros there from the start.
@@ -199,7 +203,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
   const T* src = r.src + (r.first + sub) * r.src_sh + o0;
   const int64_t src_step = RPW * r.src_sh;
-  const int run = SPLIT ? o1 - o0 : 8;
+  const int run = o1 - o0;
   uint32_t to = ring;
   auto fetch = [&](int i) {                                   // row group i / RPW
     sa::cp_async16_if(to, src, i < heads);
@@ -232,14 +236,15 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) ca[i] = w[i];
-    if (turned) {
+    if (turn0) {
       float cc[8], ss[8];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = c;
-        if (!poisoned) {
-          c = __ldg(reinterpret_cast<const float4*>(table_row + 8 * l + 4 * i));
-          s = __ldg(reinterpret_cast<const float4*>(table_row + rot / 2 + 8 * l + 4 * i));
+        if (!poisoned && (i == 0 || turn1)) {
+          const float* at = table_row + (SPLIT ? 8 * l + 4 * i : (i == 0 ? o0 : o1) / 2);
+          c = __ldg(reinterpret_cast<const float4*>(at));
+          s = __ldg(reinterpret_cast<const float4*>(at + rot / 2));
         }
         cc[4 * i] = c.x, cc[4 * i + 1] = c.y, cc[4 * i + 2] = c.z, cc[4 * i + 3] = c.w;
         ss[4 * i] = s.x, ss[4 * i + 1] = s.y, ss[4 * i + 2] = s.z, ss[4 * i + 3] = s.w;
@@ -248,6 +253,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
       for (int i = 0; i < 8; ++i) {
         const int j = 2 * (i % 4);
         const float2 mine = split(w[i]), other = split(w[(i + 4) % 8]);
+        if (i % 4 >= 2 && !turn1) continue;
         ca[i] = make_f2(cc[j] * mine.x, cc[j + 1] * mine.y);
         sa[i] = i < 4 ? make_f2(-ss[j] * other.x, -ss[j + 1] * other.y) : make_f2(ss[j] * other.x, ss[j + 1] * other.y);
       }
@@ -288,16 +294,19 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = mul(y[e], rinv);
       }
-      if (turned) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f2 a = y[e], b = y[e + 4];
-          y[e] = fma(a, ca[e], mul(b, sa[e]));
-          y[e + 4] = fma(b, ca[e + 4], mul(a, sa[e + 4]));
+      for (int run2 = 0; run2 < 4; run2 += 2) {                // pairs 0, 1, 4, 5: with neighbouring pairs the first run; 2, 3, 6, 7
+        if (run2 == 0 ? turn0 : turn1) {
+#pragma unroll
+          for (int e = run2; e < run2 + 2; ++e) {
+            const f2 a = y[e], b = y[e + 4];
+            y[e] = fma(a, ca[e], mul(b, sa[e]));
+            y[e + 4] = fma(b, ca[e + 4], mul(a, sa[e + 4]));
+          }
+        } else {
+#pragma unroll
+          for (int e = run2; e < run2 + 2; ++e) y[e] = mul(y[e], ca[e]), y[e + 4] = mul(y[e + 4], ca[e + 4]);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = mul(y[e], ca[e]);
       }
     }
     if (STORE && dst != nullptr) {
@@ -319,12 +328,8 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
       const float scale = scale_of(amax);
       const uint4 q = quantise16<TURNED>(y, scale);
       if (live && keep) {
-        if constexpr (SPLIT) {
-          *reinterpret_cast<uint2*>(codes + o0) = make_uint2(q.x, q.y);
-          *reinterpret_cast<uint2*>(codes + o1) = make_uint2(q.z, q.w);
-        } else {
-          *reinterpret_cast<uint4*>(codes + o0) = q;
-        }
+        *reinterpret_cast<uint2*>(codes + o0) = make_uint2(q.x, q.y);
+        *reinterpret_cast<uint2*>(codes + o1) = make_uint2(q.z, q.w);
         if (l == 0) *scales = KIND != kRaw && poisoned ? __uint_as_float(0x7fc00000u) : scale;
       }
       codes += codes_step;
@@ -445,6 +450,7 @@ struct KvLoadParams {
   int64_t ko_st, ko_sh, vo_st, vo_sh;
   uint32_t num_pages, page_size, table_cols;
   int batch, Hkv, D;
+  bool wide;                 // rows of the outputs begin at multiples of 32 bytes
 };
 
 constexpr int kLoadThreads = 256, kLoadTokens = 16, kLoadUnroll = 4;
@@ -534,8 +540,12 @@ __global__ void __launch_bounds__(kLoadThreads) kv_load_kernel(const __grid_cons
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hr));
         o[i] = from_f2(f.x * scale[u], f.y * scale[u], static_cast<T*>(nullptr));
       }
-      reinterpret_cast<uint4*>(dst[u])[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      reinterpret_cast<uint4*>(dst[u])[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      if (p.wide) {
+        st_global_32(dst[u], o);
+      } else {
+        reinterpret_cast<uint4*>(dst[u])[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4*>(dst[u])[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
     }
   }
 }
@@ -652,6 +662,7 @@ extern "C" int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_
   p.indptr = indptr, p.starts = starts, p.batch = static_cast<int>(batch), p.tokens = tokens;
   p.num_pages = static_cast<uint32_t>(cache->num_pages), p.page_size = static_cast<uint32_t>(cache->page_size);
   p.Hkv = num_kv_heads, p.D = head_dim;
+  p.wide = ((p.ko_st | p.ko_sh | p.vo_st | p.vo_sh) % 16 == 0) && ((reinterpret_cast<uintptr_t>(ko) | reinterpret_cast<uintptr_t>(vo)) & 31u) == 0;
   const int64_t blocks = (tokens + kLoadTokens - 1) / kLoadTokens;
   if (blocks > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
   const dim3 grid(static_cast<unsigned>(blocks), 2);

@@ -72,7 +72,8 @@ def _cache(pages, page, H, D, seed=0):
 @pytest.mark.parametrize("T,Hq,Hkv,D,rot,neox", [
     (1, 64, 8, 128, 128, True), (1, 1, 1, 16, 16, False), (2, 5, 1, 48, 32, True), (3, 7, 2, 80, 80, True),
     (17, 8, 8, 64, 32, False), (65, 12, 3, 96, 96, True), (33, 4, 4, 192, 64, True), (129, 3, 1, 256, 256, False),
-    (700, 64, 8, 128, 128, True), (1500, 32, 4, 128, 64, False), (9, 0, 2, 32, 16, True),
+    (700, 64, 8, 128, 128, True), (1500, 32, 4, 128, 64, False), (9, 0, 2, 32, 16, True), (12, 3, 2, 64, 48, False),
+    (21, 5, 1, 96, 80, False), (14, 2, 2, 112, 64, True), (6, 9, 2, 240, 16, True),
 ])
 def test_norm_rope(T, Hq, Hkv, D, rot, neox, dtype):
     from sglang_b200.layers.rotary_embedding import qk_norm_rope
