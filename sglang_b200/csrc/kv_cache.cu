@@ -453,18 +453,18 @@ struct KvLoadParams {
   bool wide;                 // rows of the outputs begin at multiples of 32 bytes
 };
 
-constexpr int kLoadThreads = 256, kLoadTokens = 16, kLoadUnroll = 4;
+constexpr int kLoadThreads = 256, kLoadUnroll = 2;
 
 // out[i] = code * scale for the tokens of all sequences, packed: row i belongs to the sequence b with
-// indptr[b] <= i < indptr[b + 1] and holds its token starts[b] + i - indptr[b].  A block takes kLoadTokens rows of keys or of
+// indptr[b] <= i < indptr[b + 1] and holds its token starts[b] + i - indptr[b].  A block takes TOKENS rows of keys or of
 // values (blockIdx.y).  Its first warp finds the rows' places: the sequence of the first by a 32-way search of indptr, those
-// of the others by walking on from there.  Then each thread turns 16 codes (one 16-byte load) into 32 bytes at a time, four
+// of the others by walking on from there.  Then each thread turns 16 codes (one 16-byte load) into 32 bytes at a time, two
 // of them in flight.
-template <typename T>
+template <typename T, int TOKENS>
 __global__ void __launch_bounds__(kLoadThreads) kv_load_kernel(const __grid_constant__ KvLoadParams p) {
   pdl_start();
-  __shared__ int s_page[kLoadTokens], s_at[kLoadTokens];      // page -1: behind the last sequence; -2: no such page
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kLoadTokens;
+  __shared__ int s_page[TOKENS], s_at[TOKENS];      // page -1: behind the last sequence; -2: no such page
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * TOKENS;
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int lo = 0, n = p.batch;                                  // the answer is lo + (entries of the n from lo on that are <= row0)
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kLoadThreads) kv_load_kernel(const __grid_cons
       n = step > 1 ? min(step - 1, n - whole * step) : 0;
     }
     const int64_t row = row0 + lane;
-    if (lane < kLoadTokens) {
+    if (lane < TOKENS) {
       int page = -1, at = 0;
       if (row < p.tokens) {
         int b = lo;
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kLoadThreads) kv_load_kernel(const __grid_cons
   const int64_t* ss = keys ? p.ks_s : p.vs_s;
   T* out = static_cast<T*>(keys ? p.k_out : p.v_out);
   const int64_t st = keys ? p.ko_st : p.vo_st, sh = keys ? p.ko_sh : p.vo_sh;
-  const int per_head = p.D / 16, vecs = p.Hkv * per_head, total = vecs * kLoadTokens;
+  const int per_head = p.D / 16, vecs = p.Hkv * per_head, total = vecs * TOKENS;
   for (int base = threadIdx.x; base < total; base += kLoadThreads * kLoadUnroll) {
     uint4 codes[kLoadUnroll];
     float scale[kLoadUnroll];
@@ -663,11 +663,19 @@ extern "C" int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_
   p.num_pages = static_cast<uint32_t>(cache->num_pages), p.page_size = static_cast<uint32_t>(cache->page_size);
   p.Hkv = num_kv_heads, p.D = head_dim;
   p.wide = ((p.ko_st | p.ko_sh | p.vo_st | p.vo_sh) % 16 == 0) && ((reinterpret_cast<uintptr_t>(ko) | reinterpret_cast<uintptr_t>(vo)) & 31u) == 0;
-  const int64_t blocks = (tokens + kLoadTokens - 1) / kLoadTokens;
+  const int sms = sm_count();
+  if (sms <= 0) return B200_ERR_CUDA;
+  // Rows of a block: 32 where that gives every SM its eight blocks (131001 x 8 x 128: 137 us, with 16 rows 148, with 8 155), else 8
+  // (401 x 8 x 128: 3.1 us, with 32 rows 5.6).
+  const int rows = (tokens + 31) / 32 * 2 >= 8LL * sms ? 32 : 8;
+  const int64_t blocks = (tokens + rows - 1) / rows;
   if (blocks > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
   const dim3 grid(static_cast<unsigned>(blocks), 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  B200_CUDA_TRY(dtype == B200_DT_BF16 ? launch_pdl(kv_load_kernel<__nv_bfloat16>, grid, dim3(kLoadThreads), 0, st, p)
-                                      : launch_pdl(kv_load_kernel<__half>, grid, dim3(kLoadThreads), 0, st, p));
+  auto go = [&](auto kern) { return launch_pdl(kern, grid, dim3(kLoadThreads), 0, st, p); };
+  if (dtype == B200_DT_BF16)
+    B200_CUDA_TRY(rows == 32 ? go(kv_load_kernel<__nv_bfloat16, 32>) : go(kv_load_kernel<__nv_bfloat16, 8>));
+  else
+    B200_CUDA_TRY(rows == 32 ? go(kv_load_kernel<__half, 32>) : go(kv_load_kernel<__half, 8>));
   return B200_OK;
 }

@@ -128,7 +128,7 @@ def test_infinities_and_nan_stay_in_their_head():
 
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("T,H,D,page", [(1, 1, 16, 1), (1, 8, 128, 16), (7, 2, 80, 3), (33, 8, 128, 16), (200, 16, 64, 128),
-                                        (1023, 3, 256, 7), (2100, 8, 128, 64), (5, 2, 96, 32), (5, 2, 48, 1)])
+                                        (1023, 3, 256, 7), (2500, 8, 128, 64), (1700, 33, 32, 16), (5, 2, 96, 32), (5, 2, 48, 1)])
 def test_store_gives_the_group_quantiser_s_codes(T, H, D, page, dtype):
     from sglang_b200.layers.quantization.kv_cache import store_kv_fp8
     qkv, _ = _inputs(T, 0, H, D, dtype, 7 * T + D)
@@ -252,7 +252,8 @@ def _paged(lens, page, starts=None, seed=0):
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("lens,page,H,D", [([1], 16, 8, 128), ([0, 5, 0, 0, 17, 0], 4, 2, 64), ([100, 1, 203, 97], 16, 8, 128),
                                            ([33] * 70 + [0] * 70 + [2], 32, 1, 16), ([3000, 5, 1111], 64, 4, 256), ([7, 9], 1, 3, 80),
-                                           ([1] * 1500, 8, 2, 32), ([0, 0, 0], 8, 2, 32)])
+                                           ([1] * 1500, 8, 2, 32), ([0, 0, 0], 8, 2, 32),
+                                           ([19000, 0, 37, 1], 16, 1, 16), ([9999, 12345], 64, 2, 48)])
 def test_load(lens, page, H, D, dtype):
     from sglang_b200.layers.quantization.kv_cache import load_kv_fp8
     for starts in (None, [(5 * b) % 23 for b in range(len(lens))]):
