@@ -17,6 +17,8 @@
 // that adds at most half a step of h (2^-9 for bf16) to the adapter's part of the sum, less than the rounding of out adds.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "gemm_common.cuh"
 
 namespace b200 {
@@ -275,18 +277,22 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __
 
 // A cluster of `splits` blocks computes up to n_alloc columns of h for one tile of up to 128 tokens, each block a part of K.
 // tcgen05: D [128 tokens x columns] += x [128 x 64] A^T [64 x columns], both operands K-major in shared memory with the
-// 128-byte swizzle.  Warps 0 and 2 fetch half of the tile's x each, with one TMA box where its tokens are neighbours, else eight
-// rows at a time or gathered four by four; warp 3 fetches the rows of A below the adapter's rank, box by box, the slices packed
+// 128-byte swizzle.  Warps 0 and 2 fetch half of the tile's x each, with one TMA box where its tokens are neighbours, else with
+// smaller ones or gathered four by four; warp 3 fetches the rows of A below the adapter's rank, box by box, the slices packed
 // one behind the other; warp 1 issues the products.  Then all four warps read the sums out of tensor memory and, with several
 // blocks, add them in block order through distributed shared memory.  The number of TMA instructions counts: with one warp
 // issuing forty boxes of eight rows per k-block, a k-block took 2.2 us (8191 x 8192 and 192 columns: 141 us; rows copied by all
-// threads with 16-byte asynchronous copies: 174 us).
-constexpr int kTileThreads = 128, kBlockK = 64, kMaxTileStages = 8, kMaxColumns = 256;
+// threads with 16-byte asynchronous copies: 174 us; four warps with boxes of 32 rows: 45 us, two with 64: 38).
+constexpr int kTileThreads = 128, kTileSmem = 201 * 1024, kBlockK = 64, kMaxTileStages = 8, kMaxColumns = 256;
 constexpr uint32_t kXBytes = kLargeRows * kBlockK * 2;
 
+struct ShrinkMaps {
+  CUtensorMap x[5], a, a_whole;        // x in boxes of 1, 8, 16, 32 and 64 rows; A in boxes of a_box rows, and of an adapter's all
+};
 struct ShrinkTiles {
   int64_t K, h_ld;
   int R, slices, n_alloc, splits, stages, a_box;
+  bool a_whole;
   int* status;
 };
 
@@ -310,10 +316,7 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap x1_map,
-                                                                         const __grid_constant__ CUtensorMap x8_map,
-                                                                         const __grid_constant__ CUtensorMap x64_map,
-                                                                         const __grid_constant__ CUtensorMap a_map,
+__global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const __grid_constant__ ShrinkMaps maps,
                                                                          PlanView plan, T* __restrict__ h,
                                                                          const __grid_constant__ ShrinkTiles p) {
   pdl_wait();
@@ -363,20 +366,26 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const _
   const int kb0 = static_cast<int>(nkb * split / p.splits), count = static_cast<int>(nkb * (split + 1) / p.splits) - kb0;
   bool ok = true;
   if (warp != 1) {
-    // x: rows 64 half ... of the tile, lanes 0-7 with eight each (tokens are in ascending order, so the ends of a run tell whether
-    // it has gaps; rows behind the tile's last are any rows, their sums are not used).  A: lane by lane one box.
+    // x: 64 of the tile's rows, lanes 0-7 with eight each (tokens are in ascending order, so the ends of a run tell whether it has
+    // gaps; rows behind the tile's last are any rows, their sums are not used).  The largest boxes that have none are taken: box is
+    // the number of rows that this lane fetches in one, 4 for two gathers, 0 if an earlier lane has its rows.
     const int half = 64 * (warp / 2), first = half + 8 * (lane % 8);
-    int y[8], last = 0;
-    bool run64 = false, run8 = false;
+    int y[8], box = 0;
     if (warp != 3) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = __ldg(plan.perm + tile.y + min(first + i, rows - 1));
-      last = __ldg(plan.perm + tile.y + min(half + 63, rows - 1));
-      const int head = __shfl_sync(0xffffffffu, y[0], 0);
-      run64 = half >= rows || last - head == min(half + 63, rows - 1) - half;
-      run8 = first >= rows || y[7] - y[0] == min(first + 7, rows - 1) - first;
+      box = y[7] - y[0] == min(first + 7, rows - 1) - min(first, rows - 1) ? 8 : 4;
+#pragma unroll
+      for (int size = 16; size <= 64; size *= 2) {
+        const int lanes = size / 8, from = lane % 8 / lanes * lanes, begin = half + 8 * from;
+        const int y0 = __shfl_sync(0xffffffffu, y[0], from), y1 = __shfl_sync(0xffffffffu, y[7], from + lanes - 1);
+        if (y1 - y0 == min(begin + size - 1, rows - 1) - min(begin, rows - 1)) box = lane % 8 == from ? size : 0;
+      }
+      if (lane >= 8) box = 0;
     }
-    const int boxes = n / p.a_box, j = c0 + lane * p.a_box;
+    // A: lane by lane one box, or one for all of it where the adapter has the full rank
+    const bool whole = p.a_whole && rank == p.R;
+    const int boxes = whole ? 1 : n / p.a_box, j = c0 + lane * p.a_box;
     const int ay = warp == 3 && lane < boxes ? tile.x * p.slices * p.R + j / width * p.R + j % width : 0;
     const uint32_t bytes = warp == 3 ? n * (kBlockK * 2) : kXBytes / 2;
     int stage = 0, phase = 1;
@@ -394,16 +403,12 @@ __global__ void __launch_bounds__(kTileThreads) lora_shrink_tiles_kernel(const _
       if (lane == 0) sa::expect_tx(bar, bytes);
       __syncwarp();
       if (warp == 3) {
-        if (lane < boxes) sa::tma_load_2d(to + lane * p.a_box * 128, &a_map, bar, k, ay);
-      } else if (run64) {
-        if (lane == 0) sa::tma_load_2d(to, &x64_map, bar, k, y[0]);
-      } else if (lane < 8) {
-        if (run8) {
-          sa::tma_load_2d(to + lane * 1024, &x8_map, bar, k, y[0]);
-        } else {
-          sa::tma_gather4(to + lane * 1024, &x1_map, bar, k, y[0], y[1], y[2], y[3]);
-          sa::tma_gather4(to + lane * 1024 + 512, &x1_map, bar, k, y[4], y[5], y[6], y[7]);
-        }
+        if (lane < boxes) sa::tma_load_2d(to + lane * p.a_box * 128, whole ? &maps.a_whole : &maps.a, bar, k, ay);
+      } else if (box == 4) {
+        sa::tma_gather4(to + lane * 1024, &maps.x[0], bar, k, y[0], y[1], y[2], y[3]);
+        sa::tma_gather4(to + lane * 1024 + 512, &maps.x[0], bar, k, y[4], y[5], y[6], y[7]);
+      } else if (box != 0) {
+        sa::tma_load_2d(to + lane * 1024, box == 64 ? &maps.x[4] : box == 32 ? &maps.x[3] : box == 16 ? &maps.x[2] : &maps.x[1], bar, k, y[0]);
       }
       if (++stage == p.stages) stage = 0, phase ^= 1;
     }
@@ -790,6 +795,31 @@ cudaError_t launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
+// How many clusters of n blocks of the large shrink, one block an SM, run at once on the current device; asked once for each n.
+constexpr int kMaxSplits = 8;
+template <typename Kern>
+int cluster_slots(Kern kern, int n) {
+  static std::atomic<int> known[64][kMaxSplits + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int v = known[dev][n].load(std::memory_order_relaxed);
+  if (v != 0) return v;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = n, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(n);
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = kTileSmem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&v, kern, &cfg) != cudaSuccess)
+    return 0;
+  known[dev][n].store(v, std::memory_order_relaxed);
+  return v;
+}
+
 template <typename T>
 int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, int64_t tokens, int64_t tiles, int64_t K, int R, int slices, T* h,
            int64_t h_ld, cudaStream_t st) {
@@ -817,21 +847,25 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
   p.a_box = R % 32 == 0 ? 32 : R % 16 == 0 ? 16 : 8;       // rows of A that are fetched at a time; slices begin at multiples
   p.n_alloc = cols < kMaxColumns ? (cols + 15) / 16 * 16 : kMaxColumns;
   const int passes = (cols + kMaxColumns - 1) / kMaxColumns;
-  // As many blocks a tile as give every SM at most one, the tiles being about as many as whole ones.
+  // As many blocks a tile as let all tiles run at once, one block an SM.  Of a cluster's blocks no two may lie in different
+  // processing clusters of the chip, so fewer clusters fit than SMs / size (of four blocks 33, of three 45); a batch has about an
+  // eighth to a quarter more tiles than whole ones.  37 tiles of 4096 x 7168 x 64: four blocks in two waves 38 us, three in one 28.
+  const int64_t whole = (tokens + kLargeRows - 1) / kLargeRows, about = passes * (whole + (adapters < whole / 4 ? adapters : whole / 4));
   p.splits = 1;
-  while (p.splits < 8 && 2 * p.splits * passes * ((tokens + kLargeRows - 1) / kLargeRows) <= sms && 2 * p.splits * kBlockK <= K) p.splits *= 2;
+  for (int n = 2; n <= kMaxSplits; ++n)
+    if (static_cast<int64_t>(n) * kBlockK <= K && about <= cluster_slots(lora_shrink_tiles_kernel<T>, n)) p.splits = n;
   const int stage_bytes = static_cast<int>(kXBytes) + p.n_alloc * kBlockK * 2;
-  p.stages = 200 * 1024 / stage_bytes < kMaxTileStages ? 200 * 1024 / stage_bytes : kMaxTileStages;
-  const size_t smem = 1024 + static_cast<size_t>(p.stages) * stage_bytes;
-  CUtensorMap x1_map, x8_map, x64_map, a_map;
-  int rc = make_map_u16_2d(&x1_map, x, tokens, K, x_ld, 1);
-  if (rc == B200_OK) rc = make_map_u16_2d(&x8_map, x, tokens, K, x_ld, 8);
-  if (rc == B200_OK) rc = make_map_u16_2d(&x64_map, x, tokens, K, x_ld, 64);
-  if (rc == B200_OK) rc = make_map_u16_2d(&a_map, A, static_cast<int64_t>(adapters) * cols, K, K, p.a_box);
+  p.stages = (kTileSmem - 1024) / stage_bytes < kMaxTileStages ? (kTileSmem - 1024) / stage_bytes : kMaxTileStages;
+  ShrinkMaps maps;
+  const int64_t a_rows = static_cast<int64_t>(adapters) * cols;
+  p.a_whole = cols <= kMaxColumns;
+  int rc = make_map_u16_2d(&maps.a, A, a_rows, K, K, p.a_box);
+  if (rc == B200_OK) rc = make_map_u16_2d(&maps.a_whole, A, a_rows, K, K, p.a_whole ? cols : p.a_box);
+  for (int i = 0; i < 5 && rc == B200_OK; ++i) rc = make_map_u16_2d(&maps.x[i], x, tokens, K, x_ld, i == 0 ? 1 : 4 << i);
   if (rc != B200_OK) return rc;
-  B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_tiles_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  B200_CUDA_TRY(launch_cluster(lora_shrink_tiles_kernel<T>, dim3(p.splits, static_cast<unsigned>(tiles), passes), dim3(kTileThreads), smem,
-                               p.splits, st, x1_map, x8_map, x64_map, a_map, plan, h, p));
+  B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_tiles_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem));
+  B200_CUDA_TRY(launch_cluster(lora_shrink_tiles_kernel<T>, dim3(p.splits, static_cast<unsigned>(tiles), passes), dim3(kTileThreads), kTileSmem,
+                               p.splits, st, maps, plan, h, p));
   return B200_OK;
 }
 
