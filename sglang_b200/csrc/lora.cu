@@ -27,8 +27,10 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kSmallRows = 16, kLargeRows = 128;
-constexpr int64_t kLargeFrom = 512;          // tokens
-__host__ __device__ inline int tile_rows(int64_t T) { return T >= kLargeFrom ? kLargeRows : kSmallRows; }
+// Rows of a tile: 128 from 256 tokens on, and 24 for every adapter that there may be.  K = 8192, qkv with R = 64, with 16 rows / 128:
+// one adapter 128 tokens 17 / 20 us, 256 29 / 21; 8 adapters 128 tokens 17 / 21, 256 25 / 22; 32 adapters 512 tokens 52 / 68,
+// 768 74 / 72.
+__host__ __device__ inline int tile_rows(int64_t T, int64_t L) { return T >= 256 && T >= 24 * L ? kLargeRows : kSmallRows; }
 constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
 constexpr int kMaxAdapters = 1024;
 constexpr int kMaxSlices = 8;
@@ -36,7 +38,7 @@ constexpr int64_t kMaxTokens = 1000000;     // max_tiles(kMaxTokens, kMaxAdapter
 
 // Device layout of a plan: int32 count[4] (tiles, -, -, -), int4 tiles[max_tiles] (adapter or -1, first, rows, rank), int32 perm[T]
 __host__ __device__ inline int64_t max_tiles(int64_t T, int64_t L) {
-  return T / tile_rows(T) + (L + 1 < T ? L + 1 : T);
+  return T / tile_rows(T, L) + (L + 1 < T ? L + 1 : T);
 }
 
 struct PlanView {
@@ -829,7 +831,7 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
     B200_CUDA_TRY(cudaMemset2DAsync(h, h_ld * sizeof(T), 0, cols * sizeof(T), tokens, st));
     return B200_OK;
   }
-  if (tile_rows(tokens) == kSmallRows) {
+  if (tile_rows(tokens, adapters) == kSmallRows) {
     // Enough blocks for six on every SM (of the tiles that a plan may have about half are used, and five blocks are resident), if
     // K has a k32 step for each of their warps.
     const int passes = (cols + 15) / 16;
@@ -870,10 +872,10 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
 }
 
 // Columns of a warp of the expand.
-int expand_columns(int64_t tokens, int R) { return tile_rows(tokens) == kSmallRows ? 64 : R <= 128 ? 32 : 16; }
+int expand_columns(int64_t tokens, int adapters, int R) { return tile_rows(tokens, adapters) == kSmallRows ? 64 : R <= 128 ? 32 : 16; }
 
 template <typename T>
-int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* scalings, PlanView plan, const Slices& sl, int64_t tokens,
+int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* scalings, int adapters, PlanView plan, const Slices& sl, int64_t tokens,
            int64_t tiles, const T* base, int64_t base_ld, T* out, int64_t out_ld, bool early, cudaStream_t st) {
   static_assert(kExpandThreads == kWalkThreads, "one grid for both");
   const int sms = sm_count();
@@ -881,7 +883,7 @@ int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* 
   constexpr int kWarps = kExpandThreads / 32;
   // small batches: as many blocks of columns a warp as leave eight warps for each SM, at most eight
   int per = 1;
-  if (tile_rows(tokens) == kSmallRows) {
+  if (tile_rows(tokens, adapters) == kSmallRows) {
     const int64_t most = tiles * sl.first_block[sl.n] / (8LL * sms);
     per = static_cast<int>(most < 1 ? 1 : most < 8 ? most : 8);
   }
@@ -892,7 +894,7 @@ int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* 
                              static_cast<int>(base_ld), out, static_cast<int>(out_ld), more...));
     return B200_OK;
   };
-  if (tile_rows(tokens) == kSmallRows) return go(lora_expand_kernel<T>, kExpandSmem, per, early);
+  if (tile_rows(tokens, adapters) == kSmallRows) return go(lora_expand_kernel<T>, kExpandSmem, per, early);
   if (R <= 32) return go(lora_expand_tiles_kernel<T, 1, 4>, walk_smem<1, 4>());
   if (R <= 64) return go(lora_expand_tiles_kernel<T, 2, 4>, walk_smem<2, 4>());
   if (R <= 128) return go(lora_expand_tiles_kernel<T, 4, 4>, walk_smem<4, 4>());
@@ -925,11 +927,15 @@ extern "C" int b200_lora_plan(const int32_t* token_adapters, int64_t T, const in
   if (rc != B200_OK) return rc;
   if ((rc = check_plan(plan, plan_bytes, T, L)) != B200_OK) return rc;
   if ((T > 0 && !token_adapters) || !ranks) return B200_ERR_NULL_PTR;
+  // The large shrink reports into the status ring, whose first use allocates: here rather than in a capture of the shrink.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  B200_CUDA_TRY(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture));
+  if (capture == cudaStreamCaptureStatusNone && tile_rows(T, L) == kLargeRows) gemm_sticky_status();
   const PlanView v = view_plan(plan, T, L);
   const size_t smem = sizeof(int) * ((kPlanWarps + 1) * (L + 1) + 2 * (L + 2));
   if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   B200_CUDA_TRY(launch_pdl(lora_plan_kernel, dim3(1), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), token_adapters, T,
-                           ranks, L, tile_rows(T), const_cast<int*>(v.count), const_cast<int4*>(v.tiles), const_cast<int*>(v.perm)));
+                           ranks, L, tile_rows(T, L), const_cast<int*>(v.count), const_cast<int4*>(v.tiles), const_cast<int*>(v.perm)));
   return B200_OK;
 }
 
@@ -968,7 +974,7 @@ int expand_entry(const void* h, int64_t h_ld, const void* B, int dtype, const vo
   if (num_slices <= 0 || !slice_sizes) return num_slices <= 0 ? B200_ERR_BAD_SHAPE : B200_ERR_NULL_PTR;
   if (num_slices > kMaxSlices) return B200_ERR_TOO_LARGE;
   if (dtype != B200_DT_BF16 && dtype != B200_DT_F16) return B200_ERR_BAD_DTYPE;
-  const int warp_cols = expand_columns(T, R), block_cols = tile_rows(T) == kSmallRows ? warp_cols : 4 * warp_cols;
+  const int warp_cols = expand_columns(T, L, R), block_cols = tile_rows(T, L) == kSmallRows ? warp_cols : 4 * warp_cols;
   Slices sl = {};
   sl.n = num_slices;
   int64_t N = 0;
@@ -992,9 +998,9 @@ int expand_entry(const void* h, int64_t h_ld, const void* B, int dtype, const vo
   const PlanView v = view_plan(plan, T, L);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == B200_DT_BF16)
-    return expand(static_cast<const __nv_bfloat16*>(h), h_ld, static_cast<const __nv_bfloat16*>(B), N, R, scalings, v, sl, T, tiles,
+    return expand(static_cast<const __nv_bfloat16*>(h), h_ld, static_cast<const __nv_bfloat16*>(B), N, R, scalings, L, v, sl, T, tiles,
                   static_cast<const __nv_bfloat16*>(base), base_ld, static_cast<__nv_bfloat16*>(out), out_ld, early, st);
-  return expand(static_cast<const __half*>(h), h_ld, static_cast<const __half*>(B), N, R, scalings, v, sl, T, tiles,
+  return expand(static_cast<const __half*>(h), h_ld, static_cast<const __half*>(B), N, R, scalings, L, v, sl, T, tiles,
                 static_cast<const __half*>(base), base_ld, static_cast<__half*>(out), out_ld, early, st);
 }
 

@@ -66,6 +66,7 @@ CASES = [
     (9, 256, [128, 0, 64], 24, 3), (16, 4096, [64, 64], 64, 2), (17, 520, [264], 128, 4), (33, 96, [40, 24, 16, 8], 256, 3),
     (129, 1024, [256, 64, 64], 64, 33), (300, 264, [136], 32, 1000), (515, 512, [320, 64, 64], 64, 3), (1000, 2048, [512, 512], 16, 2),
     (2049, 320, [192], 8, 40), (700, 136, [72, 72], 128, 2), (640, 200, [48, 16], 256, 2), (513, 8, [32, 8], 72, 2),
+    (255, 192, [40], 16, 2), (256, 192, [40], 16, 2), (263, 128, [16, 24], 24, 11), (264, 128, [16, 24], 24, 11), (257, 648, [264, 8], 64, 10),
 ]
 
 
@@ -116,7 +117,7 @@ def test_strided_views_and_odd_ids():
 def test_a_token_s_result_depends_on_its_own_row_only():
     """Infinities and NaN in one token leave every other token's bits alone; so does the company a token is in."""
     from sglang_b200.layers.lora import LoRABatch, apply_lora
-    for T in (24, 700):
+    for T in (24, 270, 700):
         x, base, A, B, ids, ranks, scal = _case(T, 320, [96, 32], 32, 3, BF, T)
         one = lambda xx, rows: apply_lora(base[rows].cuda(), xx[rows].cuda(), A.cuda(), B.cuda(),  # noqa: E731
                                           LoRABatch(ids[rows].cuda(), ranks.cuda(), scal.cuda()), [96, 32])
@@ -151,7 +152,7 @@ def test_segments_and_update():
     _close(out, want, tol)
 
 
-@pytest.mark.parametrize("T", [5, 600])
+@pytest.mark.parametrize("T", [5, 260, 600])
 def test_captured_and_replayed_on_a_side_stream(T):
     """Planning, shrink and expand in one graph; new tokens and ids are copied in before each replay.  Two graphs share nothing
     but the weights."""
