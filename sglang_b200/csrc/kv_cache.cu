@@ -176,8 +176,7 @@ enum { kRaw = -1, kNorm = 0, kNeox = 1, kPairs = 2 };
 
 // A lane holds two runs of eight elements, half of the row apart: a group's 16-byte accesses are then neighbours (with sixteen
 // elements in one run every access took half of a sector, and 8192 tokens of 36 heads 36.8 us).  With neox pairs the runs are half
-// of the rotated part apart, so that a rotation stays inside the lane, and half of the rest in the rest.  The weights are multiplied into the cosines and sines, once for all
-// rows; where the position is not in the table, all of these factors are NaN.
+// of the rotated part apart, so that a rotation stays inside the lane, and half of the rest in the rest.
 // pos: the token's position (no rotation: 0); slot: its place in the cache (CODES); both were loaded ahead and are looked at only
 // when the first rows are under way.
 template <typename T, int G, int KIND, bool STORE, bool CODES>
@@ -224,39 +223,26 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
     return;
   }
   const float* table_row = ROPE ? p.cos_sin + pos * rot : nullptr;
-  // the coefficients: y' = y ca + partner sa, the partner of the i-th pair of elements being the (i + 4)-th; elements that are not
-  // rotated have their weight in ca
-  f2 ca[8], sa[8];
+  // A weight times an element is exact in fp32 (both have at most 11 significant bits), so it comes first; rsqrt(...) comes last.  Where
+  // the position is not in the table, all factors are NaN.
+  const float nan_or_1 = poisoned ? __uint_as_float(0x7fc00000u) : 1.f;
+  f2 w[8], cs[4], sn[4], neg_sn[4];
   if (KIND != kRaw) {
-    f2 w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = both(poisoned ? __uint_as_float(0x7fc00000u) : 1.f);
-    if (r.weight != nullptr && in_row && !poisoned) {
+    for (int i = 0; i < 8; ++i) w[i] = both(nan_or_1);
+    if (r.weight != nullptr && in_row && !poisoned)
       unpack16<T, TURNED>(__ldg(reinterpret_cast<const uint4*>(r.weight + o0)), __ldg(reinterpret_cast<const uint4*>(r.weight + o1)), w);
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ca[i] = w[i];
-    if (turn0) {
-      float cc[8], ss[8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = c;
-        if (!poisoned && (i == 0 || turn1)) {
-          const float* at = table_row + (SPLIT ? 8 * l + 4 * i : (i == 0 ? o0 : o1) / 2);
-          c = __ldg(reinterpret_cast<const float4*>(at));
-          s = __ldg(reinterpret_cast<const float4*>(at + rot / 2));
-        }
-        cc[4 * i] = c.x, cc[4 * i + 1] = c.y, cc[4 * i + 2] = c.z, cc[4 * i + 3] = c.w;
-        ss[4 * i] = s.x, ss[4 * i + 1] = s.y, ss[4 * i + 2] = s.z, ss[4 * i + 3] = s.w;
+    for (int i = 0; i < 2; ++i) {
+      float4 c = make_float4(nan_or_1, nan_or_1, nan_or_1, nan_or_1), s = c;
+      if (!poisoned && (i == 0 ? turn0 : turn1)) {
+        const float* at = table_row + (SPLIT ? 8 * l + 4 * i : (i == 0 ? o0 : o1) / 2);
+        c = __ldg(reinterpret_cast<const float4*>(at));
+        s = __ldg(reinterpret_cast<const float4*>(at + rot / 2));
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = 2 * (i % 4);
-        const float2 mine = split(w[i]), other = split(w[(i + 4) % 8]);
-        if (i % 4 >= 2 && !turn1) continue;
-        ca[i] = make_f2(cc[j] * mine.x, cc[j + 1] * mine.y);
-        sa[i] = i < 4 ? make_f2(-ss[j] * other.x, -ss[j + 1] * other.y) : make_f2(ss[j] * other.x, ss[j + 1] * other.y);
-      }
+      cs[2 * i] = make_f2(c.x, c.y), cs[2 * i + 1] = make_f2(c.z, c.w);
+      sn[2 * i] = make_f2(s.x, s.y), sn[2 * i + 1] = make_f2(s.z, s.w);
+      neg_sn[2 * i] = make_f2(-s.x, -s.y), neg_sn[2 * i + 1] = make_f2(-s.z, -s.w);
     }
   }
   T* dst = STORE && r.dst != nullptr ? r.dst + (r.first + sub) * r.dst_sh : nullptr;
@@ -283,6 +269,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
     unpack16<T, TURNED>(sa::ld_v4(from), sa::ld_v4(from + kStageBytes / 2), y);
     from = from + kStageBytes == ring_end ? ring : from + kStageBytes;
     if (KIND != kRaw) {
+      f2 rinv = both(1.f);
       if (r.weight != nullptr) {
         f2 sum = mul(y[0], y[0]);
 #pragma unroll
@@ -290,23 +277,20 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
         float sq = split(sum).x + split(sum).y;
 #pragma unroll
         for (int off = G / 2; off >= 1; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-        const f2 rinv = both(rsqrtf(fmaf(sq, inv_d, p.eps)));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = mul(y[e], rinv);
+        rinv = both(rsqrtf(fmaf(sq, inv_d, p.eps)));
       }
 #pragma unroll
-      for (int run2 = 0; run2 < 4; run2 += 2) {                // pairs 0, 1, 4, 5: with neighbouring pairs the first run; 2, 3, 6, 7
-        if (run2 == 0 ? turn0 : turn1) {
+      for (int e = 0; e < 8; ++e) y[e] = mul(y[e], w[e]);
 #pragma unroll
-          for (int e = run2; e < run2 + 2; ++e) {
-            const f2 a = y[e], b = y[e + 4];
-            y[e] = fma(a, ca[e], mul(b, sa[e]));
-            y[e + 4] = fma(b, ca[e + 4], mul(a, sa[e + 4]));
-          }
-        } else {
+      for (int e = 0; e < 4; ++e) {                            // with neighbouring pairs 0 and 1 are the first run's, 2 and 3 the second's
+        if (!(e < 2 ? turn0 : turn1)) continue;
+        const f2 a = y[e], b = y[e + 4];
+        y[e] = fma(a, cs[e], mul(b, neg_sn[e]));
+        y[e + 4] = fma(b, cs[e], mul(a, sn[e]));
+      }
+      if (r.weight != nullptr) {
 #pragma unroll
-          for (int e = run2; e < run2 + 2; ++e) y[e] = mul(y[e], ca[e]), y[e + 4] = mul(y[e + 4], ca[e + 4]);
-        }
+        for (int e = 0; e < 8; ++e) y[e] = mul(y[e], rinv);
       }
     }
     if (STORE && dst != nullptr) {
@@ -339,7 +323,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
 }
 
 template <typename T, int G, int KIND>
-__global__ void __launch_bounds__(kThreads, 12) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
+__global__ void __launch_bounds__(kThreads, 11) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
   pdl_start();
   constexpr bool ROPE = KIND == kNeox || KIND == kPairs;
   __shared__ __align__(16) uint8_t rings[kThreads / 32 * kStages * kStageBytes];
