@@ -1,5 +1,6 @@
 /*
- * C ABI of libb200_block_fp8.so -- the W8A8 block-FP8 linear path for NVIDIA B200 (sm_100a).
+ * C ABI of libb200_block_fp8.so -- the W8A8 block-FP8 linear path for NVIDIA B200 (sm_100a), and what an attention layer runs
+ * between its projections and its attention kernel: adapters, head norms with the rotation, an e4m3 key/value cache.
  *
  * Every entry point takes plain device pointers, sizes and element strides; none
  * allocates, synchronises or reads device data on the host unless stated.  Kernels are
@@ -673,7 +674,8 @@ int b200_lora_apply(const void* x, int64_t x_ld, const void* A, const void* B, i
  * The output of the launch that gave up is undefined.  Launches that were already queued behind it are
  * not affected by it: each launch watches its own slot of a ring of status words, so a stale code can
  * never make a healthy kernel abandon its waits.  The first GEMM call on a device allocates the pinned
- * mirror (4 bytes); make that call before any stream capture.  No reference counterpart.
+ * mirror (4 bytes); make that call before any stream capture.  b200_lora_shrink and b200_lora_apply on large batches are GEMM
+ * entry points in this sense; b200_lora_plan outside a capture is such a first call for them.  No reference counterpart.
  */
 int b200_gemm_device_status(int* status_out);
 int b200_gemm_poll_status(int* status_out);

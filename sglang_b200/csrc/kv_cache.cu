@@ -16,7 +16,7 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 64;
+constexpr int kMaxThreads = 64;
 
 struct HeadRowsParams {
   const void *q, *k, *v;
@@ -323,13 +323,13 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
 }
 
 template <typename T, int G, int KIND>
-__global__ void __launch_bounds__(kThreads, 11) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 11) head_rows_kernel(const __grid_constant__ HeadRowsParams p) {
   pdl_start();
   constexpr bool ROPE = KIND == kNeox || KIND == kPairs;
-  __shared__ __align__(16) uint8_t rings[kThreads / 32 * kStages * kStageBytes];
+  extern __shared__ __align__(16) uint8_t rings[];
   const int lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(rings) + (threadIdx.x >> 5) * (kStages * kStageBytes) + lane * 16;
-  const uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t item = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
   uint32_t tok32 = p.chunks == 1 ? item : __umulhi(item, p.chunks_magic);      // item / chunks, or one more
   if (tok32 * p.chunks > item) --tok32;
   if (tok32 >= p.T) return;
@@ -364,12 +364,14 @@ __global__ void __launch_bounds__(kThreads, 11) head_rows_kernel(const __grid_co
 }
 
 template <typename T, int G>
-cudaError_t launch_rows(const HeadRowsParams& p, int kind, unsigned grid, cudaStream_t st) {
+cudaError_t launch_rows(const HeadRowsParams& p, int kind, unsigned grid, int warps, cudaStream_t st) {
+  const dim3 block(32 * warps);
+  const size_t smem = warps * kStages * kStageBytes;
   switch (kind) {
-    case kRaw: return launch_pdl(head_rows_kernel<T, G, kRaw>, dim3(grid), dim3(kThreads), 0, st, p);
-    case kNorm: return launch_pdl(head_rows_kernel<T, G, kNorm>, dim3(grid), dim3(kThreads), 0, st, p);
-    case kNeox: return launch_pdl(head_rows_kernel<T, G, kNeox>, dim3(grid), dim3(kThreads), 0, st, p);
-    default: return launch_pdl(head_rows_kernel<T, G, kPairs>, dim3(grid), dim3(kThreads), 0, st, p);
+    case kRaw: return launch_pdl(head_rows_kernel<T, G, kRaw>, dim3(grid), block, smem, st, p);
+    case kNorm: return launch_pdl(head_rows_kernel<T, G, kNorm>, dim3(grid), block, smem, st, p);
+    case kNeox: return launch_pdl(head_rows_kernel<T, G, kNeox>, dim3(grid), block, smem, st, p);
+    default: return launch_pdl(head_rows_kernel<T, G, kPairs>, dim3(grid), block, smem, st, p);
   }
 }
 
@@ -377,7 +379,7 @@ template <typename T, int G>
 int go_rows(HeadRowsParams p, int kind, cudaStream_t st) {
   const int sms = sm_count();
   if (sms <= 0) return B200_ERR_CUDA;
-  constexpr int RPW = 32 / G, WPB = kThreads / 32;
+  constexpr int RPW = 32 / G;
   auto chunks = [&](int heads, int u) { return (heads + RPW * u - 1) / (RPW * u); };
   // Two rows a lane group at a time, and for queries four rounds of that, where every SM still gets sixteen warps; otherwise one
   // row each, for latency.
@@ -386,9 +388,13 @@ int go_rows(HeadRowsParams p, int kind, cudaStream_t st) {
   p.chunks_q = chunks(p.Hq, wide ? 8 : 1), p.chunks_kv = chunks(p.Hkv, wide ? 2 : 1);
   p.chunks = p.chunks_q + p.chunks_kv + (p.Hv ? p.chunks_kv : 0);
   p.chunks_magic = static_cast<uint32_t>((1ULL << 32) / p.chunks + 1);
-  const int64_t blocks = (p.T * p.chunks + WPB - 1) / WPB;
-  if (blocks * WPB > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
-  B200_CUDA_TRY((launch_rows<T, G>(p, kind, static_cast<unsigned>(blocks), st)));
+  // Blocks of one warp where a warp has four rows a lane group or more on average: warps of a block end at different times (8192
+  // tokens of 32 + 4 heads 26.9 us, with two warps 31.1).  With less to do the rate at which blocks start would set the pace (keys
+  // and values of 16384 tokens, 16 heads of 64: 34.5 us, with two warps 20.4).
+  const int rows = chunks(p.Hq, 1) + chunks(p.Hkv, 1) * (p.Hv ? 2 : 1), warps = rows >= 4 * p.chunks ? 1 : kMaxThreads / 32;
+  const int64_t blocks = (p.T * p.chunks + warps - 1) / warps;
+  if (blocks * warps > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
+  B200_CUDA_TRY((launch_rows<T, G>(p, kind, static_cast<unsigned>(blocks), warps, st)));
   return B200_OK;
 }
 
