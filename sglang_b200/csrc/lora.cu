@@ -8,13 +8,13 @@
 // every adapter's weights are read for a few tokens each, and 128 in large ones.
 //
 // Both products are bound by memory: the shrink by x and A, the expand by base, out and B.  The large shrink, whose products
-// would bind it on the older matrix instructions, runs on tcgen05 (lora_shrink_tiles_kernel).  In the others operands go from global memory
-// straight into the fragments of mma.m16n8k16: the order in which k is summed is free, so a lane's fragment of two
-// consecutive k16 steps is one 16-byte load (eight consecutive k), and no shared memory or transposition is needed.  The
-// weights are the 16-row operand, the tokens the 8-column one, so a single token wastes no weight traffic.
+// would bind it on the older matrix instructions, runs on tcgen05 (lora_shrink_tiles_kernel).  The others use mma.m16n8k16; the
+// order in which k is summed is free, so a lane's fragments of two consecutive k16 steps are one 16-byte vector (eight consecutive
+// k) and nothing is transposed.  In small batches the weights are the 16-row operand and the tokens the 8-column one, so that a
+// single token wastes no weight traffic.
 //
-// Sums are held in fp32.  h is rounded once, to the type of x, because the expand multiplies it with B on the tensor cores;
-// that adds at most half a step of h (2^-9 for bf16) to the adapter's part of the sum, less than the rounding of out adds.
+// Sums are held in fp32.  h is rounded once, to the type of x, because the expand multiplies it with B on the tensor cores: half a
+// step of h (2^-8 of it for bf16, 2^-11 for fp16) in the adapter's part of the sum; in fp16 an h beyond 65504 becomes infinite.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __
     if (i + kShrinkStages - 1 < end) fetch(i + kShrinkStages - 1);
     sa::cp_async_commit();
     sa::cp_async_wait<kShrinkStages - 1>();
+    __syncwarp();
     const uint4 lo = sa::ld_v4(from), hi = sa::ld_v4(from + 512);
     mma_k32<T>(acc[0], lo, hi, sa::ld_v4(from + 1024));
     if (both) mma_k32<T>(acc[1], lo, hi, sa::ld_v4(from + 1536));
@@ -617,6 +618,7 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h,
     }
     sa::cp_async_commit();
     sa::cp_async_wait<2>();
+    __syncwarp();                                            // lanes that stored come back to those that had nothing to store
     const uint32_t from = at.place;
     const int j = at.j;
     if (j == 0) {
@@ -742,6 +744,7 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
   for (int step = 0; step < steps; ++step) {
     if (step + kWalkStages - 1 < steps) fetch(step + kWalkStages - 1);
     sa::cp_async_commit();
+    __syncwarp();                                            // lanes that stored come back to those that had nothing to store
     float acc[NT][4] = {};
     if (!none) {
 #pragma unroll

@@ -96,6 +96,55 @@ def test_apply(T, K, sizes, R, L, dtype):
     _close(apply_lora(None, xd, Ad, Bd, batch, output_sizes=sizes), want0, tol0)
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_runs_of_neighbouring_tokens(seed):
+    """Requests of several tokens: tiles whose tokens are neighbours, have gaps in different places, or end early."""
+    from sglang_b200.layers.lora import LoRABatch, apply_lora
+    g = torch.Generator().manual_seed(seed)
+    lens = [[130, 64, 96, 40, 17, 8, 200, 145], [1, 127, 129, 16, 48, 32, 260], [500, 3, 5, 9, 33, 65, 256], [24] * 30][seed]
+    which = torch.tensor([(3 * i) % 4 - 1 for i in range(len(lens))])[torch.randperm(len(lens), generator=g)]
+    T, K, sizes, R, L = sum(lens), 456, [72, 40], 32, 3
+    x, base, A, B, _, ranks, scal = _case(T, K, sizes, R, L, BF, seed)
+    ids = torch.repeat_interleave(which, torch.tensor(lens)).int()
+    batch = LoRABatch(ids.cuda(), ranks.cuda(), scal.cuda())
+    _, want, _, tol = _exact(x, base, A, B, ids, ranks, scal, sizes)
+    _close(apply_lora(base.cuda(), x.cuda(), A.cuda(), B.cuda(), batch, sizes), want, tol)
+
+
+@pytest.mark.parametrize("T", [3, 300])
+def test_nobody_has_an_adapter(T):
+    from sglang_b200.layers.lora import LoRABatch, apply_lora, lora_shrink
+    x, base, A, B, _, ranks, scal = _case(T, 128, [64], 16, 2, BF, T)
+    batch = LoRABatch(torch.full((T,), -1, dtype=torch.int32, device="cuda"), ranks.cuda(), scal.cuda())
+    xd, bd = x.cuda(), base.cuda()
+    for _ in range(3):
+        assert same_bits(apply_lora(bd, xd, A.cuda(), B.cuda(), batch), base)
+        assert same_bits(apply_lora(bd, xd, A.cuda(), B.cuda(), batch, out=torch.full_like(bd, 5.0)), base)
+        assert (apply_lora(None, xd, A.cuda(), B.cuda(), batch) == 0).all()
+        assert (lora_shrink(xd, A.cuda(), batch) == 0).all()
+
+
+def test_several_streams_at_once():
+    """Calls of one batch on several streams, each with its own tokens and output."""
+    from sglang_b200.layers.lora import LoRABatch, apply_lora
+    for T in (6, 300):
+        cases = [_case(T, 512, [128, 64], 32, 3, BF, 50 + i) for i in range(4)]
+        x0, _, A, B, ids, ranks, scal = cases[0]
+        Ad, Bd = A.cuda(), B.cuda()
+        batch = LoRABatch(ids.cuda(), ranks.cuda(), scal.cuda())
+        xs, bases = [c[0].cuda() for c in cases], [c[1].cuda() for c in cases]
+        alone = [apply_lora(b.clone(), x, Ad, Bd, batch, [128, 64]) for x, b in zip(xs, bases)]
+        torch.cuda.synchronize()
+        streams, outs = [torch.cuda.Stream() for _ in cases], [torch.empty_like(b) for b in bases]
+        for _ in range(20):
+            for s, x, b, o in zip(streams, xs, bases, outs):
+                with torch.cuda.stream(s):
+                    apply_lora(b, x, Ad, Bd, batch, [128, 64], out=o)
+        torch.cuda.synchronize()
+        for a, o in zip(alone, outs):
+            assert same_bits(a, o)
+
+
 def test_strided_views_and_odd_ids():
     """x and base as columns of wider tensors; ids outside the buffers and ranks of 0 or below count as no adapter; a rank
     above R counts as R."""
