@@ -532,8 +532,11 @@ void need_type(const Tensor& t, at::ScalarType type, const char* name, const cha
 }
 // The stride of a dimension; one that holds at most one element has none, nor has an empty tensor.
 int64_t stride_of(const Tensor& t, int d) { return t.size(d) > 1 && t.numel() > 0 ? t.stride(d) : 0; }
-// The leading dimension of a matrix.
+// The leading dimension of a matrix whose rows do not overlap.
 int64_t ld_of(const Tensor& t) { return stride_of(t, 0) != 0 ? t.stride(0) : t.size(1); }
+void need_own_rows(const Tensor& t, const char* name) {       // a row broadcast over several is refused, too
+  NEED(t.size(0) <= 1 || t.numel() == 0 || t.stride(0) >= t.size(1), std::string(name) + " must not overlap itself");
+}
 void need_rows(const Tensor& t, int64_t multiple, const char* name) {      // the last dimension dense, the others in whole vectors
   NEED(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, std::string(name) + " must be contiguous in its last dimension");
   for (int d = 0; d + 1 < t.dim(); ++d)
@@ -844,6 +847,7 @@ HOST_FN(lora) {
     NEED(A.size(1) == S * R && A.size(2) == K, "lora_a must be [num_adapters, num_slices * R, K]");
     NEED(K % 8 == 0, "K must be a multiple of 8");
     need_rows(x, 8, "x");
+    need_own_rows(x, "x");
     need_aligned(x, "x");
     need_aligned(A, "lora_a");
     NEED(A.scalar_type() == type, "lora_a must have the type of x");
@@ -852,6 +856,7 @@ HOST_FN(lora) {
     T = h.size(0), type = h.scalar_type();
     need_sizes(h, {T, S * R}, "h");
     need_rows(h, 8, "h");
+    need_own_rows(h, "h");
     need_aligned(h, "h");
   }
   NEED(is_16bit(type), "x must be bfloat16 or float16");
@@ -868,7 +873,7 @@ HOST_FN(lora) {
     need_sizes(t, {T, N}, what);
     need_rows(t, 8, what);
     need_aligned(t, what);
-    if (T > 1 && N > 0) NEED(t.stride(0) >= N, std::string(what) + " must not overlap itself");
+    need_own_rows(t, what);
   }
   const at::Device dev = one_device({&plan, &base, &x, &h, &A, &B, &scalings, &out});
   int rc = 0;

@@ -142,6 +142,20 @@ def test_lora_refusals(change, message):
         _lora_call(**change)
 
 
+@pytest.mark.parametrize("stride", [0, 8])
+def test_lora_refuses_rows_that_overlap(stride):
+    """A row broadcast over all tokens would be read as if the rows followed one another."""
+    from sglang_b200.layers.lora import lora_expand, lora_shrink
+    x = torch.zeros(5, 64, dtype=BF).as_strided((5, 64), (stride, 1))
+    with pytest.raises(RuntimeError, match="x must not overlap"):
+        _lora_call(x=x)
+    with pytest.raises(RuntimeError, match="x must not overlap"):
+        lora_shrink(x, torch.zeros(3, 32, 64, dtype=BF), _Batch(5, 3), num_slices=2)
+    h = torch.zeros(5, 32, dtype=BF).as_strided((5, 32), (stride, 1))
+    with pytest.raises(RuntimeError, match="h must not overlap"):
+        lora_expand(h, torch.zeros(3, 96, 16, dtype=BF), _Batch(5, 3), output_sizes=[64, 32])
+
+
 @pytest.mark.parametrize("ids,ranks,message", [
     (torch.zeros(4, dtype=torch.int64), torch.zeros(2, dtype=torch.int32), "token_adapters"),
     (torch.zeros(4, dtype=torch.int32), torch.zeros(2), "lora_ranks"),
