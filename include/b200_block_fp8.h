@@ -648,7 +648,8 @@ int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_table, int6
  * tokens without an adapter).  b200_lora_expand: base NULL counts as zeros; out may be base; tokens without an adapter get
  * base.  slice_sizes (host) adds up to N, each a multiple of 8.  dtype (of x, A, h, B, base, out) bf16 or fp16; K and R
  * multiples of 8, R <= 256, at most 8 slices, 1024 adapters and 1000000 tokens; leading dimensions multiples of 8, pointers
- * 16-byte aligned.  b200_lora_apply is both, h being scratch of num_tokens * num_slices * R elements.
+ * 16-byte aligned.  b200_lora_apply is both, h being scratch of num_tokens * num_slices * R elements; out may share no memory
+ * with what it reads, base itself apart.
  */
 size_t b200_lora_plan_bytes(int64_t num_tokens, int num_adapters);
 int b200_lora_plan(const int32_t* token_adapters, int64_t num_tokens, const int32_t* ranks, int num_adapters, void* plan,

@@ -657,6 +657,178 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h,
   }
 }
 
+// A handful of tokens and a small rank: both products in one launch.  A cluster of eight blocks computes all of a tile's h -- up to
+// 16 Z columns, K divided among its 32 warps, added up in the order of the separate kernels -- and every warp then expands one
+// block of 64 columns.  Clusters of the same tile repeat the shrink out of L2, which up to 32 columns costs less than a second
+// launch and h's way through memory: 1 token, K = N = 8192, rank 16 takes 5.0 us against 5.4, and the host one launch less (2.5 us).
+// With 48 or 64 columns it does not pay (7.6 and 8.2 against 5.7 and 5.9), nor with many clusters (18 for N = 36864: 6.6 against
+// 5.6; 17 tiles of four: 11.8 against 9.0).  B and base are fetched first and arrive under the shrink.
+constexpr int kFusedThreads = 128, kFusedWarps = kFusedThreads / 32, kFusedCluster = 8, kFusedColumns = 32;
+constexpr int64_t kFusedParts = 8, kFusedClusters = 36;
+template <int Z>
+struct Fused {
+  static constexpr int kStages = Z == 1 ? 5 : 3, kStageBytes = (2 * Z + 2) * 512;
+  static constexpr int kOwn = 12 * 512;                              // a warp's B and base
+  static constexpr int kRing = kFusedWarps * kStages * kStageBytes, kSmem = kRing + kFusedWarps * kOwn;
+};
+
+template <typename T, int Z>
+__global__ void __launch_bounds__(kFusedThreads) lora_fused_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ A,
+                                                                   const T* __restrict__ B, int64_t K, int64_t N, int R, int cols,
+                                                                   const float* __restrict__ scalings, PlanView plan,
+                                                                   const __grid_constant__ Slices sl, const T* base, int base_ld,
+                                                                   T* out, int out_ld) {
+  using F = Fused<Z>;
+  pdl_start();
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ float part[kFusedWarps][Z * 256], mine[Z * 256];
+  __shared__ __align__(16) T hs[16][Z * 16 + 8];                     // padded: eight rows' vectors lie in different banks
+  const int tiles = plan.count[0];
+  const int4 tile = plan.tiles[blockIdx.y];                          // in bounds whether or not it is one
+  if (static_cast<int>(blockIdx.y) >= tiles) return;                 // the whole cluster leaves together, here and below
+  const bool none = tile.x < 0;
+  if (none && base == out) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+  const int rows = tile.z, rank = none ? 0 : min(tile.w, R);
+  const bool both = rows > 8;
+  const int* perm = plan.perm + tile.y;
+  // ---- this warp's 64 columns: B and base
+  const int block = (blockIdx.z * kFusedCluster + blockIdx.x) * kFusedWarps + warp;
+  const bool busy = block < sl.first_block[sl.n];
+  int s = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxSlices; ++i) s += i < sl.n && block >= sl.first_block[i];
+  const int n = busy ? sl.first_col[s] + (block - sl.first_block[s]) * 64 + 8 * g : 0;      // the first of this lane's eight columns
+  const bool live = busy && n < sl.first_col[s + 1];
+  int token[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) token[i] = __ldg(perm + min(8 * (i / 2) + 2 * c + i % 2, rows - 1));
+  const uint32_t own = smem_u32(dyn) + F::kRing + warp * F::kOwn + lane * 16;
+  const bool some = live && rank - 8 * c > 0;                        // of the at most 32 ranks
+  const T* bp = some ? B + (static_cast<int64_t>(tile.x) * N + n) * R + 8 * c : B;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sa::cp_async_or_zero<16>(own + i * 512, some ? bp + i * R : B, some);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool in = base != nullptr && live && 8 * (i / 2) + 2 * c + i % 2 < rows;
+    sa::cp_async_or_zero<16>(own + (8 + i) * 512, in ? base + static_cast<int64_t>(token[i]) * base_ld + n : B, in);
+  }
+  sa::cp_async_commit();
+  // ---- shrink
+  const int r0 = __ldg(perm + min(g, rows - 1)), r1 = __ldg(perm + min(g + 8, rows - 1));
+  constexpr int kAll = kFusedCluster * kFusedWarps;
+  const int chunks = none ? 0 : static_cast<int>((K + 31) / 32), per = (chunks + kAll - 1) / kAll;
+  const int begin = (blockIdx.x * kFusedWarps + warp) * per, end = min(begin + per, chunks);
+  const char* src[2 * Z + 2];
+  bool there[2 * Z + 2];
+#pragma unroll
+  for (int i = 0; i < 2 * Z + 2; ++i) {
+    const int col = i < 2 * Z ? g + 8 * i : 0, row = i < 2 * Z ? 0 : g + 8 * (i - 2 * Z);
+    const bool in = i < 2 * Z ? col < cols && col % R < rank : row < rows;
+    const T* p = i < 2 * Z ? A + (static_cast<int64_t>(none ? 0 : tile.x) * cols + col) * K : x + (i == 2 * Z ? r0 : r1) * x_ld;
+    src[i] = reinterpret_cast<const char*>(in ? p + static_cast<int64_t>(begin) * 32 + 8 * c : A);
+    there[i] = in;
+  }
+  float acc[Z][2][4] = {};
+  const uint32_t ring = smem_u32(dyn) + warp * (F::kStages * F::kStageBytes) + lane * 16, ring_end = ring + F::kStages * F::kStageBytes;
+  const int ragged = K % 32 != 0 && 8 * c >= K % 32 ? chunks - 1 : -1;       // the step of which this lane has nothing
+  uint32_t to = ring, from = ring;
+  auto fetch = [&](int i) {
+    if (i == ragged) {
+#pragma unroll
+      for (int j = 0; j < 2 * Z + 2; ++j) there[j] = false, src[j] = reinterpret_cast<const char*>(A);
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * Z + 2; ++j) {
+      if (j < 2 * Z + 1 || both) sa::cp_async_or_zero<16>(to + 512 * j, src[j], there[j]);
+      src[j] += 64;
+    }
+    to = to + F::kStageBytes == ring_end ? ring : to + F::kStageBytes;
+  };
+#pragma unroll 1
+  for (int i = 0; i < F::kStages - 1; ++i) {
+    if (begin + i < end) fetch(begin + i);
+    sa::cp_async_commit();
+  }
+#pragma unroll 1
+  for (int i = begin; i < end; ++i) {
+    if (i + F::kStages - 1 < end) fetch(i + F::kStages - 1);
+    sa::cp_async_commit();
+    sa::cp_async_wait<F::kStages - 1>();
+    __syncwarp();
+    const uint4 x0 = sa::ld_v4(from + 2 * Z * 512);
+    uint4 x1 = make_uint4(0, 0, 0, 0);
+    if (both) x1 = sa::ld_v4(from + (2 * Z + 1) * 512);
+#pragma unroll
+    for (int z = 0; z < Z; ++z) {
+      const uint4 lo = sa::ld_v4(from + 2 * z * 512), hi = sa::ld_v4(from + (2 * z + 1) * 512);
+      mma_k32<T>(acc[z][0], lo, hi, x0);
+      if (both) mma_k32<T>(acc[z][1], lo, hi, x1);
+    }
+    from = from + F::kStageBytes == ring_end ? ring : from + F::kStageBytes;
+  }
+#pragma unroll
+  for (int z = 0; z < Z; ++z)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[warp][z * 256 + (8 * i + 2 * c + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[z][i][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < Z * 256; e += kFusedThreads) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFusedWarps; ++w) sum += part[w][e];
+    mine[e] = sum;
+  }
+  // each block adds up an eighth of h and gives it to all
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int i = threadIdx.x; i < Z * 256 / kFusedCluster; i += kFusedThreads) {
+    const int e = static_cast<int>(blockIdx.x) * (Z * 256 / kFusedCluster) + i, z = e / 256, row = e / 16 % 16, col = 16 * z + e % 16;
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < kFusedCluster; ++b) sum += *cluster.map_shared_rank(mine + e, b);
+    const T v = static_cast<T>(col < cols && col % R < rank ? sum : 0.f);
+#pragma unroll
+    for (int b = 0; b < kFusedCluster; ++b) *cluster.map_shared_rank(&hs[row][col], b) = v;
+  }
+  cluster.sync();                                                    // h is everywhere, and nobody reads or writes others' memory again
+  if (!busy) return;
+  // ---- expand
+  sa::cp_async_wait<0>();
+  __syncwarp();
+  float sum[2][4][4] = {};
+  if (!none) {
+    const int keep = rank - 8 * c;
+    uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+    if (keep > 0) x0 = *reinterpret_cast<const uint4*>(&hs[g][s * R + 8 * c]), x1 = *reinterpret_cast<const uint4*>(&hs[g + 8][s * R + 8 * c]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint4 lo = sa::ld_v4(own + 2 * i * 512), hi = sa::ld_v4(own + (2 * i + 1) * 512);
+      if (keep > 0 && keep < 8) lo = first_of(lo, keep), hi = first_of(hi, keep);
+      mma_k32<T>(sum[0][i], lo, hi, x0);
+      if (both) mma_k32<T>(sum[1][i], lo, hi, x1);
+    }
+  }
+  if (!live) return;
+  const float scaling = none ? 0.f : __ldg(scalings + tile.x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (8 * (i / 2) + 2 * c + i % 2 >= rows) continue;
+    uint4 v = sa::ld_v4(own + (8 + i) * 512);
+    if (!none) {
+      uint32_t* q = &v.x;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const float2 b = unpack2<T>(q[m]);
+        q[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, sum[i / 2][m][i % 2], b.x), fmaf(scaling, sum[i / 2][m][i % 2 + 2], b.y));
+      }
+    }
+    *reinterpret_cast<uint4*>(out + static_cast<int64_t>(token[i]) * out_ld + n) = v;
+  }
+}
+
 // Tiles of up to 128 tokens: a warp holds the B of NT x 8 columns of one slice in registers (tokens are the 16-row operand here)
 // and walks down the tile, 16 tokens at a time.  Row g of the 8-column operand i is column 2 NT (g / 2) + 2 i + g % 2, so that a
 // lane's 2 NT sums of a token are neighbours and base and out move 16 bytes at a time (8 with NT = 2).  RJ = ceil(R / 32).
@@ -874,6 +1046,17 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
   return B200_OK;
 }
 
+// Slices in blocks of warp_cols columns, a whole number of block_cols for each.
+Slices make_slices(const int64_t* sizes, int n, int warp_cols, int block_cols) {
+  Slices sl = {};
+  sl.n = n;
+  for (int i = 0; i < n; ++i) {
+    sl.first_col[i + 1] = sl.first_col[i] + static_cast<int>(sizes[i]);
+    sl.first_block[i + 1] = sl.first_block[i] + static_cast<int>((sizes[i] + block_cols - 1) / block_cols) * (block_cols / warp_cols);
+  }
+  return sl;
+}
+
 // Columns of a warp of the expand.
 int expand_columns(int64_t tokens, int adapters, int R) { return tile_rows(tokens, adapters) == kSmallRows ? 64 : R <= 128 ? 32 : 16; }
 
@@ -902,6 +1085,35 @@ int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* 
   if (R <= 64) return go(lora_expand_tiles_kernel<T, 2, 4>, walk_smem<2, 4>());
   if (R <= 128) return go(lora_expand_tiles_kernel<T, 4, 4>, walk_smem<4, 4>());
   return go(lora_expand_tiles_kernel<T, 8, 2>, walk_smem<8, 2>());
+}
+
+// Clusters of a tile in the fused form, one block of 64 columns a warp; 0 where it is not used.
+int fused_parts(int64_t tokens, int adapters, int64_t tiles, int cols, const Slices& sl) {
+  if (tile_rows(tokens, adapters) != kSmallRows || cols > kFusedColumns) return 0;
+  const int parts = (sl.first_block[sl.n] + kFusedCluster * kFusedWarps - 1) / (kFusedCluster * kFusedWarps);
+  return parts <= kFusedParts && tiles * parts <= kFusedClusters ? parts : 0;
+}
+
+template <typename T, int Z>
+int fused(const T* x, int64_t x_ld, const T* A, const T* B, int64_t K, int64_t N, int R, int cols, const float* scalings, PlanView plan,
+          const Slices& sl, int64_t tiles, int parts, const T* base, int base_ld, T* out, int out_ld, cudaStream_t st) {
+  B200_CUDA_TRY(cudaFuncSetAttribute(lora_fused_kernel<T, Z>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fused<Z>::kSmem));
+  B200_CUDA_TRY(launch_cluster(lora_fused_kernel<T, Z>, dim3(kFusedCluster, static_cast<unsigned>(tiles), parts), dim3(kFusedThreads),
+                               Fused<Z>::kSmem, kFusedCluster, st, x, x_ld, A, B, K, N, R, cols, scalings, plan, sl, base, base_ld, out,
+                               out_ld));
+  return B200_OK;
+}
+template <typename T>
+int fused(const void* x, int64_t x_ld, const void* A, const void* B, int64_t K, int64_t N, int R, int cols, const float* scalings,
+          PlanView plan, const Slices& sl, int64_t tiles, int parts, const void* base, int64_t base_ld, void* out, int64_t out_ld,
+          cudaStream_t st) {
+  auto go = [&](auto z) {
+    return fused<T, decltype(z)::value>(static_cast<const T*>(x), x_ld, static_cast<const T*>(A), static_cast<const T*>(B), K, N, R,
+                                        cols, scalings, plan, sl, tiles, parts, static_cast<const T*>(base), static_cast<int>(base_ld),
+                                        static_cast<T*>(out), static_cast<int>(out_ld), st);
+  };
+  if (cols <= 16) return go(std::integral_constant<int, 1>());
+  return go(std::integral_constant<int, 2>());
 }
 
 int check_plan(const void* plan, size_t bytes, int64_t T, int64_t L) {
@@ -945,8 +1157,9 @@ extern "C" int b200_lora_plan(const int32_t* token_adapters, int64_t T, const in
 namespace b200 {
 namespace {
 
+// check_only, here and in expand_entry: the arguments are looked at, nothing is launched.
 int shrink_entry(const void* x, int64_t x_ld, const void* A, int dtype, const void* plan, size_t plan_bytes, int64_t T, int L,
-                 int64_t K, int R, int num_slices, void* h, int64_t h_ld, void* stream) {
+                 int64_t K, int R, int num_slices, void* h, int64_t h_ld, bool check_only, void* stream) {
   int rc = check_sizes(T, L, R);
   if (rc != B200_OK) return rc;
   if (num_slices <= 0 || K < 0 || K % 8 != 0) return B200_ERR_BAD_SHAPE;
@@ -958,6 +1171,7 @@ int shrink_entry(const void* x, int64_t x_ld, const void* A, int dtype, const vo
   if ((rc = check_plan(plan, plan_bytes, T, L)) != B200_OK) return rc;
   if ((K > 0 && (!x || !A)) || !h) return B200_ERR_NULL_PTR;
   if (!aligned16(x) || !aligned16(A) || !aligned16(h)) return B200_ERR_MISALIGNED;
+  if (check_only) return B200_OK;
   const int64_t tiles = max_tiles(T, L);
   const PlanView v = view_plan(plan, T, L);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -968,7 +1182,6 @@ int shrink_entry(const void* x, int64_t x_ld, const void* A, int dtype, const vo
                 static_cast<__half*>(h), h_ld, st);
 }
 
-// check_only: the arguments are looked at, nothing is launched.
 int expand_entry(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes, const float* scalings,
                  int64_t T, int L, int R, const int64_t* slice_sizes, int num_slices, const void* base, int64_t base_ld, void* out,
                  int64_t out_ld, bool early, bool check_only, void* stream) {
@@ -977,17 +1190,14 @@ int expand_entry(const void* h, int64_t h_ld, const void* B, int dtype, const vo
   if (num_slices <= 0 || !slice_sizes) return num_slices <= 0 ? B200_ERR_BAD_SHAPE : B200_ERR_NULL_PTR;
   if (num_slices > kMaxSlices) return B200_ERR_TOO_LARGE;
   if (dtype != B200_DT_BF16 && dtype != B200_DT_F16) return B200_ERR_BAD_DTYPE;
-  const int warp_cols = expand_columns(T, L, R), block_cols = tile_rows(T, L) == kSmallRows ? warp_cols : 4 * warp_cols;
-  Slices sl = {};
-  sl.n = num_slices;
   int64_t N = 0;
   for (int i = 0; i < num_slices; ++i) {
     if (slice_sizes[i] < 0 || slice_sizes[i] % 8 != 0) return B200_ERR_BAD_SHAPE;
     if (slice_sizes[i] > (1 << 30) || N + slice_sizes[i] > (1 << 30)) return B200_ERR_TOO_LARGE;
     N += slice_sizes[i];
-    sl.first_col[i + 1] = static_cast<int>(N);
-    sl.first_block[i + 1] = sl.first_block[i] + static_cast<int>((slice_sizes[i] + block_cols - 1) / block_cols) * (block_cols / warp_cols);
   }
+  const int warp_cols = expand_columns(T, L, R);
+  const Slices sl = make_slices(slice_sizes, num_slices, warp_cols, tile_rows(T, L) == kSmallRows ? warp_cols : 4 * warp_cols);
   if (h_ld < num_slices * static_cast<int64_t>(R) || h_ld % 8 != 0 || out_ld < N || out_ld % 8 != 0 ||
       (base && (base_ld < N || base_ld % 8 != 0)))
     return B200_ERR_BAD_STRIDE;
@@ -1012,7 +1222,7 @@ int expand_entry(const void* h, int64_t h_ld, const void* B, int dtype, const vo
 
 extern "C" int b200_lora_shrink(const void* x, int64_t x_ld, const void* A, int dtype, const void* plan, size_t plan_bytes,
                                 int64_t T, int L, int64_t K, int R, int num_slices, void* h, int64_t h_ld, void* stream) {
-  return b200::shrink_entry(x, x_ld, A, dtype, plan, plan_bytes, T, L, K, R, num_slices, h, h_ld, stream);
+  return b200::shrink_entry(x, x_ld, A, dtype, plan, plan_bytes, T, L, K, R, num_slices, h, h_ld, false, stream);
 }
 
 extern "C" int b200_lora_expand(const void* h, int64_t h_ld, const void* B, int dtype, const void* plan, size_t plan_bytes,
@@ -1026,13 +1236,23 @@ extern "C" int b200_lora_apply(const void* x, int64_t x_ld, const void* A, const
                                size_t plan_bytes, const float* scalings, int64_t T, int L, int64_t K, int R,
                                const int64_t* slice_sizes, int num_slices, const void* base, int64_t base_ld, void* out,
                                int64_t out_ld, void* h, void* stream) {
+  using namespace b200;
   const int64_t h_ld = static_cast<int64_t>(num_slices) * R;
-  const int rc = b200::expand_entry(h, h_ld, B, dtype, plan, plan_bytes, scalings, T, L, R, slice_sizes, num_slices, base, base_ld, out,
-                                    out_ld, true, true, stream);
+  int rc = expand_entry(h, h_ld, B, dtype, plan, plan_bytes, scalings, T, L, R, slice_sizes, num_slices, base, base_ld, out, out_ld, true,
+                        true, stream);
   if (rc != B200_OK) return rc;
-  const int rc2 = b200::shrink_entry(x, x_ld, A, dtype, plan, plan_bytes, T, L, K, R, num_slices, h, h_ld, stream);
-  if (rc2 != B200_OK) return rc2;
+  if ((rc = shrink_entry(x, x_ld, A, dtype, plan, plan_bytes, T, L, K, R, num_slices, h, h_ld, true, stream)) != B200_OK) return rc;
+  const Slices sl = make_slices(slice_sizes, num_slices, 64, 64);
+  if (T > 0 && sl.first_col[num_slices] > 0 && K > 0) {
+    const int64_t tiles = max_tiles(T, L), N = sl.first_col[num_slices];
+    const int parts = fused_parts(T, L, tiles, static_cast<int>(h_ld), sl);
+    if (parts > 0)
+      return (dtype == B200_DT_BF16 ? fused<__nv_bfloat16> : fused<__half>)(
+          x, x_ld, A, B, K, N, R, static_cast<int>(h_ld), scalings, view_plan(plan, T, L), sl, tiles, parts, base, base_ld, out, out_ld,
+          static_cast<cudaStream_t>(stream));
+  }
+  if ((rc = shrink_entry(x, x_ld, A, dtype, plan, plan_bytes, T, L, K, R, num_slices, h, h_ld, false, stream)) != B200_OK) return rc;
   // with K = 0 there is no kernel before the expand that would make reading ahead sound
-  return b200::expand_entry(h, h_ld, B, dtype, plan, plan_bytes, scalings, T, L, R, slice_sizes, num_slices, base, base_ld, out, out_ld,
-                            K > 0, false, stream);
+  return expand_entry(h, h_ld, B, dtype, plan, plan_bytes, scalings, T, L, R, slice_sizes, num_slices, base, base_ld, out, out_ld, K > 0,
+                      false, stream);
 }

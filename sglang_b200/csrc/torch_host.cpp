@@ -801,6 +801,17 @@ HOST_FN(lora_plan) {
 }
 HOST_END
 
+// Whether rows of t and u [T, width] share memory.  Two ranges of columns of one buffer do not, although they lie between each other.
+bool share_rows(const Tensor& t, const Tensor& u) {
+  if (!t.defined() || !u.defined() || t.numel() == 0 || u.numel() == 0) return false;
+  const int64_t size = t.element_size(), wt = t.size(1), wu = u.size(1), st = stride_of(t, 0), su = stride_of(u, 0);
+  const char *pt = static_cast<const char*>(t.data_ptr()), *pu = static_cast<const char*>(u.data_ptr());
+  if (pt + (st * (t.size(0) - 1) + wt) * size <= pu || pu + (su * (u.size(0) - 1) + wu) * size <= pt) return false;
+  if (st != su || wt > st || wu > st) return true;
+  const int64_t d = ((pu - pt) % (st * size) + st * size) % (st * size);       // where u's columns begin, seen from t's
+  return d < wt * size || (st * size - d) < wu * size;
+}
+
 // lora(base | None, x [T, K] | None, h [T, S R] | None, lora_a [L, S R, K] | None, lora_b [L, N, R] | None, plan, num_adapters,
 //      scalings, sizes (a tuple of S) | None, num_slices, out | None) -> out [T, N]: shrink and expand; without lora_b only the
 // shrink, which returns h; without x only the expand.
@@ -874,6 +885,11 @@ HOST_FN(lora) {
     need_rows(t, 8, what);
     need_aligned(t, what);
     need_own_rows(t, what);
+  }
+  if (out.defined() && out.numel() > 0) {
+    const bool same = base.defined() && base.data_ptr() == out.data_ptr() && stride_of(base, 0) == stride_of(out, 0);
+    NEED(same || !share_rows(out, base), "out must be base_output itself or share no memory with it");
+    NEED(!share_rows(out, x) && !share_rows(out, h), "out must share no memory with x or h");
   }
   const at::Device dev = one_device({&plan, &base, &x, &h, &A, &B, &scalings, &out});
   int rc = 0;

@@ -63,9 +63,11 @@ def lora_expand(h: torch.Tensor, lora_b: torch.Tensor, batch: LoRABatch, base_ou
 def apply_lora(base_output: Optional[torch.Tensor], x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                batch: LoRABatch, output_sizes: Optional[Sequence[int]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Adds the adapters' part for x [num_tokens, K] to base_output [num_tokens, N], in place unless `out` is given; None counts
-    as zeros and gives a new tensor.  output_sizes: the columns of each slice (None: one slice).  bf16 or fp16 throughout; K, R
-    and the slices' sizes are multiples of 8, R <= 256, at most 8 slices.  The sums are fp32; x A^T, unscaled, is rounded to x's
-    type in between (in fp16 it must stay below 65504), the result once."""
+    as zeros and gives a new tensor.  The result shares memory with neither x nor, unless it is base_output itself, base_output.
+    output_sizes: the columns of each slice (None: one slice).  bf16 or fp16 throughout; K, R and the slices' sizes are multiples
+    of 8, R <= 256, at most 8 slices.  The sums are fp32; x A^T, unscaled, is rounded to x's type in between (in fp16 it must
+    stay below 65504), the result once.  The order of the sums, which is the same in every run, depends on the sizes, the number
+    of tokens among them."""
     if out is None:
         out = base_output
     sizes = None if output_sizes is None else tuple(output_sizes)

@@ -142,6 +142,24 @@ def test_lora_refusals(change, message):
         _lora_call(**change)
 
 
+def test_lora_refuses_an_output_that_is_read_elsewhere():
+    """Columns of one buffer beside one another are fine (they get as far as the question of the device)."""
+    z = torch.zeros(5, 256, dtype=BF)
+    for base, x, out, message in (
+            (z[:, :96], z[:, 96:160], None, "CUDA"), (z[:, 160:], z[:, 96:160], z[:, :96], "CUDA"),
+            (z[:, :96], z[:, 64:128], None, "no memory with x"), (z[:, 128:224], z[:, :64], z[:, 56:152], "no memory with x|base_output"),
+            (z[:, :96], z[:, 192:], z[:, 8:104], "base_output itself"), (z[:1, :96].expand(5, 96), z[:, 192:], z[:, 96:192], "overlap"),
+            (None, z[:, :64], z[:, :96], "no memory with x"),
+            (None, z.view(10, 128)[:5, :64], z[:, 160:], "no memory with x")):
+        with pytest.raises(RuntimeError, match=message):
+            _lora_call(base_output=base, x=x, out=out)
+    y = torch.zeros(10, 96, dtype=BF)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        _lora_call(base_output=y[5:], out=y[:5])
+    with pytest.raises(RuntimeError, match="base_output itself"):
+        _lora_call(base_output=y[4:9], out=y[:5])
+
+
 @pytest.mark.parametrize("stride", [0, 8])
 def test_lora_refuses_rows_that_overlap(stride):
     """A row broadcast over all tokens would be read as if the rows followed one another."""

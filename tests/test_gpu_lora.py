@@ -66,6 +66,7 @@ CASES = [
     (9, 256, [128, 0, 64], 24, 3), (16, 4096, [64, 64], 64, 2), (17, 520, [264], 128, 4), (33, 96, [40, 24, 16, 8], 256, 3),
     (129, 1024, [256, 64, 64], 64, 33), (300, 264, [136], 32, 1000), (515, 512, [320, 64, 64], 64, 3), (1000, 2048, [512, 512], 16, 2),
     (2049, 320, [192], 8, 40), (700, 136, [72, 72], 128, 2), (640, 200, [48, 16], 256, 2), (513, 8, [32, 8], 72, 2),
+    (16, 256, [512, 64], 16, 2), (5, 264, [2048, 1024, 1024], 8, 2), (33, 520, [64], 32, 2), (3, 8200, [16384], 24, 9), (12, 1032, [8, 72], 16, 3),
     (255, 192, [40], 16, 2), (256, 192, [40], 16, 2), (263, 128, [16, 24], 24, 11), (264, 128, [16, 24], 24, 11), (257, 648, [264, 8], 64, 10),
 ]
 
@@ -127,8 +128,8 @@ def test_nobody_has_an_adapter(T):
 def test_several_streams_at_once():
     """Calls of one batch on several streams, each with its own tokens and output."""
     from sglang_b200.layers.lora import LoRABatch, apply_lora
-    for T in (6, 300):
-        cases = [_case(T, 512, [128, 64], 32, 3, BF, 50 + i) for i in range(4)]
+    for T, R in ((6, 16), (6, 32), (300, 32)):
+        cases = [_case(T, 512, [128, 64], R, 3, BF, 50 + i) for i in range(4)]
         x0, _, A, B, ids, ranks, scal = cases[0]
         Ad, Bd = A.cuda(), B.cuda()
         batch = LoRABatch(ids.cuda(), ranks.cuda(), scal.cuda())
@@ -166,8 +167,8 @@ def test_strided_views_and_odd_ids():
 def test_a_token_s_result_depends_on_its_own_row_only():
     """Infinities and NaN in one token leave every other token's bits alone; so does the company a token is in."""
     from sglang_b200.layers.lora import LoRABatch, apply_lora
-    for T in (24, 270, 700):
-        x, base, A, B, ids, ranks, scal = _case(T, 320, [96, 32], 32, 3, BF, T)
+    for T, R in ((10, 16), (24, 32), (270, 32), (700, 32)):
+        x, base, A, B, ids, ranks, scal = _case(T, 320, [96, 32], R, 3, BF, T)
         one = lambda xx, rows: apply_lora(base[rows].cuda(), xx[rows].cuda(), A.cuda(), B.cuda(),  # noqa: E731
                                           LoRABatch(ids[rows].cuda(), ranks.cuda(), scal.cuda()), [96, 32])
         every = torch.arange(T)
@@ -201,12 +202,12 @@ def test_segments_and_update():
     _close(out, want, tol)
 
 
-@pytest.mark.parametrize("T", [5, 260, 600])
-def test_captured_and_replayed_on_a_side_stream(T):
+@pytest.mark.parametrize("T,R", [(5, 16), (5, 32), (260, 32), (600, 32)])
+def test_captured_and_replayed_on_a_side_stream(T, R):
     """Planning, shrink and expand in one graph; new tokens and ids are copied in before each replay.  Two graphs share nothing
     but the weights."""
     from sglang_b200.layers.lora import LoRABatch, apply_lora
-    K, sizes, R, L = 256, [64, 64], 32, 6
+    K, sizes, L = 256, [64, 64], 6
     _, _, A, B, _, ranks, scal = _case(1, K, sizes, R, L, BF, 1)
     Ad, Bd, graphs = A.cuda(), B.cuda(), []
     for _ in range(2):
