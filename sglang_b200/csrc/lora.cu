@@ -174,87 +174,105 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int keep) {
 }
 
 // ------------------------------------------------------------------------------------------------------- shrink
-constexpr int kShrinkThreads = 128, kShrinkWarps = kShrinkThreads / 32, kShrinkStages = 5;
-constexpr int kShrinkSmem = kShrinkWarps * kShrinkStages * 2048;
+constexpr int kShrinkThreads = 128, kShrinkWarps = kShrinkThreads / 32;
+template <int Z>
+struct Shrink {
+  static constexpr int kStages = Z == 1 ? 5 : 4, kStageBytes = (2 * Z + 2) * 512;
+  static constexpr int kSmem = kShrinkWarps * kStages * kStageBytes;
+};
 
-// A cluster of up to eight blocks computes 16 columns of h for one tile of up to 16 tokens, all its warps dividing K; the partial
+// A cluster of up to eight blocks computes Z groups of 16 columns of h for one tile of up to 16 tokens, all its warps dividing K; the partial
 // sums are added in a fixed order, first over a block's warps, then over the blocks through distributed shared memory.  A warp's
 // operands come through a ring of k32 steps in shared memory in which each lane has its own place (nothing to synchronise):
 // with loads into registers instead, 128 tokens of 32 adapters over K = 8192 and three slices of 64 took 25.6 us.
-template <typename T>
+template <typename T, int Z>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ A,
                                                                      int64_t K, int R, int cols, PlanView plan,
                                                                      T* __restrict__ h, int64_t h_ld) {
+  using S = Shrink<Z>;
   pdl_start();
   extern __shared__ __align__(128) uint8_t dyn[];
-  __shared__ float part[kShrinkWarps][256];
-  __shared__ float mine[256];
+  __shared__ float part[kShrinkWarps][Z * 256];
+  __shared__ float mine[Z * 256];
   const int tiles = plan.count[0];
   const int4 tile = plan.tiles[blockIdx.y];                          // in bounds whether or not it is one
   if (static_cast<int>(blockIdx.y) >= tiles) return;                 // the whole cluster leaves together, here and below
-  const int c0 = blockIdx.z * 16, splits = gridDim.x;
+  const int splits = gridDim.x, c0 = blockIdx.z * (Z * 16);
   const int rows = tile.z, rank = tile.x < 0 ? 0 : min(tile.w, R);
-  if (c0 % R >= rank && (c0 + 8 >= cols || (c0 + 8) % R >= rank)) {  // behind the rank (R % 8 == 0), or no adapter: zeros
+  bool any = false;
+#pragma unroll
+  for (int i = c0; i < c0 + Z * 16; i += 8) any |= i < cols && i % R < rank;
+  if (!any) {                                                        // behind the rank (R % 8 == 0), or no adapter: zeros
     if (blockIdx.x == 0)
-      for (int e = threadIdx.x; e < 256; e += kShrinkThreads)
-        if (e / 16 < rows && c0 + e % 16 < cols) h[static_cast<int64_t>(plan.perm[tile.y + e / 16]) * h_ld + c0 + e % 16] = static_cast<T>(0.f);
+      for (int e = threadIdx.x; e < Z * 256; e += kShrinkThreads) {
+        const int row = e / 16 % 16, col = c0 + e / 256 * 16 + e % 16;
+        if (row < rows && col < cols) h[static_cast<int64_t>(plan.perm[tile.y + row]) * h_ld + col] = static_cast<T>(0.f);
+      }
     return;
   }
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
   const int r0 = __ldg(plan.perm + tile.y + min(g, rows - 1)), r1 = __ldg(plan.perm + tile.y + min(g + 8, rows - 1));
   const int chunks = static_cast<int>((K + 31) / 32), per = (chunks + splits * kShrinkWarps - 1) / (splits * kShrinkWarps);
   const int begin = (blockIdx.x * kShrinkWarps + warp) * per, end = min(begin + per, chunks);
-  // this lane's four operands: rows lane / 4 and lane / 4 + 8 of A and of x; absent ones are zero-filled copies of nothing
-  const char* src[4];
-  bool there[4];
+  // this lane's operands: rows lane / 4 and lane / 4 + 8 of A (of each group) and of x; absent ones are zero-filled copies of nothing
+  const char* src[2 * Z + 2];
+  bool there[2 * Z + 2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int col = c0 + g + 8 * (i % 2);
-    const bool in = i < 2 ? col < cols && col % R < rank : g + 8 * (i % 2) < rows;
-    const T* row = i < 2 ? A + (static_cast<int64_t>(tile.x) * cols + col) * K : x + (i == 2 ? r0 : r1) * x_ld;
-    src[i] = reinterpret_cast<const char*>(in ? row + static_cast<int64_t>(begin) * 32 + 8 * c : A);
+  for (int i = 0; i < 2 * Z + 2; ++i) {
+    const int row = g + 8 * (i % 2), col = c0 + i / 2 * 16 + row;
+    const bool in = i < 2 * Z ? col < cols && col % R < rank : row < rows;
+    const T* p = i < 2 * Z ? A + (static_cast<int64_t>(tile.x) * cols + col) * K : x + (i % 2 == 0 ? r0 : r1) * x_ld;
+    src[i] = reinterpret_cast<const char*>(in ? p + static_cast<int64_t>(begin) * 32 + 8 * c : A);
     there[i] = in;
   }
   const bool both = rows > 8;
-  float acc[2][4] = {};
-  const uint32_t ring = smem_u32(dyn) + warp * (kShrinkStages * 2048) + lane * 16, ring_end = ring + kShrinkStages * 2048;
+  float acc[Z][2][4] = {};
+  const uint32_t ring = smem_u32(dyn) + warp * (S::kStages * S::kStageBytes) + lane * 16, ring_end = ring + S::kStages * S::kStageBytes;
   const int ragged = K % 32 != 0 && 8 * c >= K % 32 ? chunks - 1 : -1;       // the step of which this lane has nothing
   uint32_t to = ring, from = ring;
-  auto fetch = [&](int i) {                                          // a stage: [A lo, A hi, x lo, x hi][lane]
+  auto fetch = [&](int i) {                                          // a stage: [A lo, A hi (of each group), x lo, x hi][lane]
     if (i == ragged) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) there[j] = false, src[j] = reinterpret_cast<const char*>(A);
+      for (int j = 0; j < 2 * Z + 2; ++j) there[j] = false, src[j] = reinterpret_cast<const char*>(A);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j < 3 || both) sa::cp_async_or_zero<16>(to + 512 * j, src[j], there[j]);
+    for (int j = 0; j < 2 * Z + 2; ++j) {
+      if (j < 2 * Z + 1 || both) sa::cp_async_or_zero<16>(to + 512 * j, src[j], there[j]);
       src[j] += 64;
     }
-    to = to + 2048 == ring_end ? ring : to + 2048;
+    to = to + S::kStageBytes == ring_end ? ring : to + S::kStageBytes;
   };
 #pragma unroll 1
-  for (int i = 0; i < kShrinkStages - 1; ++i) {
+  for (int i = 0; i < S::kStages - 1; ++i) {
     if (begin + i < end) fetch(begin + i);
     sa::cp_async_commit();
   }
 #pragma unroll 2
   for (int i = begin; i < end; ++i) {
-    if (i + kShrinkStages - 1 < end) fetch(i + kShrinkStages - 1);
+    if (i + S::kStages - 1 < end) fetch(i + S::kStages - 1);
     sa::cp_async_commit();
-    sa::cp_async_wait<kShrinkStages - 1>();
+    sa::cp_async_wait<S::kStages - 1>();
     __syncwarp();
-    const uint4 lo = sa::ld_v4(from), hi = sa::ld_v4(from + 512);
-    mma_k32<T>(acc[0], lo, hi, sa::ld_v4(from + 1024));
-    if (both) mma_k32<T>(acc[1], lo, hi, sa::ld_v4(from + 1536));
-    from = from + 2048 == ring_end ? ring : from + 2048;
+    const uint4 x0 = sa::ld_v4(from + 2 * Z * 512);
+    uint4 x1 = make_uint4(0, 0, 0, 0);
+    if (both) x1 = sa::ld_v4(from + (2 * Z + 1) * 512);
+#pragma unroll
+    for (int z = 0; z < Z; ++z) {
+      const uint4 lo = sa::ld_v4(from + 2 * z * 512), hi = sa::ld_v4(from + (2 * z + 1) * 512);
+      mma_k32<T>(acc[z][0], lo, hi, x0);
+      if (both) mma_k32<T>(acc[z][1], lo, hi, x1);
+    }
+    from = from + S::kStageBytes == ring_end ? ring : from + S::kStageBytes;
   }
-  // part[warp][token][column]
+  // part[warp][group][token][column]
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int z = 0; z < Z; ++z)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part[warp][(8 * i + 2 * c + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[i][j];
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[warp][z * 256 + (8 * i + 2 * c + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[z][i][j];
   __syncthreads();
-  for (int e = threadIdx.x; e < 256; e += kShrinkThreads) {
+  for (int e = threadIdx.x; e < Z * 256; e += kShrinkThreads) {
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kShrinkWarps; ++w) sum += part[w][e];
@@ -262,9 +280,9 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const T* __
   }
   cg::cluster_group cluster = cg::this_cluster();
   if (splits > 1) cluster.sync();
-  const int share = 256 / splits;                                    // one block: each thread reads what it has written
+  const int share = Z * 256 / splits;                                // one block: each thread reads what it has written
   for (int i = threadIdx.x; i < share; i += kShrinkThreads) {
-    const int e = static_cast<int>(blockIdx.x) * share + i, row = e / 16, col = c0 + e % 16;
+    const int e = static_cast<int>(blockIdx.x) * share + i, row = e / 16 % 16, col = c0 + e / 256 * 16 + e % 16;
     float sum = 0.f;
     if (splits == 1) {
       sum = mine[e];
@@ -511,15 +529,17 @@ constexpr int kExpandThreads = 128;
 
 // A warp takes `per` neighbouring blocks of 64 columns (each within a slice) for one tile of up to 16 tokens.  Weight row (tile i,
 // half f, lane / 4) of its four 16-row operands is column 8 (lane / 4) + 2 i + f, so that the eight sums that a lane holds for a
-// token are neighbours: base and out move 16 bytes at a time.  Operands come through a ring of (block, 32 ranks) steps in shared
-// memory in which each lane has its own places: [B: 8][base: 4][h: 2] vectors.
+// token are neighbours: base and out move 16 bytes at a time.  B comes through a ring of (block, 32 ranks) steps in shared memory in
+// which each lane has its own places; base and h go straight into registers.  What bounds it is how many warps fit: with base and
+// h in a ring of three steps, 8 warps an SM, 128 tokens of 32 adapters (ranks 16 to 64, N = 10240) took 12.3 us, now 9.6; with
+// three steps and 16 warps 9.7, with two and 20 warps, whose registers spill, 10.3.
 // early: the shrink before it is this library's own, launched in the same call, and triggered after its wait; what was there
 // before the shrink (the plan, B and base) may then be read ahead of the wait, which only h has to be behind.
-constexpr int kExpandStages = 3, kExpandStageBytes = 14 * 512;
+constexpr int kExpandStages = 2, kExpandStageBytes = 8 * 512;
 constexpr int kExpandSmem = kExpandThreads / 32 * kExpandStages * kExpandStageBytes;
 
 template <typename T>
-__global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h, int h_ld, const T* __restrict__ B, int64_t N, int R,
+__global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const T* h, int h_ld, const T* __restrict__ B, int64_t N, int R,
                                                                      const float* __restrict__ scalings, PlanView plan,
                                                                      const __grid_constant__ Slices sl, const T* base, int base_ld,
                                                                      T* out, int out_ld, int per, bool early) {
@@ -551,9 +571,7 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h,
     uint32_t place;
   };
   auto enter = [&](At& p) {                                  // slice and first column (of this lane's eight) of its block
-    p.s = 0;
-#pragma unroll
-    for (int i = 1; i < kMaxSlices; ++i) p.s += i < sl.n && p.block >= sl.first_block[i];
+    while (p.s + 1 < sl.n && p.block >= sl.first_block[p.s + 1]) ++p.s;
     p.n = sl.first_col[p.s] + (p.block - sl.first_block[p.s]) * 64 + 8 * g;
     p.live = p.n < sl.first_col[p.s + 1];
   };
@@ -576,48 +594,49 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h,
     const uint32_t ld = static_cast<uint32_t>(row_bytes);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sa::cp_async_or_zero<16>(p.place + i * 512, src + i * ld, in);
-    if (base != nullptr && p.j + 1 == chunks) {              // with the block's last step, which stores
+  };
+  uint4 v[4];                                                // base, of a block ahead
+  auto fetch_base = [&](const At& p) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i >= 2 && !both) continue;
-        const bool mine = p.live && 8 * (i / 2) + 2 * c + i % 2 < rows;
-        sa::cp_async_or_zero<16>(p.place + (8 + i) * 512, mine ? base + static_cast<int64_t>(token[i]) * base_ld + p.n : base, mine);
-      }
+    for (int i = 0; i < 4; ++i) {
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (base != nullptr && p.live && 8 * (i / 2) + 2 * c + i % 2 < rows)
+        v[i] = *reinterpret_cast<const uint4*>(base + static_cast<int64_t>(token[i]) * base_ld + p.n);
     }
   };
   const T* h0[2] = {h + static_cast<int64_t>(h_row[0]) * h_ld + 8 * c, h + static_cast<int64_t>(h_row[1]) * h_ld + 8 * c};
+  uint4 hv[2];
   auto fetch_h = [&](const At& p) {
     const bool in = rank - 32 * p.j - 8 * c > 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool mine = in && g + 8 * i < rows;
-      if (i == 0 || both) sa::cp_async_or_zero<16>(p.place + (12 + i) * 512, mine ? h0[i] + p.s * R + 32 * p.j : h, mine);
+      hv[i] = make_uint4(0, 0, 0, 0);
+      if (in && g + 8 * i < rows) hv[i] = *reinterpret_cast<const uint4*>(h0[i] + p.s * R + 32 * p.j);
     }
   };
-  static_assert(kExpandStages == 3, "two steps ahead");
   fetch_weights(in_flight);
-  At second = in_flight;
-  if (steps > 1) {
-    advance(second);
-    fetch_weights(second);
-  }
-  if (early) pdl_wait();
-  pdl_trigger();
-  fetch_h(in_flight);
   sa::cp_async_commit();
-  if (steps > 1) fetch_h(second);
-  sa::cp_async_commit();
-  in_flight = second;
-  float acc[2][4][4];
-#pragma unroll 1
-  for (int step = 0; step < steps; ++step, advance(at)) {
-    if (step + 2 < steps) {
+#pragma unroll
+  for (int i = 1; i < kExpandStages - 1; ++i) {
+    if (steps > i) {
       advance(in_flight);
       fetch_weights(in_flight);
-      fetch_h(in_flight);
     }
     sa::cp_async_commit();
-    sa::cp_async_wait<2>();
+  }
+  fetch_base(at);
+  if (early) pdl_wait();
+  pdl_trigger();
+  fetch_h(at);
+  float acc[2][4][4];
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    if (step + kExpandStages - 1 < steps) {
+      advance(in_flight);
+      fetch_weights(in_flight);
+    }
+    sa::cp_async_commit();
+    sa::cp_async_wait<kExpandStages - 1>();
     __syncwarp();                                            // lanes that stored come back to those that had nothing to store
     const uint32_t from = at.place;
     const int j = at.j;
@@ -627,33 +646,34 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_kernel(const T* h,
     }
     if (!none) {
       const int keep = rank - 32 * j - 8 * c;
-      const uint4 x0 = sa::ld_v4(from + 12 * 512);
-      uint4 x1 = make_uint4(0, 0, 0, 0);
-      if (both) x1 = sa::ld_v4(from + 13 * 512);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint4 lo = sa::ld_v4(from + 2 * i * 512), hi = sa::ld_v4(from + (2 * i + 1) * 512);
         if (keep > 0 && keep < 8) lo = first_of(lo, keep), hi = first_of(hi, keep);
-        mma_k32<T>(acc[0][i], lo, hi, x0);
-        if (both) mma_k32<T>(acc[1][i], lo, hi, x1);
+        mma_k32<T>(acc[0][i], lo, hi, hv[0]);
+        if (both) mma_k32<T>(acc[1][i], lo, hi, hv[1]);
       }
     }
-    if (j + 1 < chunks || !at.live) continue;
+    const At old = at;
+    advance(at);
+    if (step + 1 < steps && (at.j != old.j || at.s != old.s)) fetch_h(at);
+    if (j + 1 < chunks) continue;
+    if (old.live) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (8 * (i / 2) + 2 * c + i % 2 >= rows) continue;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (base != nullptr) v = sa::ld_v4(from + (8 + i) * 512);
-      if (!none) {
-        uint32_t* q = &v.x;
+      for (int i = 0; i < 4; ++i) {
+        if (8 * (i / 2) + 2 * c + i % 2 >= rows) continue;
+        if (!none) {
+          uint32_t* q = &v[i].x;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const float2 b = unpack2<T>(q[m]);
-          q[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[i / 2][m][i % 2], b.x), fmaf(scaling, acc[i / 2][m][i % 2 + 2], b.y));
+          for (int m = 0; m < 4; ++m) {
+            const float2 b = unpack2<T>(q[m]);
+            q[m] = pack2(static_cast<T*>(nullptr), fmaf(scaling, acc[i / 2][m][i % 2], b.x), fmaf(scaling, acc[i / 2][m][i % 2 + 2], b.y));
+          }
         }
+        *reinterpret_cast<uint4*>(out + static_cast<int64_t>(token[i]) * out_ld + old.n) = v[i];
       }
-      *reinterpret_cast<uint4*>(out + static_cast<int64_t>(token[i]) * out_ld + at.n) = v;
     }
+    if (step + 1 < steps) fetch_base(at);
   }
 }
 
@@ -1007,15 +1027,29 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
     return B200_OK;
   }
   if (tile_rows(tokens, adapters) == kSmallRows) {
-    // Enough blocks for six on every SM (of the tiles that a plan may have about half are used, and five blocks are resident), if
-    // K has a k32 step for each of their warps.
+    // K is divided as far as all blocks can be resident, five on an SM, if it has a k32 step for each of their warps.  Two groups of
+    // columns a block, which is four on an SM, where single ones would not be divided at all, or full tiles not by eight.  Blocks of
+    // one group divided by 8 / 4 / 2, and of two by 8 / 4 / 2 (us; K = 8192, with the expand, 4 and 5 stages): 128 tokens of 32
+    // adapters, 3 slices of 16: 18.6 15.6 17.5, 19.8 16.1 18.3; of 64 34.4 27.8 24.9, 37.2 29.6 25.5 with mixed ranks, 42.0 36.8
+    // 34.8, 45.1 36.8 33.6 with rank 64 only; 200 tokens of one adapter 21.9 19.5 17.2, 19.1 14.8 19.
     const int passes = (cols + 15) / 16;
-    int splits = 1;
-    while (splits < 8 && tiles * passes * splits < 6LL * sms && splits * 32 * kShrinkWarps < K) splits *= 2;
-    B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShrinkSmem));
-    B200_CUDA_TRY(launch_cluster(lora_shrink_kernel<T>, dim3(splits, static_cast<unsigned>(tiles), passes), dim3(kShrinkThreads),
-                                 kShrinkSmem, splits, st, x, x_ld, A, K, R, cols, plan, h, h_ld));
-    return B200_OK;
+    const int64_t few = adapters < tokens ? adapters : tokens, half = (tokens + kSmallRows - 1) / kSmallRows + few / 2, about = few > half ? few : half;
+    auto divided = [&](int64_t blocks, int64_t most) {
+      int n = 1;
+      while (n < 8 && 2 * n * blocks <= most && n * 32 * kShrinkWarps < K) n *= 2;
+      return n;
+    };
+    auto go = [&](auto z, int splits) -> int {
+      constexpr int Z = decltype(z)::value;
+      B200_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_kernel<T, Z>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shrink<Z>::kSmem));
+      B200_CUDA_TRY(launch_cluster(lora_shrink_kernel<T, Z>, dim3(splits, static_cast<unsigned>(tiles), (passes + Z - 1) / Z),
+                                   dim3(kShrinkThreads), Shrink<Z>::kSmem, splits, st, x, x_ld, A, K, R, cols, plan, h, h_ld));
+      return B200_OK;
+    };
+    const int64_t blocks = about * passes, most = 5LL * sms;
+    if (2 * blocks > most || (8 * blocks > most && tokens >= kSmallRows * static_cast<int64_t>(adapters)))
+      return go(std::integral_constant<int, 2>(), divided((blocks + 1) / 2, 4LL * sms));
+    return go(std::integral_constant<int, 1>(), divided(blocks, most));
   }
   if (gemm_sticky_status() != 0) return B200_ERR_DEVICE_TIMEOUT;
   ShrinkTiles p = {K, h_ld, R, slices};
@@ -1067,10 +1101,11 @@ int expand(const T* h, int64_t h_ld, const T* B, int64_t N, int R, const float* 
   const int sms = sm_count();
   if (sms <= 0) return B200_ERR_CUDA;
   constexpr int kWarps = kExpandThreads / 32;
-  // small batches: as many blocks of columns a warp as leave eight warps for each SM, at most eight
+  // small batches: as many blocks of columns a warp as leave 24 warps for each SM (16 are resident), at most eight.  1, 2, 4, 8 of
+  // them: 41 tiles of N = 36864, R = 32: 21.3, 20.6, 19.0, 17.9 us; of 10240, ranks 16 to 64: 9.6, 10.7, 11.9, 16.1
   int per = 1;
   if (tile_rows(tokens, adapters) == kSmallRows) {
-    const int64_t most = tiles * sl.first_block[sl.n] / (8LL * sms);
+    const int64_t most = tiles * sl.first_block[sl.n] / (24LL * sms);
     per = static_cast<int>(most < 1 ? 1 : most < 8 ? most : 8);
   }
   const dim3 grid(static_cast<unsigned>((sl.first_block[sl.n] + kWarps * per - 1) / (kWarps * per)), static_cast<unsigned>(tiles));
