@@ -177,7 +177,7 @@ enum { kRaw = -1, kNorm = 0, kNeox = 1, kPairs = 2 };
 // A lane holds two runs of eight elements, half of the row apart: a group's 16-byte accesses are then neighbours (with sixteen
 // elements in one run every access took half of a sector, and 8192 tokens of 36 heads 36.8 us).  With neox pairs the runs are half
 // of the rotated part apart, so that a rotation stays inside the lane, and half of the rest in the rest.
-// pos: the token's position (no rotation: 0); slot: its place in the cache (CODES); both were loaded ahead and are looked at only
+// pos: the token's position (none given: 0); slot: its place in the cache (CODES); both were loaded ahead and are looked at only
 // when the first rows are under way.
 template <typename T, int G, int KIND, bool STORE, bool CODES>
 __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& r, uint32_t ring, int lane, int64_t pos, int64_t slot,
@@ -218,7 +218,7 @@ __device__ __forceinline__ void do_rows(const HeadRowsParams& p, const Rows<T>& 
   }
   const bool poisoned = ROPE && pos >= p.max_position;         // a position that the table lacks: NaN, not a read behind it
   const bool keep = CODES && slot >= 0 && slot < p.num_slots;
-  if ((ROPE && pos < 0) || !(keep || (STORE && r.dst != nullptr))) {     // padding, or nowhere to go: nothing is written
+  if (pos < 0 || !(keep || (STORE && r.dst != nullptr))) {     // padding, or nowhere to go: nothing is written
     sa::cp_async_wait<0>();
     return;
   }
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kMaxThreads, 11) head_rows_kernel(const __grid
   if (tok32 >= p.T) return;
   const int64_t tok = tok32;
   int chunk = static_cast<int>(item - tok32 * p.chunks);
-  const int64_t pos = ROPE ? load_index(p.positions, p.pos_i64, tok) : 0;
+  const int64_t pos = ROPE || (KIND == kNorm && p.positions != nullptr) ? load_index(p.positions, p.pos_i64, tok) : 0;
   const int64_t slot = p.Hv != 0 && chunk >= p.chunks_q ? load_index(p.slots, p.slots_i64, tok) : -1;
   Rows<T> r = {};
   if (chunk < p.chunks_q) {
@@ -588,7 +588,7 @@ int rows_entry(const b200_heads* q, const b200_heads* k, const b200_heads* v, co
   for (int i = 0; i < 31; ++i)
     if (p.page_size == 1u << i) p.page_shift = i;
   // only a store alone takes its rows as they are: k_out without a rotation or a weight is a copy, which kNorm makes
-  const int kind = cos_sin ? (is_neox ? kNeox : kPairs) : Hq == 0 && !k_weight && !k_out ? kRaw : kNorm;
+  const int kind = cos_sin ? (is_neox ? kNeox : kPairs) : Hq == 0 && !k_weight && !k_out && !positions ? kRaw : kNorm;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == B200_DT_BF16 ? dispatch_rows<__nv_bfloat16>(p, kind, st) : dispatch_rows<__half>(p, kind, st);
 }

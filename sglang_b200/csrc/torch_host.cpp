@@ -654,9 +654,9 @@ HOST_FN(head_rows) {
     NEED(v.scalar_type() == type, "k and v must have the same type");
   }
   int64_t rot = 0, rows = 0;
+  if (pos.defined()) need_index(pos, T, "positions");
   if (cs.defined()) {
     NEED(pos.defined(), "positions must be given with cos_sin_cache");
-    need_index(pos, T, "positions");
     need_type(cs, at::kFloat, "cos_sin_cache", "float32");
     NEED(cs.dim() == 2 && cs.is_contiguous(), "cos_sin_cache must be a contiguous [max_position, rotary_dim] tensor");
     rows = cs.size(0), rot = cs.size(1);
@@ -697,7 +697,7 @@ HOST_FN(head_rows) {
     if (T > 0 && Hq + Hkv > 0) {
       const b200_heads qh = q.defined() ? heads_of(q) : b200_heads{}, kh = heads_of(k), vh = v.defined() ? heads_of(v) : b200_heads{};
       const b200_heads qoh = qo.defined() ? heads_of(qo) : b200_heads{}, koh = ko.defined() ? heads_of(ko) : b200_heads{};
-      const void* pp = pos.defined() && cs.defined() ? pos.data_ptr() : nullptr;
+      const void* pp = pos.defined() ? pos.data_ptr() : nullptr;
       const float* cp = cs.defined() ? static_cast<const float*>(cs.data_ptr()) : nullptr;
       const int pos64 = pos.defined() && pos.scalar_type() == at::kLong;
       const void *qwp = qw.defined() ? qw.data_ptr() : nullptr, *kwp = kw.defined() ? kw.data_ptr() : nullptr;

@@ -24,7 +24,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Ten
     Every head is normalised with its weight [head_dim] (None: not), then its first cos_sin_cache.shape[1] elements are rotated
     by row positions[t] of cos_sin_cache [max_position, rotary_dim] (fp32, cosines | sines; None: no rotation): pairs
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with is_neox=False.  All in fp32, rounded once.  A token with a negative position
-    is padding: its rows of q_out and k_out stay as they are.  A position that the table lacks gives NaN.
+    is padding (also without a table): its rows of q_out and k_out stay as they are.  A position that the table lacks gives NaN.
     head_dim and rotary_dim are multiples of 16, head_dim at most 256; token and head strides multiples of 8 elements."""
     return _lib.host().head_rows("qk_norm_rope", q, k, None, positions, cos_sin_cache, q_weight, k_weight, norm_eps, is_neox,
                                  q_out, k_out, True, None, None, None, None, None)

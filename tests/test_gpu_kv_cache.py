@@ -112,6 +112,34 @@ def test_norm_rope_padding_and_positions_outside_the_table():
         assert (out[[1, 4]] == 9.0).all() and out[[3, 5]].isnan().all()
 
 
+@pytest.mark.parametrize("queries,weights", [(2, True), (2, False), (0, True), (0, False)])
+def test_padding_without_a_rotation(queries, weights):
+    """A negative position marks a token as padding whether or not there is a table."""
+    from sglang_b200.layers.quantization.kv_cache import qk_norm_rope_store_kv_fp8
+    from sglang_b200.layers.rotary_embedding import qk_norm_rope
+    T, H, D = 5, 3, 64
+    pos = torch.tensor([7, -1, 0, -5, 1 << 20], device="cuda")
+    idle = (pos < 0).cpu()
+    q, k, v = (torch.randn(T, h, D, device="cuda").to(BF) for h in (queries, H, H))
+    w = torch.ones(D, device="cuda", dtype=BF) if weights else None
+    qo, ko = torch.full_like(q, 9.0), torch.full_like(k, 9.0)
+    qk_norm_rope(q, k, pos, None, w, w, q_out=qo, k_out=ko)
+    assert (qo[pos < 0] == 9).all() and (ko[pos < 0] == 9).all()
+    want_q, want_k = qk_norm_rope(q, k, None, None, w, w)
+    assert torch.equal(qo[pos >= 0], want_q[pos >= 0]) and torch.equal(ko[pos >= 0], want_k[pos >= 0])
+    caches = []
+    for p in (pos, None):
+        cache = [torch.zeros(2, 4, H, D, device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
+        cache += [torch.full((2, 4, H), 3.0, device="cuda") for _ in range(2)]
+        qk_norm_rope_store_kv_fp8(q, k, v, p, None, *cache, torch.arange(T, device="cuda"), w, w)
+        caches.append([c.cpu() for c in cache])
+    for got, want in zip(*caches):
+        got, want = (c.view(torch.uint8) if c.dtype != torch.float32 else c for c in (got, want))
+        got, want = got.reshape(8, H, -1)[:T], want.reshape(8, H, -1)[:T]
+        assert torch.equal(got[~idle], want[~idle])
+        assert (got[idle] == (3 if got.dtype == torch.float32 else 0)).all()
+
+
 def test_infinities_and_nan_stay_in_their_head():
     from sglang_b200.layers.rotary_embedding import qk_norm_rope
     qkv, (qw, kw) = _inputs(4, 4, 2, 128, BF, 5)
