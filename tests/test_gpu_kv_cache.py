@@ -180,6 +180,32 @@ def test_store_gives_the_group_quantiser_s_codes(T, H, D, page, dtype):
         assert same_bits(scale.flatten(0, 1), want_s)
 
 
+@pytest.mark.parametrize("T,H,D,page", [(40000, 1, 128, 16), (30011, 2, 64, 48), (20001, 3, 128, 64), (70003, 1, 32, 7), (9001, 5, 48, 1), (1500, 1, 112, 16),
+                                        (12345, 2, 256, 16)])
+def test_store_of_many_tokens_with_few_heads(T, H, D, page):
+    """Rows of several tokens in one warp: the codes and scales are still the group quantiser's (heads of 32 and 48: those of a
+    store of a few tokens at a time), skipped slots and the rest of the cache stay."""
+    from sglang_b200.layers.quantization.kv_cache import store_kv_fp8
+    g = torch.Generator().manual_seed(T)
+    k, v = (torch.randn(T, H, D, generator=g).to(BF).cuda() for _ in range(2))
+    pages = (T + 100 + page - 1) // page
+    slots = torch.randperm(pages * page, generator=g)[:T]
+    slots[::7] = -1
+    slots[3] = pages * page
+    def empty():
+        return ([torch.zeros(pages, page, H, D, device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
+                + [torch.full((pages, page, H), 5.0, device="cuda") for _ in range(2)])
+    got, want = empty(), empty()
+    store_kv_fp8(k, v, *got, slots.cuda())
+    for at in range(0, T, 1000):
+        store_kv_fp8(k[at:at + 1000], v[at:at + 1000], *want, slots[at:at + 1000].cuda())
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    spare = torch.ones(pages * page, dtype=torch.bool)
+    spare[slots[(slots >= 0) & (slots < pages * page)]] = False
+    assert (got[2].cpu().view(-1, H)[spare] == 5).all() and (got[2].cpu().view(-1, H)[~spare] != 5).all()
+
+
 def test_store_special_values_as_the_group_quantiser():
     """Infinities, NaN, zeros, the smallest numbers and a scale whose significand is all ones."""
     from sglang_b200.layers.quantization.kv_cache import store_kv_fp8
