@@ -36,10 +36,12 @@ constexpr int kMaxAdapters = 1024;
 constexpr int kMaxSlices = 8;
 constexpr int64_t kMaxTokens = 1000000;     // max_tiles(kMaxTokens, kMaxAdapters) is a legal grid.y
 
-// Device layout of a plan: int32 count[4] (tiles, -, -, -), int4 tiles[max_tiles] (adapter or -1, first, rows, rank), int32 perm[T]
-__host__ __device__ inline int64_t max_tiles(int64_t T, int64_t L) {
-  return T / tile_rows(T, L) + (L + 1 < T ? L + 1 : T);
-}
+__host__ __device__ inline int64_t max_tiles(int64_t T, int64_t L, int rows) { return T / rows + (L + 1 < T ? L + 1 : T); }
+__host__ __device__ inline int64_t max_tiles(int64_t T, int64_t L) { return max_tiles(T, L, tile_rows(T, L)); }
+// Device layout of a plan: int32 count[4] (tiles, -, -, -), int4 tiles[plan_tiles] (adapter or -1, first, rows, rank), int32 perm[T].
+// The tiles have the room that small ones would need, so that a plan's size grows with every token and tells T: with the room
+// of the tiles that there are, 212 tokens in tiles of 16 and 256 in tiles of 128 had plans of one size and different layouts.
+__host__ __device__ inline int64_t plan_tiles(int64_t T, int64_t L) { return max_tiles(T, L, kSmallRows); }
 
 struct PlanView {
   const int* count;
@@ -49,7 +51,7 @@ struct PlanView {
 inline PlanView view_plan(const void* plan, int64_t T, int64_t L) {
   const char* b = static_cast<const char*>(plan);
   return {reinterpret_cast<const int*>(b), reinterpret_cast<const int4*>(b + 16),
-          reinterpret_cast<const int*>(b + 16 + 16 * max_tiles(T, L))};
+          reinterpret_cast<const int*>(b + 16 + 16 * plan_tiles(T, L))};
 }
 
 // ------------------------------------------------------------------------------------------------------- plan
@@ -1167,7 +1169,7 @@ int check_sizes(int64_t T, int64_t L, int64_t R) {
 
 extern "C" size_t b200_lora_plan_bytes(int64_t T, int L) {
   if (T < 0 || L <= 0) return 0;
-  return static_cast<size_t>(16 + 16 * b200::max_tiles(T, L) + 4 * T);
+  return static_cast<size_t>(16 + 16 * b200::plan_tiles(T, L) + 4 * T);
 }
 
 extern "C" int b200_lora_plan(const int32_t* token_adapters, int64_t T, const int32_t* ranks, int L, void* plan,

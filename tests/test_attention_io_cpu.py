@@ -237,3 +237,23 @@ def test_c_abi_codes():
                                   one, old, None)
     assert ex(T=0) == 0 and ex(sizes=(64, 36)) == -3 and ex(old=88) == -4 and ex(bld=88) == -4 and ex(hld=24) == -4
     assert ex(h=None) == -1 and ex(h=P(8)) == -5 and ex(sizes=(8,) * 9) == -9
+
+
+@pytest.mark.parametrize("L", [1, 3, 10, 40, 1000])
+def test_plans_of_different_batches_differ_in_size(L):
+    """By its size a plan is told from one for another number of tokens, whose permutation lies elsewhere in it."""
+    from sglang_b200 import _lib
+    sizes = [_lib.lib().b200_lora_plan_bytes(T, L) for T in range(30000)]
+    assert all(a < b for a, b in zip(sizes, sizes[1:]))
+
+
+def test_lora_refuses_the_batch_of_fewer_tokens():
+    """212 tokens of 3 adapters in tiles of 16 and 256 in tiles of 128."""
+    from sglang_b200.layers.lora import lora_expand, lora_shrink
+    x, out = torch.zeros(256, 64, dtype=BF), torch.zeros(256, 96, dtype=BF)
+    with pytest.raises(RuntimeError, match="another number of tokens"):
+        _lora_call(base_output=out, x=x, batch=_Batch(212, 3))
+    with pytest.raises(RuntimeError, match="another number of tokens"):
+        lora_shrink(x, torch.zeros(3, 32, 64, dtype=BF), _Batch(212, 3), num_slices=2)
+    with pytest.raises(RuntimeError, match="another number of tokens"):
+        lora_expand(x[:, :32].contiguous(), torch.zeros(3, 96, 16, dtype=BF), _Batch(212, 3), output_sizes=[64, 32])
