@@ -41,7 +41,9 @@ class LoRABatch:
 
     def update(self) -> None:
         """Groups again after token_adapters or lora_ranks have been written in place (the next replay of a captured graph, of
-        which this call may be a part)."""
+        which this call may be a part).  Their lengths stay."""
+        if self.lora_ranks.shape[0] != self.num_adapters:
+            raise RuntimeError(f"the batch was made for {self.num_adapters} adapters, not {self.lora_ranks.shape[0]}")
         _lib.host().lora_plan(self.token_adapters, self.lora_ranks, self.plan)
 
 

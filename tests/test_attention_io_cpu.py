@@ -257,3 +257,27 @@ def test_lora_refuses_the_batch_of_fewer_tokens():
         lora_shrink(x, torch.zeros(3, 32, 64, dtype=BF), _Batch(212, 3), num_slices=2)
     with pytest.raises(RuntimeError, match="another number of tokens"):
         lora_expand(x[:, :32].contiguous(), torch.zeros(3, 96, 16, dtype=BF), _Batch(212, 3), output_sizes=[64, 32])
+
+
+def test_update_refuses_other_numbers_of_adapters_or_tokens(monkeypatch):
+    """Two adapters and five for three tokens have plans of one size."""
+    from types import SimpleNamespace
+
+    from sglang_b200 import _lib
+    from sglang_b200.layers import lora
+    host, planned = _lib.host(), []
+
+    def plan(ids, ranks, plan):
+        planned.append(ranks.shape[0])
+        return torch.zeros(_lib.lib().b200_lora_plan_bytes(ids.shape[0], ranks.shape[0]), dtype=torch.uint8)
+    with monkeypatch.context() as m:
+        m.setattr(lora._lib, "host", lambda: SimpleNamespace(lora_plan=plan))
+        batch = lora.LoRABatch(torch.zeros(3, dtype=torch.int32), torch.ones(2, dtype=torch.int32), torch.ones(2))
+        batch.lora_ranks = torch.ones(5, dtype=torch.int32)
+        with pytest.raises(RuntimeError, match="2 adapters, not 5"):
+            batch.update()
+        assert planned == [2]
+    assert _lib.host() is host
+    batch.lora_ranks, batch.token_adapters = torch.ones(2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="plan must have shape"):
+        batch.update()
