@@ -35,8 +35,11 @@ class LoRABatch:
     @classmethod
     def from_segments(cls, weight_indices: torch.Tensor, seg_lens: torch.Tensor, num_tokens: int, lora_ranks: torch.Tensor,
                       scalings: torch.Tensor) -> "LoRABatch":
-        """Request i, with adapter weight_indices[i], holds the next seg_lens[i] tokens; num_tokens is their sum."""
-        ids = torch.repeat_interleave(weight_indices.to(torch.int32), seg_lens, output_size=num_tokens)
+        """Request i, with adapter weight_indices[i], holds the next seg_lens[i] tokens of num_tokens; tokens behind the last
+        request (a padded batch) have no adapter."""
+        # a search instead of repeat_interleave, which needs num_tokens to be the exact sum and asserts it on the device
+        request = torch.searchsorted(seg_lens.cumsum(0), torch.arange(num_tokens, device=seg_lens.device), right=True)
+        ids = torch.nn.functional.pad(weight_indices.to(torch.int32), (0, 1), value=-1)[request]
         return cls(ids, lora_ranks, scalings)
 
     def update(self) -> None:

@@ -281,3 +281,19 @@ def test_update_refuses_other_numbers_of_adapters_or_tokens(monkeypatch):
     batch.lora_ranks, batch.token_adapters = torch.ones(2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="plan must have shape"):
         batch.update()
+
+
+@pytest.mark.parametrize("num_tokens", [0, 1, 5, 6, 11])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_tokens_behind_the_segments_have_no_adapter(monkeypatch, num_tokens, index):
+    """A padded batch has more tokens than its requests, one cut short has fewer."""
+    from types import SimpleNamespace
+
+    from sglang_b200.layers import lora
+    monkeypatch.setattr(lora._lib, "host", lambda: SimpleNamespace(lora_plan=lambda *a: None))
+    ranks, scal = torch.ones(5, dtype=torch.int32), torch.ones(5)
+    batch = lora.LoRABatch.from_segments(torch.tensor([4, -1, 0, 2], dtype=index), torch.tensor([2, 1, 0, 3], dtype=index), num_tokens, ranks, scal)
+    want = torch.tensor(([4, 4, -1, 2, 2, 2] + [-1] * 5)[:num_tokens], dtype=torch.int32)
+    assert batch.token_adapters.dtype == torch.int32 and torch.equal(batch.token_adapters, want)
+    none = torch.zeros(0, dtype=index)
+    assert torch.equal(lora.LoRABatch.from_segments(none, none, num_tokens, ranks, scal).token_adapters, torch.full((num_tokens,), -1, dtype=torch.int32))
