@@ -609,11 +609,12 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const T*
   const T* h0[2] = {h + static_cast<int64_t>(h_row[0]) * h_ld + 8 * c, h + static_cast<int64_t>(h_row[1]) * h_ld + 8 * c};
   uint4 hv[2];
   auto fetch_h = [&](const At& p) {
-    const bool in = rank - 32 * p.j - 8 * c > 0;
+    const int keep = rank - 32 * p.j - 8 * c;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       hv[i] = make_uint4(0, 0, 0, 0);
-      if (in && g + 8 * i < rows) hv[i] = *reinterpret_cast<const uint4*>(h0[i] + p.s * R + 32 * p.j);
+      if (keep > 0 && g + 8 * i < rows) hv[i] = *reinterpret_cast<const uint4*>(h0[i] + p.s * R + 32 * p.j);
+      if (keep < 8) hv[i] = first_of(hv[i], keep);           // zeros of B alone would not do: what is behind the rank may be NaN
     }
   };
   fetch_weights(in_flight);
@@ -926,6 +927,14 @@ __global__ void __launch_bounds__(kWalkThreads) lora_expand_tiles_kernel(const T
     sa::cp_async_commit();
   }
   sa::cp_async_wait<kWalkStages - 1>();                      // h
+  if (rank % 8 != 0) {                                       // what is behind the rank may be NaN; each thread looks after what it copied
+    for (int e = threadIdx.x; e < kLargeRows * RJ * 4; e += kWalkThreads) {
+      if (e % (RJ * 4) != rank / 8) continue;
+      const uint32_t at = h_at(e / (RJ * 4), rank / 8);
+      const uint4 v = first_of(sa::ld_v4(at), rank % 8);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NT; ++i)

@@ -183,6 +183,31 @@ def test_a_token_s_result_depends_on_its_own_row_only():
         assert same_bits(one(x, order), clean[order.cuda()])
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("T,R,L,ranks", [(3, 16, 2, [5, 12]), (40, 64, 4, [64, 33, 1, 31]), (300, 32, 3, [4, 17, 32]), (700, 64, 2, [3, 63]),
+                                         (600, 128, 2, [97, 127]), (513, 256, 2, [250, 129])])
+def test_expand_uses_nothing_behind_a_rank(T, R, L, ranks, dtype):
+    """h from elsewhere, with infinities and NaN behind every adapter's rank and in the rows of tokens without one."""
+    from sglang_b200.layers.lora import LoRABatch, lora_expand
+    sizes = [72, 24]
+    x, base, A, B, ids, ranks, scal = _case(T, 64, sizes, R, L, dtype, T + R, ranks=ranks)
+    h = torch.randn(T, 2, R, generator=torch.Generator().manual_seed(R)).to(dtype)
+    out = base.double().clone()
+    tol = torch.zeros_like(out)
+    step, e = 2.0 ** -22, torch.finfo(dtype).eps / 2
+    for a in range(L):
+        rows, r = (ids == a).nonzero().flatten(), int(ranks[a])
+        h[rows, :, r:] = float("nan") if a % 2 else float("inf")
+        for s, (at, n) in enumerate(((0, 72), (72, 24))):
+            hh, bb = h[rows, s, :r].double(), B[a, at:at + n, :r].double()
+            out[rows, at:at + n] += float(scal[a]) * hh @ bb.T
+            # fp32 sums of products of 16-bit numbers, as at the top of this file; the result is rounded once
+            tol[rows, at:at + n] = abs(float(scal[a])) * (R / 16 + 4) * step * hh.abs() @ bb.abs().T * (1 + e)
+    h[ids < 0] = float("nan")
+    got = lora_expand(h.view(T, 2 * R).cuda(), B.cuda(), LoRABatch(ids.cuda(), ranks.cuda(), scal.cuda()), base.cuda(), sizes)
+    _close(got, out, tol + e * out.abs() + 2.0 ** -23 * out.abs() + torch.finfo(dtype).smallest_normal * e)
+
+
 def test_segments_and_update():
     from sglang_b200.layers.lora import LoRABatch, apply_lora
     T, sizes = 90, [64]
