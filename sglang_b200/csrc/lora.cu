@@ -1193,8 +1193,11 @@ extern "C" int b200_lora_plan(const int32_t* token_adapters, int64_t T, const in
   B200_CUDA_TRY(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture));
   if (capture == cudaStreamCaptureStatusNone && tile_rows(T, L) == kLargeRows) gemm_sticky_status();
   const PlanView v = view_plan(plan, T, L);
-  const size_t smem = sizeof(int) * ((kPlanWarps + 1) * (L + 1) + 2 * (L + 2));
-  if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  auto smem_of = [](int n) { return static_cast<int>(sizeof(int)) * ((kPlanWarps + 1) * (n + 1) + 2 * (n + 2)); };
+  const int smem = smem_of(L);
+  // Always the most that there can be: the limit is the kernel's, for all threads, and a smaller one of another thread could come
+  // between this call and the launch.
+  if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(kMaxAdapters)));
   B200_CUDA_TRY(launch_pdl(lora_plan_kernel, dim3(1), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), token_adapters, T,
                            ranks, L, tile_rows(T, L), const_cast<int*>(v.count), const_cast<int4*>(v.tiles), const_cast<int*>(v.perm)));
   return B200_OK;

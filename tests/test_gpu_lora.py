@@ -146,6 +146,31 @@ def test_several_streams_at_once():
             assert same_bits(a, o)
 
 
+def test_plans_of_several_threads():
+    """Many and few adapters planned by two threads at once: the plan's kernel needs 143 KB of shared memory or 54 KB."""
+    import threading
+
+    from sglang_b200.layers.lora import LoRABatch
+    failed = []
+
+    def work(L):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ids = torch.zeros(8, dtype=torch.int32, device="cuda")
+            batch = LoRABatch(ids, torch.ones(L, dtype=torch.int32, device="cuda"), torch.ones(L, device="cuda"))
+            try:
+                for _ in range(20000):
+                    batch.update()
+            except RuntimeError as e:
+                failed.append((L, str(e)))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(L,)) for L in (1024, 400)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
 def test_strided_views_and_odd_ids():
     """x and base as columns of wider tensors; ids outside the buffers and ranks of 0 or below count as no adapter; a rank
     above R counts as R."""
