@@ -698,7 +698,8 @@ HOST_FN(head_rows) {
       const b200_heads qh = q.defined() ? heads_of(q) : b200_heads{}, kh = heads_of(k), vh = v.defined() ? heads_of(v) : b200_heads{};
       const b200_heads qoh = qo.defined() ? heads_of(qo) : b200_heads{}, koh = ko.defined() ? heads_of(ko) : b200_heads{};
       const void* pp = pos.defined() ? pos.data_ptr() : nullptr;
-      const float* cp = cs.defined() ? static_cast<const float*>(cs.data_ptr()) : nullptr;
+      // a table without rows has no address, but is not no table: any will do, as no position is read from it
+      const float* cp = cs.defined() ? static_cast<const float*>(rows > 0 ? cs.data_ptr() : (Hkv > 0 ? k : q).data_ptr()) : nullptr;
       const int pos64 = pos.defined() && pos.scalar_type() == at::kLong;
       const void *qwp = qw.defined() ? qw.data_ptr() : nullptr, *kwp = kw.defined() ? kw.data_ptr() : nullptr;
       const int dt = dt_of(type);

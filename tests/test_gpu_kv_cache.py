@@ -112,6 +112,25 @@ def test_norm_rope_padding_and_positions_outside_the_table():
         assert (out[[1, 4]] == 9.0).all() and out[[3, 5]].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_a_table_without_rows_lacks_every_position(dtype):
+    from sglang_b200.layers.quantization.kv_cache import load_kv_fp8, qk_norm_rope_store_kv_fp8
+    from sglang_b200.layers.rotary_embedding import qk_norm_rope
+    qkv, (qw, kw) = _inputs(3, 4, 2, 64, dtype, 3)
+    q, k, v = _split(qkv.cuda(), 4, 2)
+    pos, table = torch.tensor([0, -1, 7]).cuda(), torch.empty(0, 64, device="cuda")
+    for w in ((qw.cuda(), kw.cuda()), (None, None)):
+        for neox in (True, False):
+            qo, ko = torch.full_like(q, 9.0), torch.full_like(k, 9.0)
+            qk_norm_rope(q, k, pos, table, *w, is_neox=neox, q_out=qo, k_out=ko)
+            for out in (qo, ko):
+                assert out[[0, 2]].isnan().all() and (out[1] == 9.0).all()
+    cache = _cache(1, 4, 2, 64)
+    out = qk_norm_rope_store_kv_fp8(q, k, v, pos, table, *cache, torch.arange(3).cuda())
+    kl, vl = load_kv_fp8(*cache, torch.tensor([[0]]).int().cuda(), torch.tensor([0, 3]).int().cuda(), 3)
+    assert out[[0, 2]].isnan().all() and kl[[0, 2]].isnan().all() and not vl.isnan().any()
+
+
 @pytest.mark.parametrize("queries,weights", [(2, True), (2, False), (0, True), (0, False)])
 def test_padding_without_a_rotation(queries, weights):
     """A negative position marks a token as padding whether or not there is a table."""
