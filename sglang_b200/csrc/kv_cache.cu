@@ -723,7 +723,7 @@ extern "C" int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_
   int rc = check_cache(cache);
   if (rc != B200_OK) return rc;
   if (tokens == 0 || batch == 0 || num_kv_heads == 0) return B200_OK;
-  if (!page_table || !indptr || !k_out || !v_out) return B200_ERR_NULL_PTR;
+  if ((!page_table && page_table_cols > 0) || !indptr || !k_out || !v_out) return B200_ERR_NULL_PTR;
   if (page_table_stride < 0) return B200_ERR_BAD_STRIDE;
   KvLoadParams p = {};
   const void *ko = nullptr, *vo = nullptr;

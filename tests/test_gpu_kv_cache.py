@@ -355,6 +355,15 @@ def test_load_of_missing_pages_reads_as_nan():
         assert t.cpu()[bad].isnan().all() and not t.cpu()[~bad].isnan().any()
 
 
+def test_load_through_a_table_without_columns():
+    """No page of any sequence is in it: the rows of the sequences are NaN, those behind them stay."""
+    from sglang_b200.layers.quantization.kv_cache import load_kv_fp8
+    cache = _cache(2, 4, 2, 64)
+    out = torch.full((5, 2, 64), 3.0, dtype=BF, device="cuda")
+    k, v = load_kv_fp8(*cache, torch.empty(2, 0, dtype=torch.int32, device="cuda"), torch.tensor([0, 1, 3]).int().cuda(), 5, k_out=out)
+    assert k[:3].isnan().all() and v[:3].isnan().all() and (k[3:] == 3.0).all()
+
+
 def test_permuted_and_sliced_caches():
     """[2, num_pages, num_kv_heads, page_size, head_dim] pools, passed as views."""
     from sglang_b200.layers.quantization.kv_cache import load_kv_fp8, store_kv_fp8
