@@ -22,6 +22,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <stdexcept>
 #include <string>
@@ -564,6 +565,76 @@ at::Device one_device(std::initializer_list<const Tensor*> all) {
   }
   return dev;
 }
+// The bytes of a tensor: runs of `width` neighbouring ones, `count[d]` of them `step[d]` apart in each of n dimensions, the largest
+// step first; `span[d]` is how far those of the dimensions from d on reach.  What is broadcast counts once.
+struct Bytes {
+  const char* at;
+  int n = 0;
+  int64_t count[8], step[8], span[9];
+};
+Bytes bytes_of(const Tensor& t) {
+  Bytes b;
+  b.at = static_cast<const char*>(t.const_data_ptr());
+  int64_t width = static_cast<int64_t>(t.element_size());
+  for (int d = 0; d < t.dim(); ++d) {
+    if (t.size(d) <= 1 || t.stride(d) == 0) continue;
+    const int64_t step = t.stride(d) * static_cast<int64_t>(t.element_size());
+    int i = b.n++;
+    for (; i > 0 && b.step[i - 1] < step; --i) b.step[i] = b.step[i - 1], b.count[i] = b.count[i - 1];
+    b.step[i] = step, b.count[i] = t.size(d);
+  }
+  while (b.n > 0 && b.step[b.n - 1] == width) width *= b.count[--b.n];
+  b.span[b.n] = width;
+  for (int d = b.n - 1; d >= 0; --d) b.span[d] = b.span[d + 1] + (b.count[d] - 1) * b.step[d];
+  return b;
+}
+// Whether the bytes of a from dimension i on and those of b from j on meet, b's beginning `off` bytes behind a's.  Two dimensions of one
+// step are walked through together: only how many steps the two are apart matters.  Exact, unless there are more than 64
+// places to look at in some dimension, which count as meeting.
+bool meet(const Bytes& a, int i, const Bytes& b, int j, int64_t off) {
+  if (off >= a.span[i] || -off >= b.span[j]) return false;
+  if (i == a.n && j == b.n) return true;
+  const bool in_a = i < a.n && (j == b.n || a.step[i] >= b.step[j]), in_b = j < b.n && (i == a.n || b.step[j] >= a.step[i]);
+  const int64_t step = in_a ? a.step[i] : b.step[j];
+  const int ni = i + in_a, nj = j + in_b;
+  // by m steps a is ahead: -b.span[nj] < off - m step < a.span[ni]
+  auto floor_div = [](int64_t x, int64_t y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };
+  int64_t from = floor_div(off - a.span[ni], step) + 1, to = -floor_div(-(off + b.span[nj]), step) - 1;
+  from = std::max(from, in_b ? 1 - b.count[j] : 0);
+  to = std::min(to, in_a ? a.count[i] - 1 : 0);
+  if (to - from >= 64) return true;
+  for (int64_t m = from; m <= to; ++m)
+    if (meet(a, ni, b, nj, off - m * step)) return true;
+  return false;
+}
+bool share_memory(const Tensor& t, const Tensor& u) {
+  if (!t.defined() || !u.defined() || t.numel() == 0 || u.numel() == 0) return false;
+  const Bytes a = bytes_of(t), b = bytes_of(u);
+  return meet(a, 0, b, 0, b.at - a.at);
+}
+bool same_view(const Tensor& t, const Tensor& u) {
+  if (!t.defined() || !u.defined() || t.const_data_ptr() != u.const_data_ptr() || t.sizes() != u.sizes()) return false;
+  for (int d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) != u.stride(d)) return false;
+  return true;
+}
+// What a call writes must lie in places of its own: not overlap itself, nor, unless it is `in_place`, anything else that the call has.
+struct Held {
+  Held(const Tensor& t, const char* name) : t(t), name(name), any(t.defined() && t.numel() > 0) {
+    if (any) b = bytes_of(t);
+  }
+  const Tensor& t;
+  const char* name;
+  bool any;
+  Bytes b;
+};
+void need_own_memory(const Held& out, const Held* in_place, at::ArrayRef<Held> all) {
+  if (!out.any) return;
+  for (int d = 0; d < out.b.n; ++d) NEED(out.b.step[d] >= out.b.span[d + 1], std::string(out.name) + " must not overlap itself");
+  for (const Held& o : all)
+    NEED(!o.any || &o == &out || !meet(out.b, 0, o.b, 0, o.b.at - out.b.at) || (&o == in_place && same_view(out.t, o.t)),
+         std::string(out.name) + " must share no memory with " + o.name + (&o == in_place ? " or be it" : ""));
+}
 b200_heads heads_of(const Tensor& t) { return {t.data_ptr(), stride_of(t, 0), stride_of(t, 1)}; }
 
 struct CacheArgs {
@@ -687,6 +758,16 @@ HOST_FN(head_rows) {
     for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{cache.k, "k_cache"}, {cache.v, "v_cache"}, {cache.ks, "k_scale"}, {cache.vs, "v_scale"}})
       need_writable(t, what);
   }
+  if (store || qo.defined() || ko.defined()) {
+    const Held all[] = {{q, "q"}, {k, "k"}, {qo, "q_out"}, {ko, "k_out"}, {cache.k, "k_cache"}, {cache.v, "v_cache"}, {cache.ks, "k_scale"},
+                        {cache.vs, "v_scale"}, {v, "v"}, {pos, "positions"}, {cs, "cos_sin_cache"}, {qw, "q_weight"}, {kw, "k_weight"},
+                        {slots, "slots"}};
+    // keys and values that are the same data may go to one cache: both write the same bytes
+    const bool one = store && !pos.defined() && !kw.defined() && same_view(k, v);
+    need_own_memory(all[2], &all[0], all);
+    need_own_memory(all[3], &all[1], all);
+    for (int i = 4; i < 8; ++i) need_own_memory(all[i], one ? &all[i ^ 1] : nullptr, all);
+  }
   const at::Device dev = one_device({&k, &q, &v, &pos, &cs, &qw, &kw, &qo, &ko, &cache.k, &cache.v, &cache.ks, &cache.vs, &slots});
   int rc = 0;
   {
@@ -752,6 +833,11 @@ HOST_FN(load_kv) {
     NEED(t.scalar_type() == type, std::string(what) + " must be of out_dtype");
     need_writable(t, what);
   }
+  if (ko.defined() || vo.defined()) {
+    const Held all[] = {{ko, "k_out"}, {vo, "v_out"}, {cache.k, "k_cache"}, {cache.v, "v_cache"}, {cache.ks, "k_scale"}, {cache.vs, "v_scale"},
+                        {table, "page_table"}, {indptr, "kv_indptr"}, {starts, "kv_start"}};
+    for (int i = 0; i < 2; ++i) need_own_memory(all[i], nullptr, all);
+  }
   const at::Device dev = one_device({&cache.k, &cache.v, &cache.ks, &cache.vs, &table, &indptr, &starts, &ko, &vo});
   int rc;
   {
@@ -801,17 +887,6 @@ HOST_FN(lora_plan) {
   return THPVariable_Wrap(std::move(plan));
 }
 HOST_END
-
-// Whether rows of t and u [T, width] share memory.  Two ranges of columns of one buffer do not, although they lie between each other.
-bool share_rows(const Tensor& t, const Tensor& u) {
-  if (!t.defined() || !u.defined() || t.numel() == 0 || u.numel() == 0) return false;
-  const int64_t size = t.element_size(), wt = t.size(1), wu = u.size(1), st = stride_of(t, 0), su = stride_of(u, 0);
-  const char *pt = static_cast<const char*>(t.data_ptr()), *pu = static_cast<const char*>(u.data_ptr());
-  if (pt + (st * (t.size(0) - 1) + wt) * size <= pu || pu + (su * (u.size(0) - 1) + wu) * size <= pt) return false;
-  if (st != su || wt > st || wu > st) return true;
-  const int64_t d = ((pu - pt) % (st * size) + st * size) % (st * size);       // where u's columns begin, seen from t's
-  return d < wt * size || (st * size - d) < wu * size;
-}
 
 // lora(base | None, x [T, K] | None, h [T, S R] | None, lora_a [L, S R, K] | None, lora_b [L, N, R] | None, plan, num_adapters,
 //      scalings, sizes (a tuple of S) | None, num_slices, out | None) -> out [T, N]: shrink and expand; without lora_b only the
@@ -889,8 +964,8 @@ HOST_FN(lora) {
   }
   if (out.defined() && out.numel() > 0) {
     const bool same = base.defined() && base.data_ptr() == out.data_ptr() && stride_of(base, 0) == stride_of(out, 0);
-    NEED(same || !share_rows(out, base), "out must be base_output itself or share no memory with it");
-    NEED(!share_rows(out, x) && !share_rows(out, h), "out must share no memory with x or h");
+    NEED(same || !share_memory(out, base), "out must be base_output itself or share no memory with it");
+    NEED(!share_memory(out, x) && !share_memory(out, h), "out must share no memory with x or h");
   }
   const at::Device dev = one_device({&plan, &base, &x, &h, &A, &B, &scalings, &out});
   int rc = 0;

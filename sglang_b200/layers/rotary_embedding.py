@@ -19,7 +19,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Ten
                  is_neox: bool = True, q_out: Optional[torch.Tensor] = None,
                  k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """q [T, num_q_heads, head_dim] and k [T, num_kv_heads, head_dim] (bf16 / fp16, e.g. views of a packed qkv output) ->
-    (q_out, k_out), new contiguous tensors unless given; q_out may be q itself and k_out k itself, but nothing else may overlap.
+    (q_out, k_out), new contiguous tensors unless given; q_out may be q itself and k_out k itself; other overlaps are refused.
 
     Every head is normalised with its weight [head_dim] (None: not), then its first cos_sin_cache.shape[1] elements are rotated
     by row positions[t] of cos_sin_cache [max_position, rotary_dim] (fp32, cosines | sines; None: no rotation): pairs

@@ -297,3 +297,87 @@ def test_tokens_behind_the_segments_have_no_adapter(monkeypatch, num_tokens, ind
     assert batch.token_adapters.dtype == torch.int32 and torch.equal(batch.token_adapters, want)
     none = torch.zeros(0, dtype=index)
     assert torch.equal(lora.LoRABatch.from_segments(none, none, num_tokens, ranks, scal).token_adapters, torch.full((num_tokens,), -1, dtype=torch.int32))
+
+
+def test_outputs_that_are_read_or_written_elsewhere_are_refused():
+    """The heads of one qkv output beside one another are fine, also in place (such calls get as far as the question of the device)."""
+    qkv, more = torch.zeros(3, 8, 64, dtype=BF), torch.zeros(3, 8, 64, dtype=BF)
+    q, k = qkv[:, :4], qkv[:, 4:6]
+    flat = torch.zeros(2000, dtype=BF)
+    for change, message in (
+            (dict(q=q, k=k), "CUDA"), (dict(q=q, k=k, q_out=q, k_out=k), "CUDA"), (dict(q=q, k=k, q_out=more[:, 2:6], k_out=more[:, :2]), "CUDA"),
+            (dict(q=q, k=k, q_out=more[:, :4], k_out=more[:, 3:5]), "q_out must share no memory with k_out"),
+            (dict(q=q, k=k, q_out=qkv[:, 2:6]), "q_out must share no memory with q or be it"),
+            (dict(q=q, k=k, q_out=qkv[:, 4:]), "q_out must share no memory with k"), (dict(q=q, k=k, k_out=q[:, :2]), "k_out must share no memory with q"),
+            (dict(q=q, k=k, q_out=q[[0]].expand(3, 4, 64)), "expanded"),
+            (dict(q=q, k=k, q_out=flat.as_strided((3, 4, 64), (256, 48, 1))), "q_out must not overlap itself"),
+            (dict(q=q, k=k, q_out=flat.as_strided((3, 4, 64), (128, 64, 1))), "q_out must not overlap itself"),
+            (dict(q=q, k=k, q_out=flat.as_strided((3, 4, 64), (64, 192, 1))), "CUDA"),
+            # heads and tokens in turn: every other run of 64
+            (dict(q=q, k=flat.as_strided((3, 2, 64), (512, 128, 1)), k_out=flat.as_strided((3, 2, 64), (512, 128, 1), 64)), "CUDA"),
+            (dict(q=q, k=flat.as_strided((3, 2, 64), (512, 128, 1)), k_out=flat.as_strided((3, 2, 64), (512, 128, 1), 56)), "k_out must share no memory with k"),
+            # rows of another length, and tokens of one tensor in the gaps of the other
+            (dict(q=q, k=flat.as_strided((3, 2, 64), (512, 128, 1)), k_out=flat.as_strided((3, 2, 64), (640, 64, 1), 256)), "CUDA"),
+            (dict(q=q, k=flat.as_strided((3, 2, 64), (512, 128, 1)), k_out=flat.as_strided((3, 2, 64), (640, 64, 1), 192)), "CUDA"),
+            (dict(q=q, k=flat.as_strided((3, 2, 64), (512, 128, 1)), k_out=flat.as_strided((3, 2, 64), (640, 64, 1), 128)), "k_out must share"),
+            (dict(positions=more.view(torch.int64).view(-1)[:3], q=more[:, :4].clone(), k_out=more[:, :2]), "k_out must share no memory with positions"),
+            (dict(q_weight=more[0, 1], k_out=more[:, :2]), "k_out must share no memory with q_weight")):
+        with pytest.raises(RuntimeError, match=message):
+            _heads_call(**change)
+
+
+def test_caches_that_overlap_are_refused():
+    """A pool that holds keys, values and scales in turn is fine."""
+    k, v = torch.zeros(3, 2, 64, dtype=BF), torch.zeros(3, 2, 64, dtype=BF)
+    pool, scales = torch.zeros(5, 2, 4, 2, 64).to(F8), torch.zeros(5, 4, 2, 2)
+    page = torch.zeros(5, 2 * 4 * 2 * 68, dtype=torch.uint8)          # of keys, values and their scales, for each page
+    codes = [page[:, i * 512:(i + 1) * 512].view(F8).view(5, 4, 2, 64) for i in range(2)]
+    fp32 = [page[:, 1024 + i * 32:1056 + i * 32].view(torch.float32).view(5, 4, 2) for i in range(2)]
+    both = dict(k_cache=pool[:, 0], v_cache=pool[:, 1], k_scale=scales[..., 0], v_scale=scales[..., 1])
+    one = dict(both, v_cache=pool[:, 0], v_scale=scales[..., 0])
+    for change, message in (
+            (both, "CUDA"), (dict(k_cache=codes[0], v_cache=codes[1], k_scale=fp32[0], v_scale=fp32[1]), "CUDA"), (dict(one, v=k, k=k), "CUDA"),
+            (one, "k_cache must share no memory with v_cache"),
+            (dict(both, v_cache=pool.view(10, 4, 2, 64)[1:6]), "k_cache must share no memory with v_cache"),
+            (dict(both, v_scale=scales[..., 0]), "k_scale must share no memory with v_scale"),
+            (dict(both, k_scale=page[:, :32].view(torch.float32).view(5, 4, 2), k_cache=codes[0]), "k_cache must share no memory with k_scale"),
+            (dict(both, k_cache=pool.view(-1).as_strided((5, 4, 2, 64), (512, 64, 64, 1))), "k_cache must not overlap itself"),
+            (dict(both, slots=scales.view(torch.int32).view(-1)[:3]), "k_scale must share no memory with slots"),
+            (dict(both, k=pool.view(-1).view(BF)[:384].view(3, 2, 64)), "k_cache must share no memory with k")):
+        with pytest.raises(RuntimeError, match=message):
+            _store_call(**dict(dict(k=k, v=v), **change))
+    from sglang_b200.layers.quantization.kv_cache import qk_norm_rope_store_kv_fp8
+    args = (k, k, k, torch.zeros(3, dtype=torch.int64), None)
+    with pytest.raises(RuntimeError, match="k_cache must share no memory with v_cache"):      # the keys of a padded token are left out; values, too
+        qk_norm_rope_store_kv_fp8(*args, *one.values(), torch.zeros(3, dtype=torch.int32))
+    out = torch.zeros(7, 4, 64, dtype=BF)
+    for change, message in ((dict(k_out=out[:, :2], v_out=out[:, 2:]), "CUDA"), (dict(k_out=out[:, :2], v_out=out[:, 1:3]), "k_out must share no memory with v_out"),
+                            (dict(v_out=out.view(-1)[:1280].as_strided((7, 2, 64), (128, 48, 1))), "v_out must not overlap itself"),
+                            (dict(k_out=torch.zeros(7, 2, 64, dtype=BF), kv_indptr=out.view(torch.int32).view(-1)[:3], v_out=out[:, :2]), "kv_indptr")):
+        with pytest.raises(RuntimeError, match=message):
+            _load_call(**change)
+
+
+def test_memory_is_compared_byte_for_byte():
+    """Random views of one buffer as output and input of a call: refused exactly when they share an element."""
+    import random
+    rng, buf = random.Random(0), torch.zeros(4000, dtype=BF)
+    seen = [0, 0]
+    for _ in range(3000):
+        T, H = rng.randint(1, 4), rng.randint(1, 3)
+        strides = [(rng.choice([32, 64, 96, 128, 256]), rng.choice([16, 32, 48, 64, 512])) for _ in range(2)]
+        at = [8 * rng.randint(0, 60) for _ in range(2)]
+        k, out = (buf.as_strided((T, H, 16), (*s, 1), o) for s, o in zip(strides, at))
+        places = [torch.arange(4000).as_strided((T, H, 16), (*s, 1), o).flatten() for s, o in zip(strides, at)]
+        if len(places[1].unique()) < places[1].numel():
+            continue
+        meets = bool(torch.isin(places[0], places[1]).any())
+        with pytest.raises(RuntimeError) as e:
+            _heads_call(q=torch.zeros(T, 1, 16, dtype=BF), k=k, k_out=out, positions=torch.zeros(T, dtype=torch.int64), cos_sin_cache=None,
+                        q_weight=None, k_weight=None)
+        if "overlap itself" in str(e.value):       # dimensions that interlock
+            continue
+        in_place = at[0] == at[1] and (T == 1 or strides[0][0] == strides[1][0]) and (H == 1 or strides[0][1] == strides[1][1])
+        seen[meets] += 1
+        assert ("CUDA" in str(e.value)) == (not meets or in_place), (T, H, strides, at, str(e.value))
+    assert min(seen) > 300
