@@ -609,12 +609,11 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const T*
   const T* h0[2] = {h + static_cast<int64_t>(h_row[0]) * h_ld + 8 * c, h + static_cast<int64_t>(h_row[1]) * h_ld + 8 * c};
   uint4 hv[2];
   auto fetch_h = [&](const At& p) {
-    const int keep = rank - 32 * p.j - 8 * c;
+    const bool in = rank - 32 * p.j - 8 * c > 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       hv[i] = make_uint4(0, 0, 0, 0);
-      if (keep > 0 && g + 8 * i < rows) hv[i] = *reinterpret_cast<const uint4*>(h0[i] + p.s * R + 32 * p.j);
-      if (keep < 8) hv[i] = first_of(hv[i], keep);           // zeros of B alone would not do: what is behind the rank may be NaN
+      if (in && g + 8 * i < rows) hv[i] = *reinterpret_cast<const uint4*>(h0[i] + p.s * R + 32 * p.j);
     }
   };
   fetch_weights(in_flight);
@@ -649,6 +648,8 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const T*
     }
     if (!none) {
       const int keep = rank - 32 * j - 8 * c;
+      // Zeros of B alone would not do: h may be NaN behind the rank.  Here and not behind its load, which would be waited for.
+      if (keep > 0 && keep < 8) hv[0] = first_of(hv[0], keep), hv[1] = first_of(hv[1], keep);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint4 lo = sa::ld_v4(from + 2 * i * 512), hi = sa::ld_v4(from + (2 * i + 1) * 512);
