@@ -741,9 +741,13 @@ extern "C" int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_
   p.wide = ((p.ko_st | p.ko_sh | p.vo_st | p.vo_sh) % 16 == 0) && ((reinterpret_cast<uintptr_t>(ko) | reinterpret_cast<uintptr_t>(vo)) & 31u) == 0;
   const int sms = sm_count();
   if (sms <= 0) return B200_ERR_CUDA;
-  // Rows of a block: 32 where that gives every SM its eight blocks (131001 x 8 x 128: 137 us, with 16 rows 148, with 8 155), else 8
-  // (401 x 8 x 128: 3.1 us, with 32 rows 5.6).
-  const int rows = (tokens + 31) / 32 * 2 >= 8LL * sms ? 32 : 8;
+  // Rows of a block: 32 from 18944 tokens on (148 SMs; eight blocks for every SM, of which six are resident), else 8; with rows of
+  // fewer than 64 vectors, of which eight leave threads idle, from so many fewer tokens on.  8 / 32 rows (us, heads of 128): 8 heads
+  // 401 tokens 3.2 / 5.9, 12000 17.0 / 17.4, 16000 21.6 / 22.2, 18000 24.0 / 23.8, 24000 30.8 / 29.1, 80000 93 / 83; 4 heads 8000
+  // 8.6 / 9.2, 10000 10.5 / 9.8, 20000 18.8 / 14.5; 2 heads 3000 3.2 / 3.6, 5000 4.7 / 4.1, 20000 13.5 / 8.6; one head 2000
+  // 3.0 / 2.7, 20000 11.1 / 6.0; 16 heads 16000 37 / 42, 24000 53 / 54.
+  const int64_t vecs = static_cast<int64_t>(num_kv_heads) * (head_dim / 16);
+  const int rows = tokens >= 2LL * sms * (vecs < 64 ? vecs : 64) ? 32 : 8;
   const int64_t blocks = (tokens + rows - 1) / rows;
   if (blocks > 0x7fffffffLL) return B200_ERR_TOO_LARGE;
   const dim3 grid(static_cast<unsigned>(blocks), 2);

@@ -342,6 +342,20 @@ def test_load(lens, page, H, D, dtype):
             assert same_bits(got[:n], want)
 
 
+@pytest.mark.parametrize("n,H,D", [(1183, 1, 64), (1184, 1, 64), (2367, 1, 128), (2369, 1, 128), (4735, 2, 128), (4737, 2, 128), (9473, 4, 128),
+                                   (18943, 8, 128), (18945, 8, 128), (5329, 3, 96)])
+def test_load_on_both_sides_of_the_block_sizes(n, H, D):
+    """Blocks of 8 rows and of 32, the larger from fewer tokens on where rows are short; the last one ends early."""
+    from sglang_b200.layers.quantization.kv_cache import load_kv_fp8
+    pages, table, indptr, slots = _paged([n // 3, 1, n - n // 3 - 1], 16)
+    kc, vc, ks, vs = _cache(pages, 16, H, D)
+    out = [torch.full((n + 40, H, D), 3.0, dtype=BF, device="cuda") for _ in range(2)]
+    load_kv_fp8(kc, vc, ks, vs, table.cuda(), indptr.cuda(), n + 40, k_out=out[0], v_out=out[1])
+    for got, cache, scale in ((out[0], kc, ks), (out[1], vc, vs)):
+        want = (cache.cpu().float().flatten(0, 1)[slots] * scale.cpu().flatten(0, 1)[slots][..., None]).to(BF)
+        assert same_bits(got[:n], want) and (got[n:] == 3.0).all()
+
+
 def test_load_of_missing_pages_reads_as_nan():
     from sglang_b200.layers.quantization.kv_cache import load_kv_fp8
     pages, table, indptr, slots = _paged([20, 9], 4)
