@@ -1039,9 +1039,13 @@ int shrink(const T* x, int64_t x_ld, const T* A, int adapters, PlanView plan, in
     return B200_OK;
   }
   if (tile_rows(tokens, adapters) == kSmallRows) {
-    // K is divided as far as all blocks can be resident, five on an SM, if it has a k32 step for each of their warps.  Two groups of
-    // columns a block, which is four on an SM, where single ones would not be divided at all, or full tiles not by eight.  Blocks of
-    // one group divided by 8 / 4 / 2, and of two by 8 / 4 / 2 (us; K = 8192, with the expand, 4 and 5 stages): 128 tokens of 32
+    // K is divided as far as five blocks for every SM go, if it has a k32 step for each of their warps.  Two groups of columns a
+    // block, and four blocks for an SM, where single ones would not be divided at all, or full tiles not by eight.  Shared memory,
+    // the static part counted, holds one block less of either kind; but the number of tiles is an estimate that errs upwards, and blocks
+    // behind a rank leave at once.  Counted with four and three instead, 81 random batches took 3.8 % longer than with the best
+    // division of each (at worst 1.56 times as long), with five and four 3.3 % (1.50); with the sums where the rings are, so that five
+    // and four fit, the blocks of most batches crowd on fewer SMs (128 tokens of 32 adapters, 3 slices of 64: 16.2 -> 18.9 us).
+    // Blocks of one group divided by 8 / 4 / 2, and of two by 8 / 4 / 2 (us; K = 8192, with the expand, 4 and 5 stages): 128 tokens of 32
     // adapters, 3 slices of 16: 18.6 15.6 17.5, 19.8 16.1 18.3; of 64 34.4 27.8 24.9, 37.2 29.6 25.5 with mixed ranks, 42.0 36.8
     // 34.8, 45.1 36.8 33.6 with rank 64 only; 200 tokens of one adapter 21.9 19.5 17.2, 19.1 14.8 19.
     const int passes = (cols + 15) / 16;
