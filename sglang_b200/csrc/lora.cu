@@ -616,16 +616,9 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const T*
       if (in && g + 8 * i < rows) hv[i] = *reinterpret_cast<const uint4*>(h0[i] + p.s * R + 32 * p.j);
     }
   };
+  static_assert(kExpandStages == 2, "one step is fetched ahead");
   fetch_weights(in_flight);
   sa::cp_async_commit();
-#pragma unroll
-  for (int i = 1; i < kExpandStages - 1; ++i) {
-    if (steps > i) {
-      advance(in_flight);
-      fetch_weights(in_flight);
-    }
-    sa::cp_async_commit();
-  }
   fetch_base(at);
   if (early) pdl_wait();
   pdl_trigger();
