@@ -293,6 +293,31 @@ def test_fused_store(T, Hq, Hkv, D, rot, neox, page, dtype):
     assert same_bits(dev[:, Hq:], qkv[:, Hq:])
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("D,neox", [(32, True), (64, False), (128, True), (256, False)])
+def test_fused_keys_get_the_correctly_rounded_quotient(D, neox, dtype):
+    """With no norm and sines of zero a key is fp32(x cos), which is known to the bit, and so are its codes and scale: also where the
+    scale's significand is all ones (largest magnitudes just below 448 times a power of two), which no 16-bit number divided by
+    448 gives and which the quotient by the reciprocal is not made for."""
+    from sglang_b200.layers.quantization.kv_cache import qk_norm_rope_store_kv_fp8
+    T, H = 64, 2
+    g = torch.Generator().manual_seed(D)
+    x = (torch.rand(T, H, D, generator=g) * 2 - 1).to(dtype)
+    x[x == 0] = 0.5
+    x[:, :, 5] = -1.0                                          # the largest magnitude of every row
+    below = torch.tensor([448.0 * 2.0 ** -e for e in range(32)])
+    cos = torch.cat([torch.nextafter(below, torch.zeros(32)), torch.rand(32, generator=g) * 3 + 0.1])
+    table = torch.cat([cos[:, None].expand(T, D // 2), torch.zeros(T, D // 2)], 1).contiguous()
+    y = x.float() * cos[:, None, None]                         # one fp32 product each, as in the kernel
+    codes, s = O.quant_group_fp8_cuda_semantics(y.reshape(T, H * D), D)
+    assert (s[:32].view(torch.int32) & 0x7fffff == 0x7fffff).all()
+    kc, vc, ks, vs = _cache(4, 16, H, D)
+    xd = x.cuda()
+    qk_norm_rope_store_kv_fp8(xd[:, :1], xd, xd.clone(), torch.arange(T).cuda(), table.cuda(), kc, vc, ks, vs, torch.arange(T).cuda(), is_neox=neox)
+    assert same_bits(ks.view(T, H), s)
+    assert torch.equal(kc.cpu().view(torch.uint8).view(T, H * D), codes.view(torch.uint8))
+
+
 def test_fused_store_of_a_position_outside_the_table_reads_as_nan():
     from sglang_b200.layers.quantization.kv_cache import load_kv_fp8, qk_norm_rope_store_kv_fp8
     qkv, (qw, kw) = _inputs(2, 4, 2, 64, BF, 11)

@@ -233,6 +233,25 @@ def test_expand_uses_nothing_behind_a_rank(T, R, L, ranks, dtype):
     _close(got, out, tol + e * out.abs() + 2.0 ** -23 * out.abs() + torch.finfo(dtype).smallest_normal * e)
 
 
+@pytest.mark.parametrize("T,R", [(3, 16), (40, 64), (300, 64)])
+def test_h_beyond_the_range_of_fp16(T, R):
+    """x A^T is rounded to x's type before it is scaled: beyond 65504 it is infinite in fp16, for its own token only; bf16 holds it."""
+    from sglang_b200.layers.lora import LoRABatch, apply_lora, lora_shrink
+    for dtype in (F16, BF):
+        x, base, A, B, ids, ranks, scal = _case(T, 512, [64], R, 1, dtype, T, ranks=[R])
+        ids[:] = 0
+        A[0, 3], x[1] = 2.0, 100.0                             # h[1, 3] = 102400
+        B.fill_(0.25)
+        scal.fill_(2.0 ** -10)
+        batch = LoRABatch(ids.cuda(), ranks.cuda(), scal.cuda())
+        h = lora_shrink(x.cuda(), A.cuda(), batch).cpu()
+        out = apply_lora(base.cuda(), x.cuda(), A.cuda(), B.cuda(), batch).cpu()
+        rest = torch.arange(T) != 1
+        assert h[rest].isfinite().all() and out[rest].isfinite().all()
+        assert h[1, 3] == (float("inf") if dtype == F16 else 102400.0)
+        assert out[1].isfinite().all() if dtype == BF else not out[1].isfinite().any()
+
+
 def test_segments_and_update():
     from sglang_b200.layers.lora import LoRABatch, apply_lora
     T, sizes = 90, [64]
