@@ -684,6 +684,12 @@ void need_out(const Tensor& t, const Tensor& like, const char* name) {
   need_writable(t, name);
 }
 
+// Tensors of the caller's that a kernel has written: autograd then knows that what it kept of them is no more.
+void wrote(std::initializer_list<const Tensor*> all) {
+  for (const Tensor* t : all)
+    if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject* wrap_or_none(Tensor t) {
   if (!t.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(t));
@@ -800,6 +806,7 @@ HOST_FN(head_rows) {
     }
   }
   if (rc != 0) return raise_status(name, rc);
+  wrote({&qo, &ko, &cache.k, &cache.v, &cache.ks, &cache.vs});
   return pair_or_none(std::move(qo), std::move(ko));
 }
 HOST_END
@@ -853,6 +860,7 @@ HOST_FN(load_kv) {
                           static_cast<int>(cache.heads), static_cast<int>(cache.dim), stream_of(dev));
   }
   if (rc != 0) return raise_status("load_kv_fp8", rc);
+  wrote({&ko, &vo});
   return pair_or_none(std::move(ko), std::move(vo));
 }
 HOST_END
@@ -884,6 +892,7 @@ HOST_FN(lora_plan) {
                         static_cast<int>(L), plan.data_ptr(), static_cast<size_t>(bytes), stream_of(dev));
   }
   if (rc != 0) return raise_status("lora_plan", rc);
+  wrote({&plan});
   return THPVariable_Wrap(std::move(plan));
 }
 HOST_END
@@ -990,6 +999,7 @@ HOST_FN(lora) {
                             base_ld, out.data_ptr(), ld_of(out), st);
   }
   if (rc != 0) return raise_status("lora", rc);
+  wrote({&out});
   return THPVariable_Wrap(B.defined() ? std::move(out) : std::move(h));
 }
 HOST_END

@@ -6,6 +6,7 @@ base_output is what the projection gave, e.g. Fp8LinearMethod.apply.  A projecti
 one low-rank product per slice: lora_a holds the slices' A one below the other, and output_sizes says which columns of the
 output belong to which.  Adapters live in buffers of a common largest rank R, lora_a [num_adapters, num_slices * R, K] and
 lora_b [num_adapters, N, R], slice s of A in rows s * R ... ; what lies behind an adapter's own rank is not used.
+No gradient passes through any of this; what is written in place counts as modified for autograd.
 
 The reference's counterparts: LoRABatchInfo, sgemm_lora_a_fwd, sgemm_lora_b_fwd, qkv_lora_b_fwd and gate_up_lora_b_fwd
 (python/sglang/srt/lora/triton_ops, lora/layers.py).

@@ -3,7 +3,8 @@
 The reference runs them one after the other: RMSNorm on q.view(-1, head_dim) and k.view(-1, head_dim)
 (python/sglang/srt/layers/layernorm.py), then RotaryEmbedding.forward on the result
 (python/sglang/srt/layers/rotary_embedding.py).  qk_norm_rope_store_kv_fp8 in layers/quantization/kv_cache.py writes the
-keys and values into a quantised cache in the same pass.
+keys and values into a quantised cache in the same pass.  No gradient passes through; what is written in place counts as
+modified for autograd.
 """
 from __future__ import annotations
 

@@ -120,3 +120,45 @@ def test_together(lens, cached, ids):
     torch.cuda.synchronize()
     for a, b in zip(eager, captured):
         assert same_bits(a, b)
+
+
+def test_what_is_written_in_place_counts_as_modified():
+    """Autograd refuses to go back through what it kept of a tensor that a call has overwritten; tensors of inference mode, which have
+    no such count, are written all the same."""
+    from sglang_b200.layers.lora import LoRABatch, apply_lora
+    from sglang_b200.layers.quantization.kv_cache import load_kv_fp8, qk_norm_rope_store_kv_fp8, store_kv_fp8
+    from sglang_b200.layers.rotary_embedding import qk_norm_rope
+    T = 3
+
+    def run():
+        ids = torch.zeros(T, dtype=torch.int32, device="cuda")
+        z = lambda *s: torch.randn(*s, device="cuda").to(BF)  # noqa: E731
+        batch = LoRABatch(ids, torch.full((1,), 8, dtype=torch.int32, device="cuda"), torch.ones(1, device="cuda"))
+        base, x, A, B, q, k, v, w = z(T, 64), z(T, 128), z(1, 8, 128), z(1, 64, 8), z(T, 2, 64), z(T, 1, 64), z(T, 1, 64), z(64)
+        caches = [torch.zeros(1, 4, 1, 64, device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
+        caches += [torch.zeros(1, 4, 1, device="cuda") for _ in range(2)]
+        slots, ko, vo = torch.arange(T, device="cuda"), z(T, 1, 64), z(T, 1, 64)
+        out = torch.empty_like(base)
+        return ((lambda: batch.update(), [batch.plan], [ids]), (lambda: apply_lora(base, x, A, B, batch), [base], [x, A, B]),
+                (lambda: apply_lora(base, x, A, B, batch, out=out), [out], [base, x]), (lambda: qk_norm_rope(q, k, None, None, w, w, q_out=q, k_out=k), [q, k], [w]),
+                (lambda: store_kv_fp8(k, v, *caches, slots), caches, [k, v, slots]),
+                (lambda: qk_norm_rope_store_kv_fp8(q, k, v, None, None, *caches, slots, w, w, q_out=q), caches + [q], [k, v]),
+                (lambda: load_kv_fp8(*caches, ids[:1, None], slots[:2].int(), T, k_out=ko, v_out=vo), [ko, vo], caches))
+    for call, written, read in run():
+        before = [t._version for t in written], [t._version for t in read]
+        call()
+        assert all(t._version > n for t, n in zip(written, before[0])) and [t._version for t in read] == before[1]
+    with torch.inference_mode():
+        calls = run()
+    for call, _, _ in calls:
+        call()
+    leaf = torch.randn(T, 64, device="cuda", dtype=BF, requires_grad=True)
+    base = leaf * 1
+    kept = base.exp().sum() + (base * base).sum()
+    ids = torch.zeros(T, dtype=torch.int32, device="cuda")
+    batch = LoRABatch(ids, torch.full((1,), 8, dtype=torch.int32, device="cuda"), torch.ones(1, device="cuda"))
+    with torch.no_grad():
+        apply_lora(base, torch.ones(T, 128, device="cuda", dtype=BF), torch.ones(1, 8, 128, device="cuda", dtype=BF),
+                   torch.ones(1, 64, 8, device="cuda", dtype=BF), batch)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
