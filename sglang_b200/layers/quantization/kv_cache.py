@@ -5,8 +5,10 @@
 
 Any page, token and head strides (multiples of 16 elements in the codes), so a pool with another order of dimensions is passed
 as a permuted view.  Slot s is place s % page_size of page s // page_size.  The codes and scales of a token are those that
-sglang_per_token_group_quant_fp8 with group_size = head_dim gives.  No gradient passes through; what is written counts as
-modified for autograd.
+sglang_per_token_group_quant_fp8 with group_size = head_dim gives, special values included: a NaN does not count for the scale and
+gets the code of -448, so that it reads back as minus the head's largest finite magnitude (a head of NaN alone as -1e-10); an
+infinity makes the scale infinite and reads back as minus infinity, the rest of its head as NaN.  No gradient passes through;
+what is written counts as modified for autograd.
 
 The reference keeps FP8 keys and values with one scale for the whole layer (python/sglang/srt/layers/quantization/kv_cache.py,
 MHATokenToKVPool.set_kv_buffer in python/sglang/srt/mem_cache/memory_pool.py); a scale for each token and head needs no

@@ -241,6 +241,22 @@ def test_store_special_values_as_the_group_quantiser():
         assert same_bits(scale.view(8, 2), s)
 
 
+def test_what_special_values_read_back_as():
+    from sglang_b200.layers.quantization.kv_cache import load_kv_fp8, store_kv_fp8
+    x = torch.ones(4, 1, 32, dtype=BF)
+    x[0, 0, 3], x[0, 0, 4], x[1, 0, 5], x[2, 0, 6] = float("nan"), -3.5, float("inf"), float("-inf")
+    x[3] = float("nan")
+    cache = _cache(1, 4, 1, 32)
+    store_kv_fp8(x.cuda(), x.cuda(), *cache, torch.arange(4).cuda())
+    k, v = load_kv_fp8(*cache, torch.zeros(1, 1).int().cuda(), torch.tensor([0, 4]).int().cuda(), 4)
+    for out in (k.cpu()[:, 0], v.cpu()[:, 0]):
+        assert out[0, 3] == -3.5 and out[0, 4] == -3.5 and (out[0, 5:] == 1).all()
+        for t, d in ((1, 5), (2, 6)):
+            rest = torch.arange(32) != d
+            assert out[t, d] == float("-inf") and out[t, rest].isnan().all()
+        assert (out[3] == torch.tensor(-1e-10).to(BF)).all()
+
+
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("T,Hq,Hkv,D,rot,neox,page", [(1, 64, 8, 128, 128, True, 64), (1, 1, 1, 32, 16, False, 1),
                                                       (30, 10, 2, 96, 48, True, 5), (64, 8, 8, 64, 64, False, 16),
