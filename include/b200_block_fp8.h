@@ -606,7 +606,8 @@ int b200_qk_norm_rope(const b200_heads* q, const b200_heads* k, const b200_heads
  * Keys and values of num_tokens tokens quantised into the cache: scale = max(1e-10, max|y|) / 448 for each token and head,
  * code = e4m3(y / scale) -- bit for bit what b200_per_token_group_quant_fp8 with group = head_dim makes of them.  Token t goes
  * to slot slots[t] (int32, or int64 with slots_i64); a slot outside [0, num_pages * page_size) is skipped.  Tokens of one call
- * that share a slot leave it undefined.  Every other slot stays as it was.
+ * that share a slot leave it undefined.  Every other slot stays as it was.  A NaN counts as -448 times the scale of the head's other
+ * elements, an infinity makes the scale infinite, as in that quantiser.
  */
 int b200_store_kv_fp8(const b200_heads* k, const b200_heads* v, int dtype, const b200_kv_cache* cache, const void* slots,
                       int slots_i64, int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
@@ -627,7 +628,7 @@ int b200_qk_norm_rope_store_kv_fp8(const b200_heads* q, const b200_heads* k, con
  * Rows [indptr[b], indptr[b + 1]) are the tokens starts[b], starts[b] + 1, ... of sequence b (starts NULL: from 0), token i
  * lying at place i % page_size of page page_table[b * page_table_stride + i / page_size].  indptr [batch + 1] does not
  * decrease; rows of the `num_tokens` outside [indptr[0], indptr[batch]) are left as they were.  A row whose page is missing
- * (outside the table, or no page of the cache) becomes NaN.
+ * (outside the table, or no page of the cache) becomes NaN; page_table may be NULL when it has no columns.
  */
 int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_table, int64_t page_table_stride,
                      int64_t page_table_cols, const int32_t* indptr, const int32_t* starts, int64_t batch,
@@ -643,7 +644,8 @@ int b200_load_kv_fp8(const b200_kv_cache* cache, const int32_t* page_table, int6
  * Stands in for the sgemm_lora_a / sgemm_lora_b / qkv_lora_b / gate_up_lora_b kernels of python/sglang/srt/lora/triton_ops.
  *
  * b200_lora_plan groups the tokens by adapter into `plan` (16-byte aligned device memory of b200_lora_plan_bytes); shrink and
- * expand take it, with the same num_tokens and L.  It has to be made again when ids or ranks change.
+ * expand take it, with the same num_tokens and L.  It has to be made again when ids or ranks change.  L also chooses the kernels:
+ * tiles of 128 tokens from 256 tokens and 24 for each of the L adapters on, whether or not all of them are in use, else of 16.
  * b200_lora_shrink writes h [num_tokens, num_slices * R] in x's type (fp32 sums, rounded once; zero behind a rank, and for
  * tokens without an adapter).  b200_lora_expand: base NULL counts as zeros; out may be base; tokens without an adapter get
  * base.  slice_sizes (host) adds up to N, each a multiple of 8.  dtype (of x, A, h, B, base, out) bf16 or fp16; K and R

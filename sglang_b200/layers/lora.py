@@ -26,7 +26,10 @@ class LoRABatch:
 
     token_adapters  int32 [num_tokens]: index into the adapter buffers; anything outside them (-1) means none
     lora_ranks      int32 [num_adapters]: each adapter's rank; 0 means that the buffer is empty
-    scalings        fp32 [num_adapters]"""
+    scalings        fp32 [num_adapters]
+
+    The kernels are chosen by the numbers of tokens and of adapter buffers, in use or not: 8191 tokens of one adapter (K = 8192,
+    N = 10240, rank 64) take 111 us with 8 buffers and 321 with 512, where they count as a small batch."""
 
     def __init__(self, token_adapters: torch.Tensor, lora_ranks: torch.Tensor, scalings: torch.Tensor) -> None:
         self.token_adapters, self.lora_ranks, self.scalings = token_adapters, lora_ranks, scalings
