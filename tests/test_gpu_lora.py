@@ -271,6 +271,30 @@ def test_segments_and_update():
     _close(out, want, tol)
 
 
+@pytest.mark.parametrize("T,live", [(90, 57), (90, 0), (90, 200), (600, 411)])
+def test_a_padded_batch_of_segments(T, live):
+    """Requests that hold fewer tokens than the batch, or more: also planned and run in a graph, for the lengths at its replay."""
+    from sglang_b200.layers.lora import LoRABatch, apply_lora
+    x, base, A, B, _, ranks, scal = _case(T, 64, [64], 16, 3, F16, 9)
+    which, lens = torch.tensor([2, 1, -1, 0]), torch.tensor([live // 2, live // 5, live // 5, live - live // 2 - 2 * (live // 5)])
+    ids = torch.full((T + live,), -1, dtype=torch.int32)
+    ids[:live] = torch.repeat_interleave(which, lens).int()
+    ids = ids[:T]
+    _, want, _, tol = _exact(x, base, A, B, ids, ranks, scal, [64])
+    xd, bd, Ad, Bd, rd, sd, wd, ld = (t.cuda() for t in (x, base, A, B, ranks, scal, which, lens))
+    out = apply_lora(bd, xd, Ad, Bd, LoRABatch.from_segments(wd, ld, T, rd, sd), out=torch.empty_like(bd))
+    _close(out, want, tol)
+    assert same_bits(out[ids < 0], base[ids < 0])
+    later, got = torch.zeros_like(ld), torch.empty_like(bd)
+    LoRABatch.from_segments(wd, later, T, rd, sd)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        apply_lora(bd, xd, Ad, Bd, LoRABatch.from_segments(wd, later, T, rd, sd), out=got)
+    later.copy_(ld)
+    g.replay()
+    assert same_bits(got, out)
+
+
 @pytest.mark.parametrize("T,R", [(5, 16), (5, 32), (260, 32), (600, 32)])
 def test_captured_and_replayed_on_a_side_stream(T, R):
     """Planning, shrink and expand in one graph; new tokens and ids are copied in before each replay.  Two graphs share nothing
