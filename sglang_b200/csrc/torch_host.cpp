@@ -619,21 +619,35 @@ bool same_view(const Tensor& t, const Tensor& u) {
   return true;
 }
 // What a call writes must lie in places of its own: not overlap itself, nor, unless it is `in_place`, anything else that the call has.
+// Nearly always the ranges of addresses settle it; only where two meet are the bytes looked at.
 struct Held {
   Held(const Tensor& t, const char* name) : t(t), name(name), any(t.defined() && t.numel() > 0) {
-    if (any) b = bytes_of(t);
+    if (!any) return;
+    dense = t.is_non_overlapping_and_dense();
+    lo = static_cast<const char*>(t.const_data_ptr());
+    int64_t last = t.numel() - 1;
+    if (!dense) {
+      last = 0;
+      for (int d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    }
+    hi = lo + (last + 1) * static_cast<int64_t>(t.element_size());
   }
   const Tensor& t;
   const char* name;
-  bool any;
-  Bytes b;
+  bool any, dense = false;
+  const char *lo = nullptr, *hi = nullptr;
 };
 void need_own_memory(const Held& out, const Held* in_place, at::ArrayRef<Held> all) {
   if (!out.any) return;
-  for (int d = 0; d < out.b.n; ++d) NEED(out.b.step[d] >= out.b.span[d + 1], std::string(out.name) + " must not overlap itself");
-  for (const Held& o : all)
-    NEED(!o.any || &o == &out || !meet(out.b, 0, o.b, 0, o.b.at - out.b.at) || (&o == in_place && same_view(out.t, o.t)),
+  if (!out.dense) {
+    const Bytes b = bytes_of(out.t);
+    for (int d = 0; d < b.n; ++d) NEED(b.step[d] >= b.span[d + 1], std::string(out.name) + " must not overlap itself");
+  }
+  for (const Held& o : all) {
+    if (!o.any || &o == &out || out.hi <= o.lo || o.hi <= out.lo) continue;
+    NEED((&o == in_place && same_view(out.t, o.t)) || !share_memory(out.t, o.t),
          std::string(out.name) + " must share no memory with " + o.name + (&o == in_place ? " or be it" : ""));
+  }
 }
 b200_heads heads_of(const Tensor& t) { return {t.data_ptr(), stride_of(t, 0), stride_of(t, 1)}; }
 
