@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kMaxThreads, 11) store_rows_kernel(const __gri
   }
 }
 
-// Eleven blocks of two warps: 80 registers, and the rotating kinds spill (96 bytes stored, 52 loaded a thread, before the rows begin).
+// Eleven blocks of two warps: 80 registers, and the rotating kinds spill (up to 96 bytes stored and 52 loaded a thread).
 // With ten nothing spills (95 registers) and there are two warps fewer: 54.3 -> 57.7 us for 8192 tokens of 64 + 8 + 8 heads of 128,
 // 27.4 -> 29.0 for 8192 of 32 + 4 with pairs rotated, 16.9 -> 17.7 for 2048; only a batch of 64 gains, 2.9 -> 2.7.
 template <typename T, int G, int KIND>
